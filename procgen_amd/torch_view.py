@@ -18,7 +18,7 @@ A handle is G device shards x K games parts (include/procgen_amd.h): part p hold
 ``first_env + i * env_stride``; ``global_indices()`` gives them, ``scatter_observations`` assembles one [N, 64, 64, 3]
 tensor on a chosen device for callers that want the gym3 layout (that one copies, by definition).
 
-PyTorch is plumbing here: this module is the only file of the package that imports it, and only when called.
+PyTorch is plumbing here: this module imports it only when called; learner_ops.py, the operators on these tensors, imports it when it is imported.
 """
 import ctypes as C
 
@@ -105,3 +105,62 @@ def scatter_observations(env, device=None, out=None):
         idx = torch.as_tensor(v.global_indices(), device=dev)
         out.index_copy_(0, idx, v.ob.to(dev, non_blocking=True))
     return out
+
+
+class Rollout:
+    """A window of `steps` steps of every env of the handle, kept on the GPU in global env order: what learner_ops takes its rewards, episode starts
+    and actions from.
+
+        window = Rollout(env, steps=256)
+        env.observe(); window.record()                            # the observation that the window begins with
+        for _ in range(256):
+            env.act(actions); env.observe(); window.record()
+        adv, ret = window.advantages(values, gamma=0.999, lam=0.95)   # values [steps + 1, N]: the value head on observations 0 .. steps
+        window.restart()                                          # the last observation is the first of the next window
+
+    rew float32 [steps, N] and action int32 [steps, N]: of the acts; first uint8 [steps + 1, N]: of the observations.  record() copies the part arrays
+    and waits for the copies, since the next act overwrites them."""
+
+    def __init__(self, env, steps, device=None):
+        import torch
+
+        if steps < 1:
+            raise ValueError(f"a window has one step at least, not {steps}")
+        self._views = device_views(env)
+        self.steps, self.recorded = steps, 0
+        self.device = torch.device(device) if device is not None else torch.device("cuda", self._views[0].device_id)
+        self.rew = torch.zeros((steps, env.num), dtype=torch.float32, device=self.device)
+        self.first = torch.zeros((steps + 1, env.num), dtype=torch.uint8, device=self.device)
+        self.action = torch.zeros((steps, env.num), dtype=torch.int32, device=self.device)
+
+    def record(self):
+        """takes the step that the last env.observe() ended into the window"""
+        import torch
+
+        k = self.recorded
+        if k > self.steps:
+            raise ValueError(f"the window of {self.steps} steps is full: restart() it")
+        for v in self._views:
+            mine = slice(v.first_env, v.first_env + v.env_stride * v.num_envs, v.env_stride)
+            self.first[k, mine].copy_(v.first, non_blocking=True)
+            if k:
+                self.rew[k - 1, mine].copy_(v.rew, non_blocking=True)
+                self.action[k - 1, mine].copy_(v.action, non_blocking=True)
+        for d in {self.device, *(torch.device("cuda", v.device_id) for v in self._views)}:
+            torch.cuda.current_stream(d).synchronize()
+        self.recorded += 1
+
+    def restart(self):
+        """begins the next window with the observation that this one ended with"""
+        if self.recorded <= self.steps:
+            raise ValueError(f"{self.recorded} of the window's {self.steps + 1} observations are recorded")
+        self.first[0].copy_(self.first[-1])
+        self.recorded = 1
+
+    def advantages(self, values, *, gamma, lam):
+        """(adv, ret) float32 [steps, N] of the full window: learner_ops.advantages of its rewards and episode starts"""
+        from . import learner_ops
+
+        if self.recorded <= self.steps:
+            raise ValueError(f"{self.recorded} of the window's {self.steps + 1} observations are recorded")
+        return learner_ops.advantages(self.rew, values, self.first, gamma=gamma, lam=lam)
