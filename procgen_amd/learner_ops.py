@@ -133,19 +133,21 @@ def _ptr(x):
 # ---- the memory of a policy ------------------------------------------------------------------------------------------------------------------
 
 
-def _recurrence_args(gate, update, h, first, state):
+def _recurrence_args(gate, update, first, state, checkpoints):
     T, N, D = gate.shape
-    a = _Recurrence(dtype=_DTYPES[gate.dtype], T=T, N=N, D=D, gate=_array3(gate), update=_array3(update), h=_array3(h), state=_ptr(state))
+    a = _Recurrence(dtype=_DTYPES[gate.dtype], T=T, N=N, D=D, gate=_array3(gate), update=_array3(update), state=_ptr(state), checkpoints=_ptr(checkpoints))
     if first is not None:
         a.first, a.first_t_stride, a.first_n_stride = first.data_ptr(), first.stride(0), first.stride(1)
-    return a
+    work = _bytes(_lib.recurrence_workspace(T, N, D), gate.device)
+    a.workspace = _ptr(work)
+    return a, work
 
 
-def _recurrence_forward(gate, update, first, state, state_out):
+def _recurrence_forward(gate, update, first, state, state_out, checkpoints=None):
     h = torch.empty_like(update)
     last = state_out if state_out is not None else torch.empty(gate.shape[1:], dtype=torch.float32, device=gate.device)
-    a = _recurrence_args(gate, update, h, first, state)
-    a.state_out = last.data_ptr()
+    a, work = _recurrence_args(gate, update, first, state, checkpoints)
+    a.h, a.state_out = _array3(h), last.data_ptr()
     _run(_lib.recurrence_forward, "gated_recurrence", gate.device, C.addressof(a))
     return h, last
 
@@ -153,15 +155,16 @@ def _recurrence_forward(gate, update, first, state, state_out):
 class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, update, first, state):
-        h, last = _recurrence_forward(gate, update, first, state, None)
-        ctx.save_for_backward(gate, update, h, first, state)
+        checkpoints = torch.empty((_lib.recurrence_checkpoints(gate.shape[0]), *gate.shape[1:]), dtype=torch.float32, device=gate.device)
+        h, last = _recurrence_forward(gate, update, first, state, None, checkpoints)
+        ctx.save_for_backward(gate, update, first, state, checkpoints)
         return h, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_h, d_last):
-        gate, update, h, first, state = ctx.saved_tensors
-        a = _recurrence_args(gate, update, h, first, state)
+        gate, update, first, state, checkpoints = ctx.saved_tensors
+        a, work = _recurrence_args(gate, update, first, state, checkpoints)
         d_gate = d_update = d_state = None
         if d_h is not None:
             a.d_h = _array3(d_h)
@@ -252,6 +255,8 @@ def advantages(rew, values, first, *, gamma, lam):
     if T and N:
         a = _Advantage(_DTYPES[values.dtype], T, N, rew.data_ptr(), *rew.stride(), values.data_ptr(), *values.stride(), first.data_ptr(), *first.stride(),
                        gamma, lam, adv.data_ptr(), ret.data_ptr(), None)
+        work = _bytes(_lib.recurrence_workspace(T, N, 1), device)
+        a.workspace = _ptr(work)
         _run(_lib.advantages, "advantages", device, C.addressof(a))
     return adv, ret
 
