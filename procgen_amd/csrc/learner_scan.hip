@@ -19,34 +19,13 @@ namespace {
 
 constexpr int K = 8, MAX_W = 8, TILE = K * MAX_W;
 
-// the element types' rows of VEC neighbouring channels; `count` of them exist (the last lane of an env may hold fewer)
+// VEC neighbouring channels of a step, as memory holds them.  Loads are unconditional (addresses are clamped into the arrays and values selected
+// afterwards): a load behind a branch of its own would be waited for before the next is issued.
 template <class E, int VEC>
-struct Row {
-    float x[VEC];
+struct Raw {
+    typename E::T x[VEC];
+    __device__ void load(const typename E::T *p) { __builtin_memcpy(x, p, sizeof x); }  // one wide load, whatever the alignment
 };
-template <class E, int VEC>
-__device__ inline Row<E, VEC> load_row(const typename E::T *p, int count) {
-    Row<E, VEC> r;
-    typename E::T raw[VEC];
-    if (count == VEC) {
-        __builtin_memcpy(raw, p, sizeof raw);  // one wide load, whatever the alignment
-    } else {
-        for (int v = 0; v < VEC; v++) raw[v] = v < count ? p[v] : (typename E::T)0.f;
-    }
-    for (int v = 0; v < VEC; v++) r.x[v] = (float)raw[v];
-    return r;
-}
-template <class E, int VEC>
-__device__ inline void store_row(typename E::T *p, int count, const Row<E, VEC> &r) {
-    typename E::T raw[VEC];
-    for (int v = 0; v < VEC; v++) raw[v] = (typename E::T)r.x[v];
-    if (count == VEC) {
-        __builtin_memcpy(p, raw, sizeof raw);
-    } else {
-        for (int v = 0; v < VEC; v++)
-            if (v < count) p[v] = raw[v];
-    }
-}
 
 template <int VEC>
 struct Map {
@@ -69,32 +48,41 @@ struct Map {
 // the pieces' maps of a tile, by wave and lane
 template <int VEC>
 struct Pieces {
-    float A[MAX_W][VEC][WAVE], B[MAX_W][VEC][WAVE];
+    struct alignas(4 * VEC) Vec {
+        float x[VEC];
+    };
+    Vec A[MAX_W][WAVE], B[MAX_W][WAVE];
     int cut[MAX_W][WAVE];
     __device__ void put(int w, int lane, const Map<VEC> &m) {
-        for (int v = 0; v < VEC; v++) A[w][v][lane] = m.A[v], B[w][v][lane] = m.B[v];
+        Vec a, b;
+        for (int v = 0; v < VEC; v++) a.x[v] = m.A[v], b.x[v] = m.B[v];
+        A[w][lane] = a, B[w][lane] = b;
         cut[w][lane] = m.cut;
     }
     __device__ Map<VEC> get(int w, int lane) const {
         Map<VEC> m;
-        for (int v = 0; v < VEC; v++) m.A[v] = A[w][v][lane], m.B[v] = B[w][v][lane];
+        const Vec a = A[w][lane], b = B[w][lane];
+        for (int v = 0; v < VEC; v++) m.A[v] = a.x[v], m.B[v] = b.x[v];
         m.cut = cut[w][lane];
         return m;
     }
 };
 
-// where a lane's chains are: env n, channels d .. d + count - 1
+// where a lane's chains are: env n, channels d .. d + VEC - 1.  The last lane of an env reaches back over its neighbour's channels where VEC does not
+// divide D, and writes only those from `skip` on; lanes behind the last chain double the last one and write nothing (skip = VEC).
 template <int VEC>
 struct Chain {
-    int n, d, count;
+    int n, d, skip;
     long long c;  // index of the first one in [N][D]
-    __device__ Chain(long long unit, int N, int D) {
-        const int lanes = (D + VEC - 1) / VEC;
-        n = (int)(unit / lanes);
-        d = (int)(unit - (long long)n * lanes) * VEC;
-        count = n < N ? min(VEC, D - d) : 0;
+    __device__ Chain(unsigned unit, int N, int D) {
+        const unsigned lanes = ((unsigned)D + VEC - 1) / VEC, units = (unsigned)N * lanes, u = min(unit, units - 1);
+        n = (int)(u / lanes);
+        const int wanted = (int)(u - (unsigned)n * lanes) * VEC;
+        d = min(wanted, D - VEC);
+        skip = unit < units ? wanted - d : VEC;
         c = (long long)n * D + d;
     }
+    __device__ bool mine(int v) const { return v >= skip; }
 };
 
 // segments of a window: `tiles` tiles each, maps[segment][A, B][chain], cuts[segment][chain], and a copy of the state that the window begins in
@@ -108,7 +96,7 @@ struct Segments {
 template <int VEC>
 __device__ inline void put_segment(const Segments &g, int s, long long chains, const Chain<VEC> &ch, const Map<VEC> &m) {
     for (int v = 0; v < VEC; v++)
-        if (v < ch.count) {
+        if (ch.mine(v)) {
             g.maps[g.at(s, 0, chains, ch.c + v)] = m.A[v];
             g.maps[g.at(s, 1, chains, ch.c + v)] = m.B[v];
             g.cuts[s * chains + ch.c + v] = m.cut;
@@ -117,13 +105,8 @@ __device__ inline void put_segment(const Segments &g, int s, long long chains, c
 template <int VEC>
 __device__ inline Map<VEC> get_segment(const Segments &g, int s, long long chains, const Chain<VEC> &ch) {
     Map<VEC> m;
-    m.identity();
-    for (int v = 0; v < VEC; v++)
-        if (v < ch.count) {
-            m.A[v] = g.maps[g.at(s, 0, chains, ch.c + v)];
-            m.B[v] = g.maps[g.at(s, 1, chains, ch.c + v)];
-        }
-    if (ch.count) m.cut = g.cuts[s * chains + ch.c];
+    for (int v = 0; v < VEC; v++) m.A[v] = g.maps[g.at(s, 0, chains, ch.c + v)], m.B[v] = g.maps[g.at(s, 1, chains, ch.c + v)];
+    m.cut = g.cuts[s * chains + ch.c];
     return m;
 }
 
@@ -143,102 +126,150 @@ __device__ inline void run_segments(float *x, const Segments &g, int from, int t
     __syncthreads();
 }
 
+// a lane's view of one array: the rows of its channels
 template <class E, int VEC>
-struct Recurrence {  // a lane's view of the arrays
-    const procgen_amd_recurrence &p;
-    const Chain<VEC> ch;
-    const uint8_t *first;
-    __device__ Recurrence(const procgen_amd_recurrence &args, long long unit)
-        : p(args), ch(unit, args.N, args.D), first(args.first ? args.first + ch.n * args.first_n_stride : nullptr) {}
-    __device__ typename E::T *at(const procgen_amd_array3 &a, int t) const {
-        return (typename E::T *)a.data + t * a.t_stride + ch.n * a.n_stride + ch.d * a.d_stride;
+struct Column {
+    typename E::T *base;
+    long long stride;
+    __device__ Column(const procgen_amd_array3 &a, const Chain<VEC> &ch) : base((typename E::T *)a.data + ch.n * a.n_stride + ch.d * a.d_stride), stride(a.t_stride) {}
+    __device__ void load(Raw<E, VEC> *to, int t, int last) const {  // steps t .. t + K - 1, none behind `last`
+#pragma unroll
+        for (int k = 0; k < K; k++) to[k].load(base + min(t + k, last) * stride);
     }
-    __device__ Row<E, VEC> load(const procgen_amd_array3 &a, int t, bool real, float otherwise) const {
-        if (real) return load_row<E, VEC>(at(a, t), ch.count);
-        Row<E, VEC> r;
-        for (int v = 0; v < VEC; v++) r.x[v] = otherwise;
-        return r;
+    __device__ void store(int t, const float *x, const Chain<VEC> &ch) const {
+        typename E::T raw[VEC], *p = base + t * stride;
+        for (int v = 0; v < VEC; v++) raw[v] = (typename E::T)x[v];
+        if (ch.skip == 0) {
+            __builtin_memcpy(p, raw, sizeof raw);
+        } else {
+            for (int v = 0; v < VEC; v++)
+                if (ch.mine(v)) p[v] = raw[v];
+        }
     }
-    __device__ bool cut(int t, bool real) const { return real && first && first[t * p.first_t_stride]; }
+};
+// the flags of a lane's env; without any, some bytes of the gates are read and masked
+struct Flags {
+    const uint8_t *base;
+    long long stride;
+    uint8_t mask;
+    __device__ Flags(const uint8_t *first, long long t_stride, long long n_stride, int n, const void *otherwise)
+        : base(first ? first + n * n_stride : (const uint8_t *)otherwise), stride(first ? t_stride : 0), mask(first ? 0xff : 0) {}
+    __device__ void load(uint8_t *to, int t, int last) const {
+#pragma unroll
+        for (int k = 0; k < K; k++) to[k] = base[min(t + k, last) * stride];
+    }
 };
 
-// K steps of a wave, t .. t + K - 1 (those at `end` and behind it are the identity)
-template <class E, int VEC, bool REVERSE>
-__device__ inline Map<VEC> compose(const Row<E, VEC> *a, const Row<E, VEC> *b, const bool *cut) {
+template <int VEC>
+__device__ inline void load_state(float *x, const float *state, const Chain<VEC> &ch) {
+    for (int v = 0; v < VEC; v++) x[v] = state ? state[ch.c + v] : 0.f;
+}
+template <int VEC>
+__device__ inline void store_state(float *state, const float *x, const Chain<VEC> &ch) {
+    for (int v = 0; v < VEC; v++)
+        if (ch.mine(v)) state[ch.c + v] = x[v];
+}
+
+// the composition of K steps: x -> gate x + update forwards; backwards the gradient y of a step's h from behind it becomes gate (d + y) before it
+template <int VEC, bool REVERSE>
+__device__ inline Map<VEC> compose(const float (*a)[VEC], const float (*b)[VEC], const bool *cut) {
     Map<VEC> m;
     m.identity();
+#pragma unroll
     for (int i = 0; i < K; i++) {
         const int k = REVERSE ? K - 1 - i : i;
         for (int v = 0; v < VEC; v++) {
-            // backwards a step takes the gradient y of its h from behind to a (d + y) before it
-            m.B[v] = REVERSE ? (cut[k] ? 0.f : a[k].x[v] * (b[k].x[v] + m.B[v])) : (cut[k] ? b[k].x[v] : fmaf(a[k].x[v], m.B[v], b[k].x[v]));
-            m.A[v] *= a[k].x[v];
+            m.B[v] = REVERSE ? (cut[k] ? 0.f : a[k][v] * (b[k][v] + m.B[v])) : (cut[k] ? b[k][v] : fmaf(a[k][v], m.B[v], b[k][v]));
+            m.A[v] *= a[k][v];
         }
         m.cut = m.cut || cut[k];
     }
     return m;
+}
+// K loaded steps in 32 bits; those at `end` and behind it become the identity
+template <class E, int VEC>
+__device__ inline void convert(float (*x)[VEC], const Raw<E, VEC> *raw, int t, int end, float otherwise) {
+#pragma unroll
+    for (int k = 0; k < K; k++)
+        for (int v = 0; v < VEC; v++) x[k][v] = t + k < end ? (float)raw[k].x[v] : otherwise;
+}
+__device__ inline void convert(bool *cut, const uint8_t *raw, uint8_t mask, int t, int end) {
+#pragma unroll
+    for (int k = 0; k < K; k++) cut[k] = t + k < end && (raw[k] & mask);
 }
 
 // the map of every segment (blockIdx.y): forwards of gate and update, backwards of gate and d_h.  The waves take a part of the segment each.
 template <class E, int VEC, bool REVERSE>
 __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_segments(procgen_amd_recurrence p, Segments g) {
     __shared__ Pieces<VEC> pieces;
-    const int lane = threadIdx.x, w = threadIdx.y, W = blockDim.y, s = blockIdx.y;
-    const Recurrence<E, VEC> r(p, (long long)blockIdx.x * WAVE + lane);
+    const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
+    const Chain<VEC> ch(blockIdx.x * WAVE + lane, p.N, p.D);
     const long long chains = (long long)p.N * p.D;
     const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE);
     const int part = (g.tiles * TILE + W * K - 1) / (W * K) * K;  // steps of a wave
-    const int from = begin + w * part, to = min(end, from + part);
+    const int from = min((long long)end, (long long)begin + (long long)w * part), to = min((long long)end, (long long)from + part);
+    const bool any = !REVERSE || p.d_h.data;
+    const Column<E, VEC> gate(p.gate, ch), other(REVERSE ? (any ? p.d_h : p.gate) : p.update, ch);
+    const Flags first(p.first, p.first_t_stride, p.first_n_stride, ch.n, gate.base);
     Map<VEC> m;
     m.identity();
-    for (int i = 0; i < part; i += K) {
-        const int t = REVERSE ? from + part - K - i : from + i;
-        Row<E, VEC> a[K], b[K];
+    for (int i = 0; i < to - from; i += K) {
+        const int t = REVERSE ? from + (to - from - 1) / K * K - i : from + i;
+        Raw<E, VEC> ra[K], rb[K];
+        uint8_t rf[K];
+        gate.load(ra, t, end - 1);
+        other.load(rb, t, end - 1);
+        first.load(rf, t, end - 1);
+        float a[K][VEC], b[K][VEC];
         bool cut[K];
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            const bool real = r.ch.count && t + k < to;
-            a[k] = r.load(p.gate, t + k, real, 1.f);
-            b[k] = r.load(REVERSE ? p.d_h : p.update, t + k, real && (!REVERSE || p.d_h.data), 0.f);
-            cut[k] = r.cut(t + k, real);
-        }
-        m.then(compose<E, VEC, REVERSE>(a, b, cut));
+        convert<E, VEC>(a, ra, t, to, 1.f);
+        convert<E, VEC>(b, rb, t, any ? to : 0, 0.f);
+        convert(cut, rf, first.mask, t, to);
+        m.then(compose<VEC, REVERSE>(a, b, cut));
     }
     pieces.put(w, lane, m);
     __syncthreads();
     if (w) return;
     m.identity();
     for (int k = 0; k < W; k++) m.then(pieces.get(REVERSE ? W - 1 - k : k, lane));
-    put_segment<VEC>(g, s, chains, r.ch, m);
-    if (!REVERSE && s == 0 && p.state)
-        for (int v = 0; v < r.ch.count; v++) g.state[r.ch.c + v] = p.state[r.ch.c + v];
+    put_segment<VEC>(g, s, chains, ch, m);
+    if (!REVERSE && s == 0 && p.state) {
+        float x[VEC];
+        load_state<VEC>(x, p.state, ch);
+        store_state<VEC>(g.state, x, ch);
+    }
 }
 
 template <class E, int VEC>
 __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_forward(procgen_amd_recurrence p, Segments g) {
     __shared__ Pieces<VEC> pieces[2];
-    const int lane = threadIdx.x, w = threadIdx.y, W = blockDim.y, s = blockIdx.y;
-    const Recurrence<E, VEC> r(p, (long long)blockIdx.x * WAVE + lane);
+    const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
+    const Chain<VEC> ch(blockIdx.x * WAVE + lane, p.N, p.D);
     const long long chains = (long long)p.N * p.D;
+    const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE), last = end - 1;
+    const Column<E, VEC> gate(p.gate, ch), update(p.update, ch), out(p.h, ch);
+    const Flags first(p.first, p.first_t_stride, p.first_n_stride, ch.n, gate.base);
+    Raw<E, VEC> ra[K], rb[K];
+    uint8_t rf[K];
+    auto load = [&](int t) {
+        gate.load(ra, t, last);
+        update.load(rb, t, last);
+        first.load(rf, t, last);
+    };
+    load(begin + w * K);
     float x[VEC];
-    for (int v = 0; v < VEC; v++) x[v] = p.state && v < r.ch.count ? (g.count > 1 ? g.state : p.state)[r.ch.c + v] : 0.f;
-    if (s) run_segments<VEC>(x, g, 0, s, chains, r.ch, pieces[0], w, W, lane);
-    const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE);
+    load_state<VEC>(x, p.state && g.count > 1 ? g.state : p.state, ch);
+    if (s) run_segments<VEC>(x, g, 0, s, chains, ch, pieces[0], w, W, lane);
     for (int t0 = begin, odd = 0; t0 < end; t0 += TILE, odd ^= 1) {
         const int t = t0 + w * K;
-        Row<E, VEC> a[K], b[K];
+        float a[K][VEC], b[K][VEC];
         bool cut[K];
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            const bool real = r.ch.count && t + k < end;
-            a[k] = r.load(p.gate, t + k, real, 1.f);
-            b[k] = r.load(p.update, t + k, real, 0.f);
-            cut[k] = r.cut(t + k, real);
-        }
-        if (p.checkpoints && w == 0)
-            for (int v = 0; v < VEC; v++)
-                if (v < r.ch.count) p.checkpoints[(long long)(t0 / TILE) * chains + r.ch.c + v] = x[v];
-        pieces[odd].put(w, lane, compose<E, VEC, false>(a, b, cut));
+        convert<E, VEC>(a, ra, t, end, 1.f);
+        convert<E, VEC>(b, rb, t, end, 0.f);
+        convert(cut, rf, first.mask, t, end);
+        if (t0 + TILE < end) load(t + TILE);  // the next tile is on its way while this one is joined
+        if (p.checkpoints && w == 0) store_state<VEC>(p.checkpoints + (long long)(t0 / TILE) * chains, x, ch);
+        pieces[odd].put(w, lane, compose<VEC, false>(a, b, cut));
         __syncthreads();
         float y[VEC];
         for (int v = 0; v < VEC; v++) y[v] = x[v];
@@ -251,14 +282,11 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_forward(procgen_amd_re
         }
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            Row<E, VEC> h;
-            for (int v = 0; v < VEC; v++) h.x[v] = y[v] = cut[k] ? b[k].x[v] : fmaf(a[k].x[v], y[v], b[k].x[v]);
-            if (r.ch.count && t + k < end) store_row<E, VEC>(r.at(p.h, t + k), r.ch.count, h);
+            for (int v = 0; v < VEC; v++) y[v] = cut[k] ? b[k][v] : fmaf(a[k][v], y[v], b[k][v]);
+            if (t + k < end) out.store(t + k, y, ch);
         }
     }
-    if (p.state_out && w == 0 && s == g.count - 1)
-        for (int v = 0; v < VEC; v++)
-            if (v < r.ch.count) p.state_out[r.ch.c + v] = x[v];
+    if (p.state_out && w == 0 && s == g.count - 1) store_state<VEC>(p.state_out, x, ch);
 }
 
 // Backwards over the tiles.  h is not read: its 32-bit value before every step comes from the checkpoint at the tile's start and the same joins as in
@@ -266,29 +294,41 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_forward(procgen_amd_re
 template <class E, int VEC>
 __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_backward(procgen_amd_recurrence p, Segments g) {
     __shared__ Pieces<VEC> fore[2], back[2];
-    const int lane = threadIdx.x, w = threadIdx.y, W = blockDim.y, s = blockIdx.y;
-    const Recurrence<E, VEC> r(p, (long long)blockIdx.x * WAVE + lane);
+    const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
+    const Chain<VEC> ch(blockIdx.x * WAVE + lane, p.N, p.D);
     const long long chains = (long long)p.N * p.D;
-    float y[VEC];  // what reaches h from the steps behind the tile
-    for (int v = 0; v < VEC; v++) y[v] = p.d_state_out && v < r.ch.count ? p.d_state_out[r.ch.c + v] : 0.f;
-    if (s < g.count - 1) run_segments<VEC>(y, g, g.count, s + 1, chains, r.ch, fore[0], w, W, lane);
-    const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE);
-    for (int t0 = begin + (end - begin - 1) / TILE * TILE, odd = 0; t0 >= begin; t0 -= TILE, odd ^= 1) {
+    const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE), last = end - 1;
+    const bool any = p.d_h.data;
+    const Column<E, VEC> gate(p.gate, ch), update(p.update, ch), d_h(any ? p.d_h : p.gate, ch), d_gate(p.d_gate, ch), d_update(p.d_update, ch);
+    const Flags first(p.first, p.first_t_stride, p.first_n_stride, ch.n, gate.base);
+    Raw<E, VEC> ra[K], rb[K], rd[K];
+    uint8_t rf[K];
+    float start[VEC];
+    auto load = [&](int t0) {
         const int t = t0 + w * K;
-        Row<E, VEC> a[K], b[K], d[K];
+        gate.load(ra, t, last);
+        d_h.load(rd, t, last);
+        update.load(rb, t, last);
+        first.load(rf, t, last);
+        load_state<VEC>(start, p.checkpoints + (long long)(t0 / TILE) * chains, ch);
+    };
+    const int top = begin + (end - begin - 1) / TILE * TILE;
+    load(top);
+    float y[VEC];  // what reaches h from the steps behind the tile
+    load_state<VEC>(y, p.d_state_out, ch);
+    if (s < g.count - 1) run_segments<VEC>(y, g, g.count, s + 1, chains, ch, fore[0], w, W, lane);
+    for (int t0 = top, odd = 0; t0 >= begin; t0 -= TILE, odd ^= 1) {
+        const int t = t0 + w * K;
+        float a[K][VEC], b[K][VEC], d[K][VEC], x[VEC], before[VEC], behind[VEC];
         bool cut[K];
-        float x[VEC], before[VEC], behind[VEC];
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            const bool real = r.ch.count && t + k < end;
-            a[k] = r.load(p.gate, t + k, real, 1.f);
-            b[k] = r.load(p.update, t + k, real, 0.f);
-            d[k] = r.load(p.d_h, t + k, real && p.d_h.data, 0.f);
-            cut[k] = r.cut(t + k, real);
-        }
-        for (int v = 0; v < VEC; v++) x[v] = v < r.ch.count ? p.checkpoints[(long long)(t0 / TILE) * chains + r.ch.c + v] : 0.f;
-        fore[odd].put(w, lane, compose<E, VEC, false>(a, b, cut));
-        back[odd].put(w, lane, compose<E, VEC, true>(a, d, cut));
+        convert<E, VEC>(a, ra, t, end, 1.f);
+        convert<E, VEC>(b, rb, t, end, 0.f);
+        convert<E, VEC>(d, rd, t, any ? end : 0, 0.f);
+        convert(cut, rf, first.mask, t, end);
+        for (int v = 0; v < VEC; v++) x[v] = start[v];
+        if (t0 > begin) load(t0 - TILE);
+        fore[odd].put(w, lane, compose<VEC, false>(a, b, cut));
+        back[odd].put(w, lane, compose<VEC, true>(a, d, cut));
         __syncthreads();
         for (int v = 0; v < VEC; v++) before[v] = x[v], behind[v] = y[v];
         for (int k = 0; k < W; k++) {
@@ -303,27 +343,25 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_backward(procgen_amd_r
 #pragma unroll
         for (int k = 0; k < K; k++)  // b becomes the value before the step
             for (int v = 0; v < VEC; v++) {
-                const float h = cut[k] ? b[k].x[v] : fmaf(a[k].x[v], before[v], b[k].x[v]);
-                b[k].x[v] = before[v];
+                const float h = cut[k] ? b[k][v] : fmaf(a[k][v], before[v], b[k][v]);
+                b[k][v] = before[v];
                 before[v] = h;
             }
 #pragma unroll
         for (int k = K - 1; k >= 0; k--) {
             for (int v = 0; v < VEC; v++) {
-                const float gr = d[k].x[v] + behind[v];
-                d[k].x[v] = gr;
-                b[k].x[v] = cut[k] ? 0.f : gr * b[k].x[v];
-                behind[v] = cut[k] ? 0.f : a[k].x[v] * gr;
+                const float gr = d[k][v] + behind[v];
+                d[k][v] = gr;
+                b[k][v] = cut[k] ? 0.f : gr * b[k][v];
+                behind[v] = cut[k] ? 0.f : a[k][v] * gr;
             }
-            if (r.ch.count && t + k < end) {
-                if (p.d_update.data) store_row<E, VEC>(r.at(p.d_update, t + k), r.ch.count, d[k]);
-                if (p.d_gate.data) store_row<E, VEC>(r.at(p.d_gate, t + k), r.ch.count, b[k]);
+            if (t + k < end) {
+                if (p.d_update.data) d_update.store(t + k, d[k], ch);
+                if (p.d_gate.data) d_gate.store(t + k, b[k], ch);
             }
         }
     }
-    if (p.d_state && w == 0 && s == 0)
-        for (int v = 0; v < VEC; v++)
-            if (v < r.ch.count) p.d_state[r.ch.c + v] = y[v];
+    if (p.d_state && w == 0 && s == 0) store_state<VEC>(p.d_state, y, ch);
 }
 
 // ---- advantages: the recurrence adv[t] = (gamma lam) adv[t+1] + delta[t], from the last step to the first, a chain per env -----------------------------
@@ -331,32 +369,39 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_backward(procgen_amd_r
 template <class E>
 struct Advantage {
     const procgen_amd_advantage &p;
-    const int n;
+    const Chain<1> ch;
     const float decay;
     const uint8_t *first;
     const typename E::T *values;
     const float *rew;
-    __device__ Advantage(const procgen_amd_advantage &args, int env)
-        : p(args), n(env), decay(args.gamma * args.lam), first(args.first + n * args.first_n_stride), values((const typename E::T *)args.values + n * args.values_n_stride),
-          rew(args.rew + n * args.rew_n_stride) {}
-    // steps t .. t + K - 1: cut[k], a[k] (1 where there is no step), b[k] = delta, v[k] = the value before the step
-    __device__ void load(int t, int end, bool *cut, float *a, float *b, float *v) const {
-        const bool here = n < p.N;
+    // steps t .. t + K - 1 as loaded: flags and values of the step behind each, the value of the first, rewards
+    uint8_t rf[K];
+    typename E::T rv[K + 1];
+    float rr[K];
+    __device__ Advantage(const procgen_amd_advantage &args)
+        : p(args), ch(blockIdx.x * WAVE + threadIdx.x, args.N, 1), decay(args.gamma * args.lam), first(args.first + ch.n * args.first_n_stride),
+          values((const typename E::T *)args.values + ch.n * args.values_n_stride), rew(args.rew + ch.n * args.rew_n_stride) {}
+    __device__ void load(int t, int last) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const bool real = here && t + k < end;
-            cut[k] = real && first[(t + k + 1) * p.first_t_stride];
-            v[k] = real ? (float)values[(t + k) * p.values_t_stride] : 0.f;
-            b[k] = real ? rew[(t + k) * p.rew_t_stride] : 0.f;
+            const int at = min(t + k, last);
+            rf[k] = first[(at + 1) * p.first_t_stride];
+            rr[k] = rew[at * p.rew_t_stride];
+            rv[k] = values[at * p.values_t_stride];
         }
-        const int next = min(t + K, end);  // the value behind the last of these steps
-        const float behind = here && t < end ? (float)values[next * p.values_t_stride] : 0.f;
+        rv[K] = values[(min(t + K - 1, last) + 1) * p.values_t_stride];
+    }
+    // cut[k], a[k] (1 where there is no step), b[k] = delta, v[k] = the value before the step
+    __device__ void convert(int t, int end, bool *cut, float *a, float *b, float *v) const {
+        const int n = min(K, end - t);
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const bool real = here && t + k < end;
-            const float after = k + 1 < K && t + k + 1 < end ? v[k + 1] : behind;
+            const bool real = k < n;
+            cut[k] = real && rf[k];
+            v[k] = (float)rv[k];
+            const float after = k + 1 < n ? (float)rv[k + 1] : (float)rv[K];
             a[k] = real ? decay : 1.f;
-            b[k] = real ? (cut[k] ? b[k] : fmaf(p.gamma, after, b[k])) - v[k] : 0.f;
+            b[k] = real ? (cut[k] ? rr[k] : fmaf(p.gamma, after, rr[k])) - v[k] : 0.f;
         }
     }
 };
@@ -375,18 +420,18 @@ __device__ inline Map<1> compose_back(const bool *cut, const float *a, const flo
 template <class E>
 __global__ __launch_bounds__(MAX_W *WAVE) void advantage_segments(procgen_amd_advantage p, Segments g) {
     __shared__ Pieces<1> pieces;
-    const int lane = threadIdx.x, w = threadIdx.y, W = blockDim.y, s = blockIdx.y;
-    const Advantage<E> r(p, blockIdx.x * WAVE + lane);
-    const Chain<1> ch(blockIdx.x * WAVE + lane, p.N, 1);
+    const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
+    Advantage<E> r(p);
     const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE);
     const int part = (g.tiles * TILE + W * K - 1) / (W * K) * K;
-    const int from = begin + w * part, to = min(end, from + part);
+    const int from = min((long long)end, (long long)begin + (long long)w * part), to = min((long long)end, (long long)from + part);
     Map<1> m;
     m.identity();
-    for (int i = 0; i < part; i += K) {
+    for (int t = from + (to - from - 1) / K * K; t >= from && t < to; t -= K) {
         bool cut[K];
         float a[K], b[K], v[K];
-        r.load(from + part - K - i, to, cut, a, b, v);
+        r.load(t, to - 1);
+        r.convert(t, to, cut, a, b, v);
         m.then(compose_back(cut, a, b));
     }
     pieces.put(w, lane, m);
@@ -394,23 +439,25 @@ __global__ __launch_bounds__(MAX_W *WAVE) void advantage_segments(procgen_amd_ad
     if (w) return;
     m.identity();
     for (int k = W - 1; k >= 0; k--) m.then(pieces.get(k, lane));
-    put_segment<1>(g, s, p.N, ch, m);
+    put_segment<1>(g, s, p.N, r.ch, m);
 }
 
 template <class E>
 __global__ __launch_bounds__(MAX_W *WAVE) void advantages(procgen_amd_advantage p, Segments g) {
     __shared__ Pieces<1> pieces[2];
-    const int lane = threadIdx.x, w = threadIdx.y, W = blockDim.y, s = blockIdx.y;
-    const Advantage<E> r(p, blockIdx.x * WAVE + lane);
-    const Chain<1> ch(blockIdx.x * WAVE + lane, p.N, 1);
-    float y = 0.f;
-    if (s < g.count - 1) run_segments<1>(&y, g, g.count, s + 1, p.N, ch, pieces[0], w, W, lane);
+    const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
+    Advantage<E> r(p);
     const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE);
-    for (int t0 = begin + (end - begin - 1) / TILE * TILE, odd = 0; t0 >= begin; t0 -= TILE, odd ^= 1) {
+    const int top = begin + (end - begin - 1) / TILE * TILE;
+    r.load(top + w * K, end - 1);
+    float y = 0.f;
+    if (s < g.count - 1) run_segments<1>(&y, g, g.count, s + 1, p.N, r.ch, pieces[0], w, W, lane);
+    for (int t0 = top, odd = 0; t0 >= begin; t0 -= TILE, odd ^= 1) {
         const int t = t0 + w * K;
         bool cut[K];
         float a[K], b[K], v[K];
-        r.load(t, end, cut, a, b, v);
+        r.convert(t, end, cut, a, b, v);
+        if (t0 > begin) r.load(t - TILE, end - 1);
         pieces[odd].put(w, lane, compose_back(cut, a, b));
         __syncthreads();
         float adv = y;
@@ -421,9 +468,9 @@ __global__ __launch_bounds__(MAX_W *WAVE) void advantages(procgen_amd_advantage 
 #pragma unroll
         for (int k = K - 1; k >= 0; k--) {
             adv = cut[k] ? b[k] : fmaf(a[k], adv, b[k]);
-            if (r.n < p.N && t + k < end) {
-                if (p.adv) p.adv[(long long)(t + k) * p.N + r.n] = adv;
-                if (p.ret) p.ret[(long long)(t + k) * p.N + r.n] = adv + v[k];
+            if (r.ch.mine(0) && t + k < end) {
+                if (p.adv) p.adv[(long long)(t + k) * p.N + r.ch.n] = adv;
+                if (p.ret) p.ret[(long long)(t + k) * p.N + r.ch.n] = adv + v[k];
             }
         }
     }
@@ -457,14 +504,13 @@ long long segment_bytes(int T, long long chains) {
     return s > 1 ? s * chains * 9 + chains * 4 : 0;
 }
 
-// neighbouring channels of a lane: as many as still leave enough blocks, where the arrays have them next to each other
+// neighbouring channels of a lane: as many as still leave enough blocks, up to 8 bytes, where the arrays have them next to each other
 int vec_for(const procgen_amd_recurrence *a, bool backward) {
     const procgen_amd_array3 *all[] = {&a->gate, &a->update, &a->h, &a->d_h, &a->d_gate, &a->d_update};
     for (int i = 0; i < (backward ? 6 : 3); i++)
         if (all[i]->data && all[i]->d_stride != 1 && a->D > 1) return 1;
-    if (a->D == 1) return 1;
-    for (int vec = backward ? 2 : 4; vec > 1; vec /= 2)
-        if ((long long)a->N * ((a->D + vec - 1) / vec) >= (long long)FULL * WAVE) return vec;
+    for (int vec = backward || a->dtype == PROCGEN_AMD_F32 ? 2 : 4; vec > 1; vec /= 2)
+        if (a->D >= vec && (long long)a->N * ((a->D + vec - 1) / vec) >= (long long)FULL * WAVE) return vec;
     return 1;
 }
 template <class Fn>
