@@ -17,7 +17,7 @@ namespace pgamd {
 namespace learner {
 namespace {
 
-constexpr int K = 8, MAX_W = 8, TILE = K * MAX_W;
+constexpr int K = 8, MAX_W = 4, TILE = K * MAX_W;
 
 // VEC neighbouring channels of a step, as memory holds them.  Loads are unconditional (addresses are clamped into the arrays and values selected
 // afterwards): a load behind a branch of its own would be waited for before the next is issued.
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(MAX_W *WAVE) void advantages(procgen_amd_advantage 
 
 bool shape_ok(int dtype, int T, int N, int D) { return known_dtype(dtype) && T >= 0 && T <= 0x7fffff00 && N >= 0 && D >= 0 && (long long)N * D <= 0x7fffff00ll; }
 
-constexpr int FULL = 512;  // blocks of 8 waves that fill the card: two on each of the 256 compute units
+constexpr int FULL = 1024;  // blocks of 8 waves that fill the card: two on each of the 256 compute units
 int tiles_of(int T) { return (T + TILE - 1) / TILE; }
 // how many segments a window of this many blocks' worth of chains is cut into: by its sizes alone, so that the workspace does not depend on strides
 int segments_of(int T, long long chains) {
@@ -509,7 +509,7 @@ int vec_for(const procgen_amd_recurrence *a, bool backward) {
     const procgen_amd_array3 *all[] = {&a->gate, &a->update, &a->h, &a->d_h, &a->d_gate, &a->d_update};
     for (int i = 0; i < (backward ? 6 : 3); i++)
         if (all[i]->data && all[i]->d_stride != 1 && a->D > 1) return 1;
-    for (int vec = backward || a->dtype == PROCGEN_AMD_F32 ? 2 : 4; vec > 1; vec /= 2)
+    for (int vec = 2; vec > 1; vec /= 2)
         if (a->D >= vec && (long long)a->N * ((a->D + vec - 1) / vec) >= (long long)FULL * WAVE) return vec;
     return 1;
 }
