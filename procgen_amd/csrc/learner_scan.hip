@@ -17,7 +17,10 @@ namespace pgamd {
 namespace learner {
 namespace {
 
-constexpr int K = 8, MAX_W = 4, TILE = K * MAX_W;
+constexpr int W_MAX = 4;          // waves of a block
+constexpr int KF = 8, KB = 4;     // steps of a wave in a tile: forwards (and advantages), backwards
+constexpr int TILE = KF * W_MAX;  // a segment is a whole number of these
+constexpr int CHECK = KB * W_MAX; // steps from one checkpoint to the next: a tile of the backward pass
 
 // VEC neighbouring channels of a step, as memory holds them.  Loads are unconditional (addresses are clamped into the arrays and values selected
 // afterwards): a load behind a branch of its own would be waited for before the next is issued.
@@ -51,8 +54,8 @@ struct Pieces {
     struct alignas(4 * VEC) Vec {
         float x[VEC];
     };
-    Vec A[MAX_W][WAVE], B[MAX_W][WAVE];
-    int cut[MAX_W][WAVE];
+    Vec A[W_MAX][WAVE], B[W_MAX][WAVE];
+    int cut[W_MAX][WAVE];
     __device__ void put(int w, int lane, const Map<VEC> &m) {
         Vec a, b;
         for (int v = 0; v < VEC; v++) a.x[v] = m.A[v], b.x[v] = m.B[v];
@@ -127,7 +130,7 @@ __device__ inline void run_segments(float *x, const Segments &g, int from, int t
 }
 
 // a lane's view of one array: the rows of its channels
-template <class E, int VEC>
+template <class E, int VEC, int K>
 struct Column {
     typename E::T *base;
     long long stride;
@@ -154,7 +157,8 @@ struct Flags {
     uint8_t mask;
     __device__ Flags(const uint8_t *first, long long t_stride, long long n_stride, int n, const void *otherwise)
         : base(first ? first + n * n_stride : (const uint8_t *)otherwise), stride(first ? t_stride : 0), mask(first ? 0xff : 0) {}
-    __device__ void load(uint8_t *to, int t, int last) const {
+    template <int K>
+    __device__ void load(uint8_t (&to)[K], int t, int last) const {
 #pragma unroll
         for (int k = 0; k < K; k++) to[k] = base[min(t + k, last) * stride];
     }
@@ -171,8 +175,8 @@ __device__ inline void store_state(float *state, const float *x, const Chain<VEC
 }
 
 // the composition of K steps: x -> gate x + update forwards; backwards the gradient y of a step's h from behind it becomes gate (d + y) before it
-template <int VEC, bool REVERSE>
-__device__ inline Map<VEC> compose(const float (*a)[VEC], const float (*b)[VEC], const bool *cut) {
+template <int VEC, bool REVERSE, int K>
+__device__ inline Map<VEC> compose(const float (&a)[K][VEC], const float (&b)[K][VEC], const bool (&cut)[K]) {
     Map<VEC> m;
     m.identity();
 #pragma unroll
@@ -187,20 +191,22 @@ __device__ inline Map<VEC> compose(const float (*a)[VEC], const float (*b)[VEC],
     return m;
 }
 // K loaded steps in 32 bits; those at `end` and behind it become the identity
-template <class E, int VEC>
-__device__ inline void convert(float (*x)[VEC], const Raw<E, VEC> *raw, int t, int end, float otherwise) {
+template <class E, int VEC, int K>
+__device__ inline void convert(float (&x)[K][VEC], const Raw<E, VEC> (&raw)[K], int t, int end, float otherwise) {
 #pragma unroll
     for (int k = 0; k < K; k++)
         for (int v = 0; v < VEC; v++) x[k][v] = t + k < end ? (float)raw[k].x[v] : otherwise;
 }
-__device__ inline void convert(bool *cut, const uint8_t *raw, uint8_t mask, int t, int end) {
+template <int K>
+__device__ inline void convert(bool (&cut)[K], const uint8_t (&raw)[K], uint8_t mask, int t, int end) {
 #pragma unroll
     for (int k = 0; k < K; k++) cut[k] = t + k < end && (raw[k] & mask);
 }
 
 // the map of every segment (blockIdx.y): forwards of gate and update, backwards of gate and d_h.  The waves take a part of the segment each.
 template <class E, int VEC, bool REVERSE>
-__global__ __launch_bounds__(MAX_W *WAVE) void recurrence_segments(procgen_amd_recurrence p, Segments g) {
+__global__ __launch_bounds__(W_MAX *WAVE) void recurrence_segments(procgen_amd_recurrence p, Segments g) {
+    constexpr int K = KF;
     __shared__ Pieces<VEC> pieces;
     const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
     const Chain<VEC> ch(blockIdx.x * WAVE + lane, p.N, p.D);
@@ -209,7 +215,7 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_segments(procgen_amd_r
     const int part = (g.tiles * TILE + W * K - 1) / (W * K) * K;  // steps of a wave
     const int from = min((long long)end, (long long)begin + (long long)w * part), to = min((long long)end, (long long)from + part);
     const bool any = !REVERSE || p.d_h.data;
-    const Column<E, VEC> gate(p.gate, ch), other(REVERSE ? (any ? p.d_h : p.gate) : p.update, ch);
+    const Column<E, VEC, K> gate(p.gate, ch), other(REVERSE ? (any ? p.d_h : p.gate) : p.update, ch);
     const Flags first(p.first, p.first_t_stride, p.first_n_stride, ch.n, gate.base);
     Map<VEC> m;
     m.identity();
@@ -222,10 +228,10 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_segments(procgen_amd_r
         first.load(rf, t, end - 1);
         float a[K][VEC], b[K][VEC];
         bool cut[K];
-        convert<E, VEC>(a, ra, t, to, 1.f);
-        convert<E, VEC>(b, rb, t, any ? to : 0, 0.f);
+        convert<E, VEC, K>(a, ra, t, to, 1.f);
+        convert<E, VEC, K>(b, rb, t, any ? to : 0, 0.f);
         convert(cut, rf, first.mask, t, to);
-        m.then(compose<VEC, REVERSE>(a, b, cut));
+        m.then(compose<VEC, REVERSE, K>(a, b, cut));
     }
     pieces.put(w, lane, m);
     __syncthreads();
@@ -241,13 +247,14 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_segments(procgen_amd_r
 }
 
 template <class E, int VEC>
-__global__ __launch_bounds__(MAX_W *WAVE) void recurrence_forward(procgen_amd_recurrence p, Segments g) {
+__global__ __launch_bounds__(W_MAX *WAVE) void recurrence_forward(procgen_amd_recurrence p, Segments g) {
+    constexpr int K = KF;
     __shared__ Pieces<VEC> pieces[2];
     const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
     const Chain<VEC> ch(blockIdx.x * WAVE + lane, p.N, p.D);
     const long long chains = (long long)p.N * p.D;
     const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE), last = end - 1;
-    const Column<E, VEC> gate(p.gate, ch), update(p.update, ch), out(p.h, ch);
+    const Column<E, VEC, K> gate(p.gate, ch), update(p.update, ch), out(p.h, ch);
     const Flags first(p.first, p.first_t_stride, p.first_n_stride, ch.n, gate.base);
     Raw<E, VEC> ra[K], rb[K];
     uint8_t rf[K];
@@ -264,12 +271,11 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_forward(procgen_amd_re
         const int t = t0 + w * K;
         float a[K][VEC], b[K][VEC];
         bool cut[K];
-        convert<E, VEC>(a, ra, t, end, 1.f);
-        convert<E, VEC>(b, rb, t, end, 0.f);
+        convert<E, VEC, K>(a, ra, t, end, 1.f);
+        convert<E, VEC, K>(b, rb, t, end, 0.f);
         convert(cut, rf, first.mask, t, end);
         if (t0 + TILE < end) load(t + TILE);  // the next tile is on its way while this one is joined
-        if (p.checkpoints && w == 0) store_state<VEC>(p.checkpoints + (long long)(t0 / TILE) * chains, x, ch);
-        pieces[odd].put(w, lane, compose<VEC, false>(a, b, cut));
+        pieces[odd].put(w, lane, compose<VEC, false, K>(a, b, cut));
         __syncthreads();
         float y[VEC];
         for (int v = 0; v < VEC; v++) y[v] = x[v];
@@ -280,6 +286,7 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_forward(procgen_amd_re
                 x[v] = q.at(x[v], v);
             }
         }
+        if (p.checkpoints && w * K % CHECK == 0 && t < end) store_state<VEC>(p.checkpoints + (long long)(t / CHECK) * chains, y, ch);
 #pragma unroll
         for (int k = 0; k < K; k++) {
             for (int v = 0; v < VEC; v++) y[v] = cut[k] ? b[k][v] : fmaf(a[k][v], y[v], b[k][v]);
@@ -292,14 +299,15 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_forward(procgen_amd_re
 // Backwards over the tiles.  h is not read: its 32-bit value before every step comes from the checkpoint at the tile's start and the same joins as in
 // the forward pass (update is read in its place, so the bytes are the same and 16-bit rounding of h does not reach d_gate).
 template <class E, int VEC>
-__global__ __launch_bounds__(MAX_W *WAVE) void recurrence_backward(procgen_amd_recurrence p, Segments g) {
+__global__ __launch_bounds__(W_MAX *WAVE) void recurrence_backward(procgen_amd_recurrence p, Segments g) {
+    constexpr int K = KB;
     __shared__ Pieces<VEC> fore[2], back[2];
     const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
     const Chain<VEC> ch(blockIdx.x * WAVE + lane, p.N, p.D);
     const long long chains = (long long)p.N * p.D;
     const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE), last = end - 1;
     const bool any = p.d_h.data;
-    const Column<E, VEC> gate(p.gate, ch), update(p.update, ch), d_h(any ? p.d_h : p.gate, ch), d_gate(p.d_gate, ch), d_update(p.d_update, ch);
+    const Column<E, VEC, K> gate(p.gate, ch), update(p.update, ch), d_h(any ? p.d_h : p.gate, ch), d_gate(p.d_gate, ch), d_update(p.d_update, ch);
     const Flags first(p.first, p.first_t_stride, p.first_n_stride, ch.n, gate.base);
     Raw<E, VEC> ra[K], rb[K], rd[K];
     uint8_t rf[K];
@@ -310,25 +318,25 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_backward(procgen_amd_r
         d_h.load(rd, t, last);
         update.load(rb, t, last);
         first.load(rf, t, last);
-        load_state<VEC>(start, p.checkpoints + (long long)(t0 / TILE) * chains, ch);
+        load_state<VEC>(start, p.checkpoints + (long long)(t0 / CHECK) * chains, ch);
     };
-    const int top = begin + (end - begin - 1) / TILE * TILE;
+    const int top = begin + (end - begin - 1) / CHECK * CHECK;
     load(top);
     float y[VEC];  // what reaches h from the steps behind the tile
     load_state<VEC>(y, p.d_state_out, ch);
     if (s < g.count - 1) run_segments<VEC>(y, g, g.count, s + 1, chains, ch, fore[0], w, W, lane);
-    for (int t0 = top, odd = 0; t0 >= begin; t0 -= TILE, odd ^= 1) {
+    for (int t0 = top, odd = 0; t0 >= begin; t0 -= CHECK, odd ^= 1) {
         const int t = t0 + w * K;
         float a[K][VEC], b[K][VEC], d[K][VEC], x[VEC], before[VEC], behind[VEC];
         bool cut[K];
-        convert<E, VEC>(a, ra, t, end, 1.f);
-        convert<E, VEC>(b, rb, t, end, 0.f);
-        convert<E, VEC>(d, rd, t, any ? end : 0, 0.f);
+        convert<E, VEC, K>(a, ra, t, end, 1.f);
+        convert<E, VEC, K>(b, rb, t, end, 0.f);
+        convert<E, VEC, K>(d, rd, t, any ? end : 0, 0.f);
         convert(cut, rf, first.mask, t, end);
         for (int v = 0; v < VEC; v++) x[v] = start[v];
-        if (t0 > begin) load(t0 - TILE);
-        fore[odd].put(w, lane, compose<VEC, false>(a, b, cut));
-        back[odd].put(w, lane, compose<VEC, true>(a, d, cut));
+        if (t0 > begin) load(t0 - CHECK);
+        fore[odd].put(w, lane, compose<VEC, false, K>(a, b, cut));
+        back[odd].put(w, lane, compose<VEC, true, K>(a, d, cut));
         __syncthreads();
         for (int v = 0; v < VEC; v++) before[v] = x[v], behind[v] = y[v];
         for (int k = 0; k < W; k++) {
@@ -368,6 +376,7 @@ __global__ __launch_bounds__(MAX_W *WAVE) void recurrence_backward(procgen_amd_r
 
 template <class E>
 struct Advantage {
+    static constexpr int K = KF;
     const procgen_amd_advantage &p;
     const Chain<1> ch;
     const float decay;
@@ -405,7 +414,8 @@ struct Advantage {
         }
     }
 };
-__device__ inline Map<1> compose_back(const bool *cut, const float *a, const float *b) {
+template <int K>
+__device__ inline Map<1> compose_back(const bool (&cut)[K], const float (&a)[K], const float (&b)[K]) {
     Map<1> m;
     m.identity();
 #pragma unroll
@@ -418,7 +428,8 @@ __device__ inline Map<1> compose_back(const bool *cut, const float *a, const flo
 }
 
 template <class E>
-__global__ __launch_bounds__(MAX_W *WAVE) void advantage_segments(procgen_amd_advantage p, Segments g) {
+__global__ __launch_bounds__(W_MAX *WAVE) void advantage_segments(procgen_amd_advantage p, Segments g) {
+    constexpr int K = KF;
     __shared__ Pieces<1> pieces;
     const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
     Advantage<E> r(p);
@@ -443,7 +454,8 @@ __global__ __launch_bounds__(MAX_W *WAVE) void advantage_segments(procgen_amd_ad
 }
 
 template <class E>
-__global__ __launch_bounds__(MAX_W *WAVE) void advantages(procgen_amd_advantage p, Segments g) {
+__global__ __launch_bounds__(W_MAX *WAVE) void advantages(procgen_amd_advantage p, Segments g) {
+    constexpr int K = KF;
     __shared__ Pieces<1> pieces[2];
     const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
     Advantage<E> r(p);
@@ -504,13 +516,14 @@ long long segment_bytes(int T, long long chains) {
     return s > 1 ? s * chains * 9 + chains * 4 : 0;
 }
 
-// neighbouring channels of a lane: as many as still leave enough blocks, up to 8 bytes, where the arrays have them next to each other
+// neighbouring channels of a lane, where the arrays have them next to each other: as many as still leave half a card's blocks, up to 8 bytes; two
+// backwards, whose three arrays would take 190 registers with four
 int vec_for(const procgen_amd_recurrence *a, bool backward) {
     const procgen_amd_array3 *all[] = {&a->gate, &a->update, &a->h, &a->d_h, &a->d_gate, &a->d_update};
     for (int i = 0; i < (backward ? 6 : 3); i++)
         if (all[i]->data && all[i]->d_stride != 1 && a->D > 1) return 1;
-    for (int vec = 2; vec > 1; vec /= 2)
-        if (a->D >= vec && (long long)a->N * ((a->D + vec - 1) / vec) >= (long long)FULL * WAVE) return vec;
+    for (int vec = backward || a->dtype == PROCGEN_AMD_F32 ? 2 : 4; vec > 1; vec /= 2)
+        if (a->D >= vec && (long long)a->N * ((a->D + vec - 1) / vec) >= FULL / 2 * (long long)WAVE) return vec;
     return 1;
 }
 template <class Fn>
@@ -530,7 +543,7 @@ using namespace pgamd::learner;
 
 extern "C" {
 
-LIBENV_API long long procgen_amd_recurrence_checkpoints(int T) { return tiles_of(T); }
+LIBENV_API long long procgen_amd_recurrence_checkpoints(int T) { return T > 0 ? ((long long)T + CHECK - 1) / CHECK : 0; }
 LIBENV_API long long procgen_amd_recurrence_workspace(int T, int N, int D) { return T > 0 && N > 0 && D > 0 ? segment_bytes(T, (long long)N * D) : 0; }
 
 LIBENV_API int procgen_amd_recurrence_forward(const struct procgen_amd_recurrence *a, int device, void *stream) {
@@ -545,7 +558,7 @@ LIBENV_API int procgen_amd_recurrence_forward(const struct procgen_amd_recurrenc
         return by_vec(vec_for(a, false), [&](auto vec) {
             typedef decltype(e) E;
             constexpr int VEC = decltype(vec)::value;
-            const dim3 grid((unsigned)(((long long)a->N * ((a->D + VEC - 1) / VEC) + WAVE - 1) / WAVE), g.count), block(WAVE, std::min(MAX_W, (a->T + K - 1) / K));
+            const dim3 grid((unsigned)(((long long)a->N * ((a->D + VEC - 1) / VEC) + WAVE - 1) / WAVE), g.count), block(WAVE, std::min(W_MAX, (a->T + KF - 1) / KF));
             if (g.count > 1) {
                 recurrence_segments<E, VEC, false><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
                 if (int err = launched()) return err;
@@ -567,8 +580,8 @@ LIBENV_API int procgen_amd_recurrence_backward(const struct procgen_amd_recurren
     return by_dtype(a->dtype, [&](auto e) {
         return by_vec(vec_for(a, true), [&](auto vec) {
             typedef decltype(e) E;
-            constexpr int VEC = std::min(2, decltype(vec)::value);  // four channels a lane take 187 registers: one block on a compute unit
-            const dim3 grid((unsigned)(((long long)a->N * ((a->D + VEC - 1) / VEC) + WAVE - 1) / WAVE), g.count), block(WAVE, std::min(MAX_W, (a->T + K - 1) / K));
+            constexpr int VEC = std::min(2, decltype(vec)::value);
+            const dim3 grid((unsigned)(((long long)a->N * ((a->D + VEC - 1) / VEC) + WAVE - 1) / WAVE), g.count), block(WAVE, std::min(W_MAX, (a->T + KB - 1) / KB));
             if (g.count > 1) {
                 recurrence_segments<E, VEC, true><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
                 if (int err = launched()) return err;
@@ -588,7 +601,7 @@ LIBENV_API int procgen_amd_advantages(const struct procgen_amd_advantage *a, int
     if (on.err != hipSuccess) return (int)on.err;
     return by_dtype(a->dtype, [&](auto e) {
         typedef decltype(e) E;
-        const dim3 grid((a->N + WAVE - 1) / WAVE, g.count), block(WAVE, std::min(MAX_W, (a->T + K - 1) / K));
+        const dim3 grid((a->N + WAVE - 1) / WAVE, g.count), block(WAVE, std::min(W_MAX, (a->T + KF - 1) / KF));
         if (g.count > 1) {
             advantage_segments<E><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
             if (int err = launched()) return err;
