@@ -5,6 +5,13 @@
 // reference row r (m', s' alike)  KL = (sum e ((l - m) - (r - m'))) / s + log(s' / s): every term is of the size of the differences, so nothing of
 // the size of the logits cancels.  The gradients of all three operators have one form,
 //     dl[j] = pick * (1[j = a] - p[j]) + p[j] * (kl * (log p[j] - log q[j] - KL) + ent * (log p[j] + H)).
+// Partial sums of a row are taken against the largest value their lane or wave has seen and rescaled when they meet (Stats::join), so a row is read once.
+//
+// Bound by memory: a column costs some 20 operations for 4 to 12 bytes.  Three kernels by the number of columns, each reading and writing a row once
+// and 16 bytes a lane:
+//   up to 64      a wave takes 64 rows through LDS, a lane per row: no reduction over lanes, coalesced although a row is no multiple of anything
+//   more          a group of 16, 64, 256 or 1024 lanes per row keeps the row in its registers between the sums and the gradient
+//   very long     the same group in batches; the gradient goes through them backwards, so the last is still in registers and the others in cache
 #include "learner.h"
 
 #include <algorithm>
@@ -13,202 +20,528 @@ namespace pgamd {
 namespace learner {
 namespace {
 
-constexpr int ROWS_PER_BLOCK = 4;  // one wave per row
+constexpr int BLOCK = 256;
 constexpr int MAX_COUNT_BLOCKS = 256;
+constexpr int MAX_BLOCKS = 2048;
 
 __device__ inline long long action_of(const procgen_amd_rows &p, long long r) {
     return p.actions_are_64_bit ? ((const long long *)p.actions)[r] : (long long)((const int *)p.actions)[r];
 }
-__device__ inline long long row_offset(const procgen_amd_rows &p, long long r, long long outer, long long inner) { return (r / p.inner) * outer + (r % p.inner) * inner; }
+__device__ inline long long row_offset(const procgen_amd_rows &p, long long r, long long outer, long long inner) {
+    return p.inner == 1 ? r * outer : (r / p.inner) * outer + (r % p.inner) * inner;
+}
 
+// sums over the columns seen so far.  m = -inf: none that is finite; s is then 0, or NaN where a NaN was among them
+template <bool REF>
 struct Stats {
-    float m, s, w;    // max, sum e, sum e (l - m)
-    float m2, s2, u;  // of the reference row, and sum e ((l - m) - (r - m2))
-};
-
-template <class E, bool REF>
-__device__ inline Stats row_stats(const typename E::T *l, const typename E::T *r, long long columns, int lane) {
-    Stats x;
-    x.m = x.m2 = -INFINITY;
-    for (long long j = lane; j < columns; j += WAVE) {
-        x.m = fmaxf(x.m, (float)l[j]);
-        if (REF) x.m2 = fmaxf(x.m2, (float)r[j]);
+    float m = -INFINITY, s = 0.f, w = 0.f;   // max, sum e, sum e (l - m)
+    float m2 = -INFINITY, s2 = 0.f, u = 0.f; // of the reference row, and sum e ((l - m) - (r - m2))
+    __device__ static float safe(float m) { return m == -INFINITY ? 0.f : m; }
+    __device__ void put(float *to) const {
+        to[0] = m, to[1] = s, to[2] = w;
+        if (REF) to[3] = m2, to[4] = s2, to[5] = u;
     }
-    x.m = wave_reduce(x.m, Max());
-    if (REF) x.m2 = wave_reduce(x.m2, Max());
-    x.s = x.w = x.s2 = x.u = 0.f;
-    if (x.m > -INFINITY || x.m != x.m)
-        for (long long j = lane; j < columns; j += WAVE) {
-            const float d = (float)l[j] - x.m, e = __expf(d);
-            x.s += e;
-            if (e != 0.f) x.w += e * d;
+    __device__ void get(const float *from) {
+        m = from[0], s = from[1], w = from[2];
+        if (REF) m2 = from[3], s2 = from[4], u = from[5];
+    }
+    __device__ bool empty() const { return m == -INFINITY && s == 0.f; }
+    // the same sums against larger maxima
+    __device__ void rescale(float to, float to2) {
+        const float d = m == -INFINITY ? 0.f : m - to, c = __expf(d), d2 = !REF || m2 == -INFINITY ? 0.f : m2 - to2;
+        if (REF) {
+            u = c == 0.f ? 0.f : c * (u + s * (d - d2));  // sums that vanish against the new maximum, far as it may be (s d overflows), are zero
+            s2 *= __expf(d2);
+            m2 = to2;
+        }
+        w = c == 0.f ? 0.f : c * (w + s * d);
+        s *= c;
+        m = to;
+    }
+    __device__ void add(float l, float r) {  // against maxima that cover them
+        const float d = l - safe(m), e = __expf(d);
+        s += e;
+        if (e != 0.f) w += e * d;
+        if (REF) {
+            const float q = r - safe(m2);
+            s2 += __expf(q);
+            if (e != 0.f) u += e * (d - q);
+        }
+    }
+    // over `width` neighbouring lanes, all of which get the same bits
+    template <int WIDTH>
+    __device__ void join() {
+        float to = m, to2 = m2;
+        for (int d = WIDTH / 2; d > 0; d >>= 1) {
+            to = fmaxf(to, __shfl_xor(to, d, WAVE));
+            if (REF) to2 = fmaxf(to2, __shfl_xor(to2, d, WAVE));
+        }
+        rescale(to, to2);
+        for (int d = WIDTH / 2; d > 0; d >>= 1) {
+            s += __shfl_xor(s, d, WAVE);
+            w += __shfl_xor(w, d, WAVE);
             if (REF) {
-                const float q = (float)r[j] - x.m2;
-                x.s2 += __expf(q);
-                if (e != 0.f) x.u += e * (d - q);
+                s2 += __shfl_xor(s2, d, WAVE);
+                u += __shfl_xor(u, d, WAVE);
             }
         }
-    x.s = wave_reduce(x.s, Sum());
-    x.w = wave_reduce(x.w, Sum());
-    if (REF) {
-        x.s2 = wave_reduce(x.s2, Sum());
-        x.u = wave_reduce(x.u, Sum());
     }
-    return x;
-}
+};
 
-template <class E>
-__global__ void action_logprobs(procgen_amd_rows p, float *logp, float *entropy, float *lse) {
-    const int lane = threadIdx.x % WAVE;
-    const long long r = (long long)blockIdx.x * ROWS_PER_BLOCK + threadIdx.x / WAVE;
-    if (r >= p.rows) return;
-    const typename E::T *l = (const typename E::T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride);
-    const Stats x = row_stats<E, false>(l, nullptr, p.columns, lane);
-    if (lane) return;
-    const long long a = action_of(p, r);
-    const bool empty = x.m == -INFINITY, known = a >= 0 && a < p.columns;
-    const float log_s = logf(x.s);
-    logp[r] = !known ? NAN : empty ? -INFINITY : ((float)l[a] - x.m) - log_s;
-    entropy[r] = empty ? 0.f : log_s - x.w / x.s;
-    if (lse) lse[r] = empty ? -INFINITY : x.m + log_s;
-}
-
-template <class E>
-__global__ void action_logprobs_backward(procgen_amd_rows p, const float *lse, const float *entropy, const float *d_logp, const float *d_entropy) {
-    const int lane = threadIdx.x % WAVE;
-    const long long r = (long long)blockIdx.x * ROWS_PER_BLOCK + threadIdx.x / WAVE;
-    if (r >= p.rows) return;
-    const typename E::T *l = (const typename E::T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride);
-    typename E::T *d = (typename E::T *)p.d_logits + r * p.columns;
-    const float pick = d_logp ? d_logp[r] : 0.f, ent = d_entropy ? d_entropy[r] : 0.f, z = lse[r], H = entropy[r];
-    const long long a = action_of(p, r);
-    const bool known = a >= 0 && a < p.columns;
-    for (long long j = lane; j < p.columns; j += WAVE) {
-        float g = 0.f;
-        if (!(pick == 0.f && ent == 0.f) && z != -INFINITY) {
-            const float log_p = (float)l[j] - z, q = __expf(log_p);
-            g = (j == a ? pick : 0.f) - pick * q;
-            if (q != 0.f) g -= ent * q * (log_p + H);
-            if (!known) g = NAN;
+// what the rows add up to, and the gradient's coefficients of one row
+struct Sums {
+    double policy = 0, kl = 0, entropy = 0, clipped = 0;
+};
+struct Coef {
+    bool known;
+    float pick, kl, ent, KL, H;  // the formula's
+    float m, log_s, inv_s, m2, log_s2;
+    template <bool REF>
+    __device__ float gradient(float l, float r, bool taken) const {
+        const float d = l - m, p = __expf(d) * inv_s, log_p = d - log_s;
+        float g = (taken ? pick : 0.f) - pick * p;
+        if (p != 0.f) {
+            float f = ent * (log_p + H);
+            if (REF) f += kl * ((log_p - ((r - m2) - log_s2)) - KL);
+            g += p * f;
         }
-        d[j] = (typename E::T)g;
+        return known ? g : NAN;
+    }
+};
+
+// Each operator's rows: what it loads for a row, what it makes of the row's sums.  finish() is called once per row by one lane at least, with `first`
+// set in exactly one; it returns whether the row's gradient is anything but zero.
+struct Logprobs {
+    static constexpr bool GRADIENT = false, SUMS = false;
+    float *logp, *entropy, *lse;
+    __device__ void begin(const procgen_amd_rows &) {}
+    __device__ bool wanted(long long) const { return true; }
+    template <bool REF>
+    __device__ bool finish(long long r, const Stats<REF> &x, bool known, float l, bool first, Coef &, Sums &) const {
+        if (!first) return false;
+        const float log_s = logf(x.s), m = Stats<REF>::safe(x.m);
+        logp[r] = !known ? NAN : x.empty() ? -INFINITY : (l - m) - log_s;
+        entropy[r] = x.empty() ? 0.f : log_s - x.w / x.s;
+        if (lse) lse[r] = x.empty() ? -INFINITY : m + log_s;
+        return false;
+    }
+};
+
+struct LogprobsBackward {  // of rows short enough to sum up again
+    static constexpr bool GRADIENT = true, SUMS = false;
+    const float *d_logp, *d_entropy;
+    __device__ void begin(const procgen_amd_rows &) {}
+    __device__ bool wanted(long long r) const { return (d_logp && d_logp[r] != 0.f) || (d_entropy && d_entropy[r] != 0.f); }
+    template <bool REF>
+    __device__ bool finish(long long r, const Stats<REF> &x, bool known, float, bool, Coef &c, Sums &) const {
+        if (x.empty()) return false;
+        c.known = known;
+        c.m = Stats<REF>::safe(x.m);
+        c.log_s = logf(x.s);
+        c.inv_s = 1.f / x.s;
+        c.H = c.log_s - x.w / x.s;
+        c.pick = d_logp ? d_logp[r] : 0.f;
+        c.ent = d_entropy ? -d_entropy[r] : 0.f;
+        return true;
+    }
+};
+
+struct Policy {
+    static constexpr bool GRADIENT = true, SUMS = true;
+    procgen_amd_policy q;
+    const long long *counts;
+    int count_blocks;
+    long long n;
+    float scale;
+    __device__ void begin(const procgen_amd_rows &p) {
+        n = p.rows;
+        if (counts) {
+            n = 0;
+            for (int i = threadIdx.x % WAVE; i < count_blocks; i += WAVE) n += counts[i];
+            n = wave_reduce(n, Sum());
+        }
+        scale = (q.scale ? *q.scale : 1.f) * (n > 0 ? (float)(1.0 / (double)n) : 0.f);
+    }
+    __device__ bool wanted(long long r) const { return !q.valid || q.valid[r]; }
+    template <bool REF>
+    __device__ bool finish(long long r, const Stats<REF> &x, bool known, float l, bool first, Coef &c, Sums &sums) const {
+        if (x.empty()) return false;
+        c.known = known;
+        c.m = Stats<REF>::safe(x.m);
+        c.log_s = logf(x.s);
+        c.inv_s = 1.f / x.s;
+        c.H = c.log_s - x.w / x.s;
+        const float logp = known ? (l - c.m) - c.log_s : NAN, ratio = __expf(logp - q.old_logprobs[r]), adv = q.adv[r], lo = 1.f - q.clip_low, hi = 1.f + q.clip_high;
+        const float held = (ratio < lo ? lo : ratio > hi ? hi : ratio) * adv, plain = ratio * adv;
+        const bool out = plain > held;  // the clipped side is the smaller one and its gradient is zero; never where something is NaN
+        float pick = out ? 0.f : -plain, KL = 0.f;
+        if (REF) {
+            c.m2 = Stats<REF>::safe(x.m2);
+            c.log_s2 = logf(x.s2);
+            KL = x.s2 == 0.f ? INFINITY : x.u / x.s + logf(x.s2 / x.s);
+        } else if (q.ref_logprobs) {
+            const float d = q.ref_logprobs[r] - logp, f = expm1f(d);
+            KL = f - d;
+            pick -= q.kl_coef * f;
+        }
+        if (first) {
+            sums.policy -= out ? held : plain;
+            sums.kl += KL;
+            sums.entropy += c.H;
+            sums.clipped += ratio < lo || ratio > hi ? 1.0 : 0.0;
+        }
+        c.KL = KL;
+        c.pick = pick * scale;
+        c.kl = q.kl_coef * scale;
+        c.ent = q.entropy_coef * scale;
+        return true;
+    }
+};
+
+// the block's sums, in a fixed order
+__device__ inline void put_sums(Sums x, double *partial) {
+    __shared__ double part[BLOCK * 4 / WAVE][4];  // 1024 lanes at the most
+    double v[4] = {x.policy, x.kl, x.entropy, x.clipped};
+    for (int k = 0; k < 4; k++) v[k] = wave_reduce(v[k], Sum());
+    __syncthreads();
+    if (threadIdx.x % WAVE == 0)
+        for (int k = 0; k < 4; k++) part[threadIdx.x / WAVE][k] = v[k];
+    __syncthreads();
+    if (threadIdx.x < 4) {
+        double y = 0;
+        for (unsigned w = 0; w < blockDim.x / WAVE; w++) y += part[w][threadIdx.x];
+        partial[(long long)blockIdx.x * 4 + threadIdx.x] = y;
     }
 }
 
-// how many rows count: one partial sum per block, added up by every block that needs the number (whole numbers: any order gives the same)
-__global__ void count_valid(const uint8_t *valid, long long rows, long long *counts) {
+template <class E>
+struct Chunk {
+    static constexpr int N = 16 / sizeof(typename E::T);
+    typename E::T x[N];
+    // forgets what the compiler has made of the values: they are widened again where they are used next, and not held in 32 bits in between
+    __device__ void forget() {
+        uint32_t w[4];
+        __builtin_memcpy(w, x, 16);
+        asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
+        __builtin_memcpy(x, w, 16);
+    }
+    __device__ void load(const typename E::T *p) { __builtin_memcpy(x, p, 16); }  // from memory, whatever the alignment
+    __device__ void store(typename E::T *p) const { __builtin_memcpy(p, x, 16); }
+    __device__ void load_aligned(const typename E::T *p) { __builtin_memcpy(x, __builtin_assume_aligned(p, 16), 16); }  // from LDS
+    __device__ void store_aligned(typename E::T *p) const { __builtin_memcpy(__builtin_assume_aligned(p, 16), x, 16); }
+};
+
+// ---- up to 64 columns: a lane per row -------------------------------------------------------------------------------------------------------------
+
+// 64 rows between memory and LDS; `rows` of them exist.  Contiguous rows go 16 bytes a lane, others element by element.
+template <class E>
+__device__ inline void rows_to_lds(typename E::T *lds, const procgen_amd_rows &p, const void *from, long long outer, long long inner, long long r0, int rows, int lane) {
+    typedef typename E::T T;
+    const int columns = (int)p.columns, n = rows * columns;
+    if (p.inner == 1 && outer == columns) {
+        const T *src = (const T *)from + r0 * columns;
+        constexpr int N = Chunk<E>::N;
+        for (int i = lane * N; i < n; i += WAVE * N) {
+            if (i + N <= n) {
+                Chunk<E> c;
+                c.load(src + i);
+                c.store_aligned(lds + i);
+            } else {
+                for (int k = i; k < n; k++) lds[k] = src[k];
+            }
+        }
+    } else {
+        for (int i = lane; i < n; i += WAVE) {
+            const int r = i / columns;
+            lds[i] = ((const T *)from)[row_offset(p, r0 + r, outer, inner) + (i - r * columns)];
+        }
+    }
+}
+__device__ inline void lds_settled() {  // a wave's own LDS is written and read in order; this holds the compiler to it
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <class E, int MOST, bool REF, class Op>
+__global__ __launch_bounds__(BLOCK) void short_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
+    typedef typename E::T T;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), columns = (int)p.columns;
+    const int bytes = (WAVE * columns * (int)sizeof(T) + 15) & ~15;
+    T *const tile = (T *)(lds + (size_t)wave * bytes * (REF ? 2 : 1)), *const tile2 = (T *)((char *)tile + bytes);
+    op.begin(p);
+    Sums sums;
+    const long long step = (long long)gridDim.x * (BLOCK / WAVE) * WAVE;
+    for (long long r0 = ((long long)blockIdx.x * (BLOCK / WAVE) + wave) * WAVE; r0 < p.rows; r0 += step) {
+        const int rows = (int)min((long long)WAVE, p.rows - r0);
+        const bool mine = lane < rows;
+        const long long r = mine ? r0 + lane : r0;
+        const bool wanted = mine && op.wanted(r);
+        const long long a = action_of(p, r);
+        rows_to_lds<E>(tile, p, p.logits, p.outer_stride, p.inner_stride, r0, rows, lane);
+        if (REF) rows_to_lds<E>(tile2, p, ref, ref_outer, ref_inner, r0, rows, lane);
+        lds_settled();
+        T *const row = tile + lane * columns;
+        const T *const row2 = tile2 + lane * columns;
+        bool some = false;
+        Coef c;
+        if (wanted) {
+            float l[MOST], l2[REF ? MOST : 1];
+            Stats<REF> x;
+#pragma unroll
+            for (int j = 0; j < MOST; j++)
+                if (j < columns) {
+                    l[j] = (float)row[j];
+                    x.m = fmaxf(x.m, l[j]);
+                    if (REF) {
+                        l2[j] = (float)row2[j];
+                        x.m2 = fmaxf(x.m2, l2[j]);
+                    }
+                }
+#pragma unroll
+            for (int j = 0; j < MOST; j++)
+                if (j < columns) x.add(l[j], REF ? l2[j] : 0.f);
+            const bool known = a >= 0 && a < columns;
+            some = op.template finish<REF>(r, x, known, known ? (float)row[a] : 0.f, true, c, sums);
+            if (Op::GRADIENT && some && p.d_logits) {
+#pragma unroll
+                for (int j = 0; j < MOST; j++)
+                    if (j < columns) row[j] = (T)c.gradient<REF>(l[j], REF ? l2[j] : 0.f, j == a);
+            }
+        }
+        if (Op::GRADIENT && p.d_logits) {
+            if (!some)
+                for (int j = 0; j < columns; j++) row[j] = (T)0.f;
+            lds_settled();
+            T *const out = (T *)p.d_logits + r0 * columns;
+            const int n = rows * columns;
+            constexpr int N = Chunk<E>::N;
+            for (int i = lane * N; i < n; i += WAVE * N) {
+                if (i + N <= n) {
+                    Chunk<E> k;
+                    k.load_aligned(tile + i);
+                    k.store(out + i);
+                } else {
+                    for (int k = i; k < n; k++) out[k] = tile[k];
+                }
+            }
+            lds_settled();
+        }
+    }
+    if (Op::SUMS && partial) put_sums(sums, partial);
+}
+
+// ---- more columns: a group of G lanes per row -----------------------------------------------------------------------------------------------------
+
+template <class E, int G, int CH, bool REF, class Op>
+__global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
+    typedef typename E::T T;
+    constexpr int N = Chunk<E>::N, THREADS = G > BLOCK ? G : BLOCK, PER_BLOCK = THREADS / G, SPAN = G * CH * N;  // columns of a batch
+    const int g = threadIdx.x % G, lane = threadIdx.x % WAVE;
+    __shared__ float wave_stats[2][G > WAVE ? G / WAVE : 1][6];
+    op.begin(p);
+    Sums sums;
+    const int columns = (int)p.columns, batches = (columns + SPAN - 1) / SPAN;
+    int odd = 0;
+    for (long long r = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / G; r < p.rows; r += (long long)gridDim.x * PER_BLOCK) {
+        const T *const row = (const T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride);
+        const T *const row2 = REF ? (const T *)ref + row_offset(p, r, ref_outer, ref_inner) : nullptr;
+        T *const out = Op::GRADIENT && p.d_logits ? (T *)p.d_logits + r * p.columns : nullptr;
+        bool some = false;
+        Chunk<E> l[CH], l2[REF ? CH : 1];
+        // Columns [at(b, i), + N) are chunk i of batch b.  The last one of a row reaches back so that it ends with the row: what it shares with its
+        // neighbour counts as -inf here and is not written.  Chunks behind the row are all -inf.
+        auto at = [&](int b, int i) { return b * SPAN + (i * G + g) * N; };
+        auto load = [&](int b) {
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                const int j = min(at(b, i), columns - N);
+                l[i].load(row + j);
+                if (REF) l2[i].load(row2 + j);
+            }
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                const int shared = at(b, i) - (columns - N);
+                if (shared > 0)
+                    for (int k = 0; k < N; k++)
+                        if (k < shared) {
+                            l[i].x[k] = (T)-INFINITY;
+                            if (REF) l2[i].x[k] = (T)-INFINITY;
+                        }
+            }
+        };
+        auto forget = [&] {
+            for (int i = 0; i < CH; i++) {
+                l[i].forget();
+                if (REF) l2[i].forget();
+            }
+        };
+        Coef c;
+        long long a = 0;
+        if (op.wanted(r)) {  // the same for the whole group
+            a = action_of(p, r);
+            const bool known = a >= 0 && a < columns;
+            const float taken = (float)row[known ? a : 0];
+            Stats<REF> x;
+            for (int b = 0; b < batches; b++) {
+                load(b);
+                float to = x.m, to2 = x.m2;
+#pragma unroll
+                for (int i = 0; i < CH; i++)
+                    for (int k = 0; k < N; k++) {
+                        to = fmaxf(to, (float)l[i].x[k]);
+                        if (REF) to2 = fmaxf(to2, (float)l2[i].x[k]);
+                    }
+                x.rescale(to, to2);
+                forget();
+#pragma unroll
+                for (int i = 0; i < CH; i++)
+                    for (int k = 0; k < N; k++) x.add((float)l[i].x[k], REF ? (float)l2[i].x[k] : 0.f);
+            }
+            x.template join<(G < WAVE ? G : WAVE)>();
+            if (G > WAVE) {
+                if (lane == 0) x.put(wave_stats[odd][threadIdx.x / WAVE]);
+                __syncthreads();
+                x = Stats<REF>();
+                if (lane < G / WAVE) x.get(wave_stats[odd][lane]);
+                x.template join<(G > WAVE ? G / WAVE : 1)>();
+                // lanes beyond the first G / WAVE hold no wave's sums: they take the first one's
+                x.m = __shfl(x.m, 0, WAVE), x.s = __shfl(x.s, 0, WAVE), x.w = __shfl(x.w, 0, WAVE);
+                if (REF) x.m2 = __shfl(x.m2, 0, WAVE), x.s2 = __shfl(x.s2, 0, WAVE), x.u = __shfl(x.u, 0, WAVE);
+                odd ^= 1;
+            }
+            some = op.template finish<REF>(r, x, known, taken, g == 0, c, sums);
+            forget();
+        }
+        if (!Op::GRADIENT || !out) continue;
+        for (int b = batches - 1; b >= 0; b--) {
+            if (some && b < batches - 1) load(b);
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                const int j = min(at(b, i), columns - N), shared = at(b, i) - j;
+                Chunk<E> d;
+                for (int k = 0; k < N; k++) d.x[k] = some ? (T)c.gradient<REF>((float)l[i].x[k], REF ? (float)l2[i].x[k] : 0.f, j + k == a) : (T)0.f;
+                if (shared == 0) {
+                    d.store(out + j);
+                } else {
+                    for (int k = 0; k < N; k++)
+                        if (k >= shared) out[j + k] = d.x[k];
+                }
+            }
+        }
+    }
+    if (Op::SUMS && partial) put_sums(sums, partial);
+}
+
+// the gradient of long rows' log-probabilities: lse and entropy are known, so every column stands for itself
+template <class E>
+__global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, const float *lse, const float *entropy, const float *d_logp, const float *d_entropy) {
+    typedef typename E::T T;
+    constexpr int N = Chunk<E>::N;
+    const int columns = (int)p.columns;
+    const long long j = ((long long)blockIdx.x * BLOCK + threadIdx.x) * N;
+    if (j >= columns) return;
+    for (long long r = blockIdx.y; r < p.rows; r += gridDim.y) {
+        const T *const row = (const T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride);
+        T *const out = (T *)p.d_logits + r * p.columns;
+        const long long a = action_of(p, r);
+        Coef c;
+        c.known = a >= 0 && a < columns;
+        c.pick = d_logp ? d_logp[r] : 0.f;
+        c.ent = d_entropy ? -d_entropy[r] : 0.f;
+        c.H = entropy[r];
+        c.m = lse[r];
+        c.log_s = 0.f;
+        c.inv_s = 1.f;
+        const bool some = !(c.pick == 0.f && c.ent == 0.f) && c.m != -INFINITY;
+        Chunk<E> x;
+        const bool whole = j + N <= columns;
+        if (whole) {
+            x.load(row + j);
+        } else {
+            for (int k = 0; k < N; k++) x.x[k] = j + k < columns ? row[j + k] : (T)0.f;
+        }
+        for (int k = 0; k < N; k++) x.x[k] = some ? (T)c.gradient<false>((float)x.x[k], 0.f, j + k == a) : (T)0.f;
+        if (whole) {
+            x.store(out + j);
+        } else {
+            for (int k = 0; k < N; k++)
+                if (j + k < columns) out[j + k] = x.x[k];
+        }
+    }
+}
+
+// ---- the mean ------------------------------------------------------------------------------------------------------------------------------------
+
+// how many rows count: one partial sum per block, added up by every wave that needs the number (whole numbers: any order gives the same)
+__global__ __launch_bounds__(BLOCK) void count_valid(const uint8_t *valid, long long rows, long long *counts) {
     long long n = 0;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows; i += (long long)gridDim.x * blockDim.x) n += valid[i] != 0;
+    const long long head = min(rows, (long long)(-(uintptr_t)valid & 15)), wide = (rows - head) / 16;  // bytes before the first aligned 16, and 16s
+    const long long i = (long long)blockIdx.x * BLOCK + threadIdx.x, step = (long long)gridDim.x * BLOCK;
+    for (long long k = i; k < wide; k += step) {
+        const uint4 v = ((const uint4 *)(valid + head))[k];
+        const unsigned x[4] = {v.x, v.y, v.z, v.w};
+        for (int w = 0; w < 4; w++)
+            for (int b = 0; b < 32; b += 8) n += (x[w] >> b & 0xff) != 0;
+    }
+    for (long long k = i; k < rows - wide * 16; k += step) n += valid[k < head ? k : k + wide * 16] != 0;
     n = wave_reduce(n, Sum());
-    __shared__ long long part[4];
+    __shared__ long long part[BLOCK / WAVE];
     if (threadIdx.x % WAVE == 0) part[threadIdx.x / WAVE] = n;
     __syncthreads();
     if (threadIdx.x == 0) counts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
-struct Coef {
-    float pick, policy, kl, entropy, clipped;  // d loss / d logp of the action taken; the row's terms
-};
-template <bool REF>
-__device__ inline Coef row_coef(const procgen_amd_policy &q, long long r, const Stats &x, float log_s, float logp) {
-    Coef c;
-    c.entropy = log_s - x.w / x.s;
-    const float ratio = expf(logp - q.old_logprobs[r]), adv = q.adv[r], lo = 1.f - q.clip_low, hi = 1.f + q.clip_high;
-    const float held = (ratio < lo ? lo : ratio > hi ? hi : ratio) * adv, plain = ratio * adv;
-    const bool out = plain > held;  // the clipped side is the smaller one (and its gradient is zero); never where something is NaN
-    c.policy = -(out ? held : plain);
-    c.pick = out ? 0.f : -plain;
-    c.clipped = ratio < lo || ratio > hi ? 1.f : 0.f;
-    c.kl = 0.f;
-    if (REF) c.kl = x.s2 > 0.f || x.s2 != x.s2 ? x.u / x.s + logf(x.s2 / x.s) : INFINITY;
-    else if (q.ref_logprobs) {
-        const float d = q.ref_logprobs[r] - logp;
-        c.kl = expm1f(d) - d;
-        c.pick -= q.kl_coef * expm1f(d);
-    }
-    return c;
-}
-
-template <class E, bool REF>
-__global__ void policy_rows(procgen_amd_rows p, procgen_amd_policy q, const long long *counts, int count_blocks, double *partial) {
-    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
-    long long n = p.rows;
-    if (counts) {
-        n = 0;
-        for (int i = lane; i < count_blocks; i += WAVE) n += counts[i];
-        n = wave_reduce(n, Sum());
-    }
-    const float scale = (q.scale ? *q.scale : 1.f) * (n > 0 ? (float)(1.0 / (double)n) : 0.f);
-    double sum[4] = {0, 0, 0, 0};
-    for (long long r = (long long)blockIdx.x * ROWS_PER_BLOCK + wave; r < p.rows; r += (long long)gridDim.x * ROWS_PER_BLOCK) {
-        const typename E::T *l = (const typename E::T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride);
-        const typename E::T *l2 = REF ? (const typename E::T *)q.ref_logits + row_offset(p, r, q.ref_outer_stride, q.ref_inner_stride) : nullptr;
-        typename E::T *d = p.d_logits ? (typename E::T *)p.d_logits + r * p.columns : nullptr;
-        const bool used = !q.valid || q.valid[r];
-        Stats x;
-        if (used) x = row_stats<E, REF>(l, l2, p.columns, lane);
-        if (!used || x.m == -INFINITY) {
-            if (d)
-                for (long long j = lane; j < p.columns; j += WAVE) d[j] = (typename E::T)0.f;
-            continue;
-        }
-        const long long a = action_of(p, r);
-        const bool known = a >= 0 && a < p.columns;
-        const float log_s = logf(x.s), logp = known ? ((float)l[a] - x.m) - log_s : NAN;
-        const Coef c = row_coef<REF>(q, r, x, log_s, logp);
-        if (lane == 0) {
-            sum[0] += c.policy;
-            sum[1] += c.kl;
-            sum[2] += c.entropy;
-            sum[3] += c.clipped;
-        }
-        if (d) {
-            const float inv_s = 1.f / x.s, log_s2 = REF ? logf(x.s2) : 0.f;
-            for (long long j = lane; j < p.columns; j += WAVE) {
-                const float dl = (float)l[j] - x.m, pj = __expf(dl) * inv_s, log_p = dl - log_s;
-                float g = (j == a ? c.pick : 0.f) - c.pick * pj;
-                if (pj != 0.f) {
-                    float f = q.entropy_coef * (log_p + c.entropy);
-                    if (REF) f += q.kl_coef * ((log_p - (((float)l2[j] - x.m2) - log_s2)) - c.kl);
-                    g += pj * f;
-                }
-                d[j] = (typename E::T)(known ? g * scale : NAN);
-            }
-        }
-    }
-    if (!partial) return;
-    __shared__ double part[ROWS_PER_BLOCK][4];
-    if (lane == 0)
-        for (int k = 0; k < 4; k++) part[wave][k] = sum[k];
+__global__ __launch_bounds__(BLOCK) void policy_means(procgen_amd_policy q, long long rows, const long long *counts, int count_blocks, const double *partial, int blocks) {
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, k = lane % 4;  // four neighbouring lanes: a block's four sums
+    double v = 0;
+    for (int i = threadIdx.x / 4; i < blocks; i += BLOCK / 4) v += partial[(long long)i * 4 + k];
+    for (int d = WAVE / 2; d >= 4; d >>= 1) v += __shfl_xor(v, d, WAVE);
+    __shared__ double part[BLOCK / WAVE][4];
+    if (lane < 4) part[wave][lane] = v;
     __syncthreads();
-    if (threadIdx.x < 4) {
-        double v = 0;
-        for (int w = 0; w < ROWS_PER_BLOCK; w++) v += part[w][threadIdx.x];
-        partial[(long long)blockIdx.x * 4 + threadIdx.x] = v;
-    }
-}
-
-__global__ void policy_means(procgen_amd_policy q, long long rows, const long long *counts, int count_blocks, const double *partial, int blocks) {
-    const int lane = threadIdx.x % WAVE, k = threadIdx.x / WAVE;  // wave k: the k-th mean
+    if (wave) return;
     long long n = rows;
     if (counts) {
         n = 0;
         for (int i = lane; i < count_blocks; i += WAVE) n += counts[i];
         n = wave_reduce(n, Sum());
     }
-    double v = 0;
-    for (int i = lane; i < blocks; i += WAVE) v += partial[(long long)i * 4 + k];
-    v = wave_reduce(v, Sum());
-    __shared__ double mean[4];
-    if (lane == 0) mean[k] = n > 0 ? v / (double)n : 0.0;
-    __syncthreads();
-    if (threadIdx.x == 0) *q.loss = (float)(mean[0] + (q.kl_coef != 0.f ? (double)q.kl_coef * mean[1] : 0.0) - (q.entropy_coef != 0.f ? (double)q.entropy_coef * mean[2] : 0.0));
-    if (lane == 0) q.stats[k] = (float)mean[k];
+    double mean[4];
+    for (int i = 0; i < 4; i++) mean[i] = n > 0 ? (part[0][i] + part[1][i] + part[2][i] + part[3][i]) / (double)n : 0.0;
+    if (lane == 0) *q.loss = (float)(mean[0] + (q.kl_coef != 0.f ? (double)q.kl_coef * mean[1] : 0.0) - (q.entropy_coef != 0.f ? (double)q.entropy_coef * mean[2] : 0.0));
+    if (lane < 4) q.stats[lane] = (float)mean[lane];
 }
 
-bool rows_ok(const procgen_amd_rows *p) { return p && known_dtype(p->dtype) && p->rows >= 0 && p->columns >= 1 && p->columns <= 0x7fffffffll && p->inner >= 1; }
-constexpr int MAX_ROW_BLOCKS = 2048;
-unsigned row_blocks(long long rows) { return (unsigned)((rows + ROWS_PER_BLOCK - 1) / ROWS_PER_BLOCK); }
+// ---- launches ------------------------------------------------------------------------------------------------------------------------------------
+
+bool rows_ok(const procgen_amd_rows *p) {
+    return p && known_dtype(p->dtype) && p->rows >= 0 && p->rows <= 0x7fffff00ll && p->columns >= 1 && p->columns <= 0x7ffffff0ll - (1 << 18) && p->inner >= 1;
+}
+
+// one kernel over all rows; returns the blocks it was launched with (the partial sums), or -1 - error
+template <class E, bool REF, class Op>
+int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long long ref_outer, long long ref_inner, double *partial, hipStream_t stream) {
+    int blocks = 0;
+    auto grid = [&](int per_block, int most) { return blocks = (int)std::min<long long>(most, (p.rows + per_block - 1) / per_block); };
+    constexpr int N = Chunk<E>::N;
+    if (p.columns <= 64) {
+        const size_t lds = ((WAVE * p.columns * sizeof(typename E::T) + 15) & ~15ull) * (BLOCK / WAVE) * (REF ? 2 : 1);
+        if (p.columns <= 16) short_rows<E, 16, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if (p.columns <= 32) short_rows<E, 32, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else short_rows<E, 64, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (p.columns <= 16 * 2 * N) {
+        long_rows<E, 16, 2, REF, Op><<<grid(BLOCK / 16, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (p.columns <= 64 * 2 * N) {
+        long_rows<E, 64, 2, REF, Op><<<grid(BLOCK / 64, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (p.columns <= 256 * 4 * N) {
+        long_rows<E, 256, 4, REF, Op><<<grid(1, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else {
+        long_rows<E, 1024, 4, REF, Op><<<grid(1, MAX_BLOCKS / 4), 1024, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    }
+    const int err = launched();
+    return err ? -1 - err : blocks;
+}
 
 }  // namespace
 }  // namespace learner
@@ -218,56 +551,62 @@ using namespace pgamd::learner;
 
 extern "C" {
 
-LIBENV_API long long procgen_amd_rows_workspace(long long rows, long long columns) { return MAX_COUNT_BLOCKS * (long long)sizeof(long long) + MAX_ROW_BLOCKS * 4ll * (long long)sizeof(double); }
+LIBENV_API long long procgen_amd_rows_workspace(long long rows, long long columns) { return MAX_COUNT_BLOCKS * (long long)sizeof(long long) + MAX_BLOCKS * 4ll * (long long)sizeof(double); }
 
 LIBENV_API int procgen_amd_action_logprobs(const struct procgen_amd_rows *p, float *logp, float *entropy, float *lse, int device, void *stream) {
-    if (!rows_ok(p) || p->rows > 0x7fffffffll) return -1;
+    if (!rows_ok(p)) return -1;
     if (p->rows == 0) return 0;
     if (!p->logits || !p->actions || !logp || !entropy) return -1;
     OnDevice on(device);
     if (on.err != hipSuccess) return (int)on.err;
-    return by_dtype(p->dtype, [&](auto e) {
-        action_logprobs<decltype(e)><<<row_blocks(p->rows), 256, 0, (hipStream_t)stream>>>(*p, logp, entropy, lse);
-        return launched();
-    });
+    const int got = by_dtype(p->dtype, [&](auto e) { return launch_rows<decltype(e), false>(*p, Logprobs{logp, entropy, lse}, nullptr, 0, 0, nullptr, (hipStream_t)stream); });
+    return got < 0 ? -1 - got : 0;
 }
 
 LIBENV_API int procgen_amd_action_logprobs_backward(const struct procgen_amd_rows *p, const float *lse, const float *entropy, const float *d_logp, const float *d_entropy, int device, void *stream) {
-    if (!rows_ok(p) || p->rows > 0x7fffffffll) return -1;
+    if (!rows_ok(p)) return -1;
     if (p->rows == 0) return 0;
     if (!p->logits || !p->actions || !p->d_logits || !lse || !entropy) return -1;
     OnDevice on(device);
     if (on.err != hipSuccess) return (int)on.err;
     return by_dtype(p->dtype, [&](auto e) {
-        action_logprobs_backward<decltype(e)><<<row_blocks(p->rows), 256, 0, (hipStream_t)stream>>>(*p, lse, entropy, d_logp, d_entropy);
+        typedef decltype(e) E;
+        if (p->columns <= 64) {
+            const int got = launch_rows<E, false>(*p, LogprobsBackward{d_logp, d_entropy}, nullptr, 0, 0, nullptr, (hipStream_t)stream);
+            return got < 0 ? -1 - got : 0;
+        }
+        const long long chunks = (p->columns + Chunk<E>::N - 1) / Chunk<E>::N;
+        const dim3 grid((unsigned)((chunks + BLOCK - 1) / BLOCK), (unsigned)std::min<long long>(p->rows, 65535));
+        logprobs_gradient<E><<<grid, BLOCK, 0, (hipStream_t)stream>>>(*p, lse, entropy, d_logp, d_entropy);
         return launched();
     });
 }
 
 LIBENV_API int procgen_amd_policy_loss(const struct procgen_amd_rows *p, const struct procgen_amd_policy *q, int device, void *stream) {
-    if (!rows_ok(p) || !q || p->rows > 0x7fffffffll || (q->ref_logits && q->ref_logprobs) || !p->workspace || !q->loss != !q->stats) return -1;
+    if (!rows_ok(p) || !q || (q->ref_logits && q->ref_logprobs) || !p->workspace || !q->loss != !q->stats) return -1;
     if (p->rows > 0 && (!p->logits || !p->actions || !q->old_logprobs || !q->adv)) return -1;
     OnDevice on(device);
     if (on.err != hipSuccess) return (int)on.err;
     long long *counts = q->valid ? (long long *)p->workspace : nullptr;
     double *partial = (double *)((long long *)p->workspace + MAX_COUNT_BLOCKS);
-    int count_blocks = 0, blocks = 0, err = 0;
+    int count_blocks = 0, blocks = 0;
     if (p->rows > 0) {
         if (counts) {
-            count_blocks = (int)std::min<long long>(MAX_COUNT_BLOCKS, (p->rows + 4095) / 4096);
-            count_valid<<<count_blocks, 256, 0, (hipStream_t)stream>>>(q->valid, p->rows, counts);
-            if ((err = launched())) return err;
+            count_blocks = (int)std::min<long long>(MAX_COUNT_BLOCKS, (p->rows + 16 * BLOCK - 1) / (16 * BLOCK));
+            count_valid<<<count_blocks, BLOCK, 0, (hipStream_t)stream>>>(q->valid, p->rows, counts);
+            if (int err = launched()) return err;
         }
-        blocks = (int)std::min<long long>(MAX_ROW_BLOCKS, row_blocks(p->rows));
-        err = by_dtype(p->dtype, [&](auto e) {
-            if (q->ref_logits) policy_rows<decltype(e), true><<<blocks, 256, 0, (hipStream_t)stream>>>(*p, *q, counts, count_blocks, q->loss ? partial : nullptr);
-            else policy_rows<decltype(e), false><<<blocks, 256, 0, (hipStream_t)stream>>>(*p, *q, counts, count_blocks, q->loss ? partial : nullptr);
-            return launched();
+        blocks = by_dtype(p->dtype, [&](auto e) {
+            typedef decltype(e) E;
+            const Policy op{*q, counts, count_blocks, 0, 0.f};
+            double *to = q->loss ? partial : nullptr;
+            if (q->ref_logits) return launch_rows<E, true>(*p, op, q->ref_logits, q->ref_outer_stride, q->ref_inner_stride, to, (hipStream_t)stream);
+            return launch_rows<E, false>(*p, op, nullptr, 0, 0, to, (hipStream_t)stream);
         });
-        if (err) return err;
+        if (blocks < 0) return -1 - blocks;
     }
     if (!q->loss) return 0;
-    policy_means<<<1, 256, 0, (hipStream_t)stream>>>(*q, p->rows, counts, count_blocks, partial, blocks);
+    policy_means<<<1, BLOCK, 0, (hipStream_t)stream>>>(*q, p->rows, counts, count_blocks, partial, blocks);
     return launched();
 }
 
