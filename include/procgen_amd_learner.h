@@ -99,7 +99,9 @@ LIBENV_API int procgen_amd_action_logprobs_backward(const struct procgen_amd_row
  *       or its estimator exp(d) - d - 1, d = ref_logprobs - logp;  or 0 when neither is given
  *     loss = mean over the rows with valid != 0 of  -objective + kl_coef * KL - entropy_coef * entropy       (0 when there is none)
  * Rows with valid == 0 are not looked at and get a zero gradient.  stats: float [4], the means of -objective, KL, entropy and of (ratio outside
- * the clip range).  d_logits of the rows: NULL, or written with the gradient of scale * loss; scale: device float, NULL = 1. */
+ * the clip range).  d_logits of the rows: NULL, or written with the gradient of scale * loss; scale: device float, NULL = 1.
+ * resume: not 0 for a second call on the same rows and workspace, whose first one had scale = NULL and a d_logits: the workspace's count of valid rows
+ * is used again, and bit 1 says that d_logits is the first call's own, so that nothing is to be done where *scale is 1. */
 struct procgen_amd_policy {
     const float *old_logprobs, *adv;              /* [rows] */
     const uint8_t *valid;                         /* [rows] or NULL */
@@ -109,7 +111,11 @@ struct procgen_amd_policy {
     float clip_low, clip_high, kl_coef, entropy_coef;
     const float *scale;
     float *loss, *stats;                          /* both NULL: only the gradient */
+    int resume;                                   /* 0, 1, or 1 | 2 */
 };
+/* the graph capture that the stream is in: its id, 0 when there is none, -1 when the runtime cannot say.  (bit 1 of resume holds within one capture, or
+ * for one call outside of any: a replay of the second call alone would find what its last run left in d_logits.) */
+LIBENV_API long long procgen_amd_capture_id(void *stream);
 LIBENV_API int procgen_amd_policy_loss(const struct procgen_amd_rows *rows, const struct procgen_amd_policy *policy, int device, void *stream);
 
 #ifdef __cplusplus

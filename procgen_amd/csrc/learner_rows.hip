@@ -113,6 +113,7 @@ struct Coef {
 // set in exactly one; it returns whether the row's gradient is anything but zero.
 struct Logprobs {
     static constexpr bool GRADIENT = false, SUMS = false;
+    __device__ bool done() const { return false; }
     float *logp, *entropy, *lse;
     __device__ void begin(const procgen_amd_rows &) {}
     __device__ bool wanted(long long) const { return true; }
@@ -129,6 +130,7 @@ struct Logprobs {
 
 struct LogprobsBackward {  // of rows short enough to sum up again
     static constexpr bool GRADIENT = true, SUMS = false;
+    __device__ bool done() const { return false; }
     const float *d_logp, *d_entropy;
     __device__ void begin(const procgen_amd_rows &) {}
     __device__ bool wanted(long long r) const { return (d_logp && d_logp[r] != 0.f) || (d_entropy && d_entropy[r] != 0.f); }
@@ -148,6 +150,7 @@ struct LogprobsBackward {  // of rows short enough to sum up again
 
 struct Policy {
     static constexpr bool GRADIENT = true, SUMS = true;
+    __device__ bool done() const { return (q.resume & 2) && *q.scale == 1.f; }  // the gradient that is there is the one that is wanted
     procgen_amd_policy q;
     const long long *counts;
     int count_blocks;
@@ -269,6 +272,7 @@ __global__ __launch_bounds__(BLOCK) void short_rows(procgen_amd_rows p, Op op, c
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), columns = (int)p.columns;
     const int bytes = (WAVE * columns * (int)sizeof(T) + 15) & ~15;
     T *const tile = (T *)(lds + (size_t)wave * bytes * (REF ? 2 : 1)), *const tile2 = (T *)((char *)tile + bytes);
+    if (op.done()) return;
     op.begin(p);
     Sums sums;
     const long long step = (long long)gridDim.x * (BLOCK / WAVE) * WAVE;
@@ -339,6 +343,7 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
     constexpr int N = Chunk<E>::N, THREADS = G > BLOCK ? G : BLOCK, PER_BLOCK = THREADS / G, SPAN = G * CH * N;  // columns of a batch
     const int g = threadIdx.x % G, lane = threadIdx.x % WAVE;
     __shared__ float wave_stats[2][G > WAVE ? G / WAVE : 1][6];
+    if (op.done()) return;
     op.begin(p);
     Sums sums;
     const int columns = (int)p.columns, batches = (columns + SPAN - 1) / SPAN;
@@ -582,8 +587,18 @@ LIBENV_API int procgen_amd_action_logprobs_backward(const struct procgen_amd_row
     });
 }
 
+LIBENV_API long long procgen_amd_capture_id(void *stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return -1;
+    }
+    return status == hipStreamCaptureStatusActive ? (long long)id : 0;
+}
+
 LIBENV_API int procgen_amd_policy_loss(const struct procgen_amd_rows *p, const struct procgen_amd_policy *q, int device, void *stream) {
-    if (!rows_ok(p) || !q || (q->ref_logits && q->ref_logprobs) || !p->workspace || !q->loss != !q->stats) return -1;
+    if (!rows_ok(p) || !q || (q->ref_logits && q->ref_logprobs) || !p->workspace || !q->loss != !q->stats || (q->resume && (q->loss || !q->scale || (p->rows > 0 && !p->d_logits)))) return -1;
     if (p->rows > 0 && (!p->logits || !p->actions || !q->old_logprobs || !q->adv)) return -1;
     OnDevice on(device);
     if (on.err != hipSuccess) return (int)on.err;
@@ -593,8 +608,10 @@ LIBENV_API int procgen_amd_policy_loss(const struct procgen_amd_rows *p, const s
     if (p->rows > 0) {
         if (counts) {
             count_blocks = (int)std::min<long long>(MAX_COUNT_BLOCKS, (p->rows + 16 * BLOCK - 1) / (16 * BLOCK));
-            count_valid<<<count_blocks, BLOCK, 0, (hipStream_t)stream>>>(q->valid, p->rows, counts);
-            if (int err = launched()) return err;
+            if (!q->resume) {
+                count_valid<<<count_blocks, BLOCK, 0, (hipStream_t)stream>>>(q->valid, p->rows, counts);
+                if (int err = launched()) return err;
+            }
         }
         blocks = by_dtype(p->dtype, [&](auto e) {
             typedef decltype(e) E;

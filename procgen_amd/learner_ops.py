@@ -52,7 +52,7 @@ class _Rows(C.Structure):  # struct procgen_amd_rows
 class _Policy(C.Structure):  # struct procgen_amd_policy
     _fields_ = [("old_logprobs", C.c_void_p), ("adv", C.c_void_p), ("valid", C.c_void_p), ("ref_logits", C.c_void_p), ("ref_outer_stride", C.c_longlong),
                 ("ref_inner_stride", C.c_longlong), ("ref_logprobs", C.c_void_p), ("clip_low", C.c_float), ("clip_high", C.c_float), ("kl_coef", C.c_float),
-                ("entropy_coef", C.c_float), ("scale", C.c_void_p), ("loss", C.c_void_p), ("stats", C.c_void_p)]
+                ("entropy_coef", C.c_float), ("scale", C.c_void_p), ("loss", C.c_void_p), ("stats", C.c_void_p), ("resume", C.c_int)]
 
 
 class _Library:
@@ -67,7 +67,7 @@ class _Library:
             P, I, L = C.c_void_p, C.c_int, C.c_longlong
             for fn, res, args in (("recurrence_checkpoints", L, [I]), ("recurrence_workspace", L, [I, I, I]), ("recurrence_forward", I, [P, I, P]),
                                   ("recurrence_backward", I, [P, I, P]), ("advantages", I, [P, I, P]), ("rows_workspace", L, [L, L]),
-                                  ("action_logprobs", I, [P, P, P, P, I, P]), ("action_logprobs_backward", I, [P, P, P, P, P, I, P]), ("policy_loss", I, [P, P, I, P])):
+                                  ("action_logprobs", I, [P, P, P, P, I, P]), ("action_logprobs_backward", I, [P, P, P, P, P, I, P]), ("policy_loss", I, [P, P, I, P]), ("capture_id", L, [P])):
                 f = getattr(lib, "procgen_amd_" + fn)
                 f.restype, f.argtypes = res, args
                 setattr(self, fn, f)
@@ -346,31 +346,42 @@ class PolicyLoss(NamedTuple):
     stats: torch.Tensor  # float32 [4]: the means of -objective, KL, entropy and of (ratio outside the clip range), constants
 
 
-def _policy_args(coefs, logits, actions, old, adv, valid, ref_logits, ref_logprobs):
+def _policy_args(coefs, work, logits, actions, old, adv, valid, ref_logits, ref_logprobs):
     a = _rows(logits, actions)
+    a.workspace = work.data_ptr()
     clip, kl_coef, entropy_coef = coefs
     q = _Policy(old.data_ptr(), adv.data_ptr(), _ptr(valid), _ptr(ref_logits), 0, 0, _ptr(ref_logprobs), *clip, kl_coef, entropy_coef)
     if ref_logits is not None:
         (a.inner, a.outer_stride, a.inner_stride), (_, q.ref_outer_stride, q.ref_inner_stride) = _common_layout(logits, ref_logits)
-    work = _bytes(_lib.rows_workspace(a.rows, a.columns), logits.device)
-    a.workspace = work.data_ptr()
-    return a, q, work
+    return a, q
 
 
-def _policy_forward(coefs, *tensors):
-    device = tensors[0].device
+def _policy_forward(coefs, d_logits, *tensors):
+    logits = tensors[0]
+    device, columns = logits.device, logits.shape[-1]
     loss, stats = torch.empty((), dtype=torch.float32, device=device), torch.empty(4, dtype=torch.float32, device=device)
-    a, q, work = _policy_args(coefs, *tensors)
-    q.loss, q.stats = loss.data_ptr(), stats.data_ptr()
+    work = _bytes(_lib.rows_workspace(logits.numel() // columns, columns), device)
+    a, q = _policy_args(coefs, work, *tensors)
+    a.d_logits, q.loss, q.stats = _ptr(d_logits), loss.data_ptr(), stats.data_ptr()
     _run(_lib.policy_loss, "policy_loss", device, C.addressof(a), C.addressof(q))
-    return loss, stats
+    return loss, stats, work
+
+
+def _capture(device):
+    return _lib.capture_id(torch.cuda.current_stream(device).cuda_stream)
 
 
 class _PolicyLoss(torch.autograd.Function):
+    """The forward call writes the gradient too, from the row that it has in registers.  The first backward pass hands it out, after a kernel that goes
+    over the rows again only where the loss's own gradient is not 1; each further one (retain_graph)
+    computes its own, and so does a backward pass that is captured apart from its forward call."""
+
     @staticmethod
     def forward(ctx, coefs, *tensors):
-        loss, stats = _policy_forward(coefs, *tensors)
-        ctx.coefs = coefs
+        logits = tensors[0]
+        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        loss, stats, ctx.work = _policy_forward(coefs, d_logits, *tensors)
+        ctx.coefs, ctx.d_logits, ctx.capture = coefs, d_logits, _capture(logits.device)
         ctx.save_for_backward(*tensors)
         ctx.mark_non_differentiable(stats)
         return loss, stats
@@ -379,8 +390,13 @@ class _PolicyLoss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_loss, _):
         logits = ctx.saved_tensors[0]
-        a, q, work = _policy_args(ctx.coefs, *ctx.saved_tensors)
-        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        d_logits, ctx.d_logits = ctx.d_logits, None
+        a, q = _policy_args(ctx.coefs, ctx.work, *ctx.saved_tensors)
+        q.resume = 1
+        if d_logits is not None and ctx.capture == _capture(logits.device) >= 0:
+            q.resume = 3
+        else:
+            d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         a.d_logits, q.scale = d_logits.data_ptr(), d_loss.data_ptr()
         _run(_lib.policy_loss, "policy_loss", logits.device, C.addressof(a), C.addressof(q))
         return (None, d_logits) + (None,) * 6
@@ -444,4 +460,4 @@ def policy_loss(logits, actions, old_logprobs, advantages, *, clip=0.2, kl_coef=
     actions, old_logprobs, advantages, valid, ref_logprobs = (None if x is None else x.contiguous() for x in (actions, old_logprobs, advantages, valid, ref_logprobs))
     coefs = (float(low), float(high)), float(kl_coef), float(entropy_coef)
     tensors = logits, actions, old_logprobs, advantages, valid, ref_logits, ref_logprobs
-    return PolicyLoss(*(_PolicyLoss.apply(coefs, *tensors) if _wants_grad(logits) else _policy_forward(coefs, *tensors)))
+    return PolicyLoss(*(_PolicyLoss.apply(coefs, *tensors) if _wants_grad(logits) else _policy_forward(coefs, None, *tensors)[:2]))
