@@ -4,7 +4,9 @@
 // With m = max l, e[j] = exp(l[j] - m), s = sum e:  p[j] = e[j] / s,  log p[j] = (l[j] - m) - log s,  H = log s - (sum e (l - m)) / s, and against a
 // reference row r (m', s' alike)  KL = (sum e ((l - m) - (r - m'))) / s + log(s' / s): every term is of the size of the differences, so nothing of
 // the size of the logits cancels.  The gradients of all three operators have one form,
-//     dl[j] = pick * (1[j = a] - p[j]) + p[j] * (kl * (log p[j] - log q[j] - KL) + ent * (log p[j] + H)).
+//     dl[j] = pick * (1[j = a] - p[j]) + p[j] * (kl * (log p[j] - log q[j] - KL) + ent * (log p[j] + H))
+//           = e[j] * (cd * (l[j] - m) + cq * (r[j] - m') + c0)  (+ pick at a)
+// with three coefficients of the row: an exponential, two FMAs and a product a column.
 // Partial sums of a row are taken against the largest value their lane or wave has seen and rescaled when they meet (Stats::join), so a row is read once.
 //
 // Bound by memory: a column costs some 20 operations for 4 to 12 bytes.  Three kernels by the number of columns, each reading and writing a row once
@@ -30,6 +32,9 @@ __device__ inline long long action_of(const procgen_amd_rows &p, long long r) {
 __device__ inline long long row_offset(const procgen_amd_rows &p, long long r, long long outer, long long inner) {
     return p.inner == 1 ? r * outer : (r / p.inner) * outer + (r % p.inner) * inner;
 }
+
+// a difference whose exponential is 0 in 32 bits, as a number that a zero can be multiplied with
+__device__ inline float floor_of(float d) { return fmaxf(d, -1000.f); }
 
 // sums over the columns seen so far.  m = -inf: none that is finite; s is then 0, or NaN where a NaN was among them
 template <bool REF>
@@ -59,13 +64,13 @@ struct Stats {
         m = to;
     }
     __device__ void add(float l, float r) {  // against maxima that cover them
-        const float d = l - safe(m), e = __expf(d);
+        const float d = l - safe(m), e = __expf(d), f = floor_of(d);
         s += e;
-        if (e != 0.f) w += e * d;
+        w = fmaf(e, f, w);
         if (REF) {
             const float q = r - safe(m2);
             s2 += __expf(q);
-            if (e != 0.f) u += e * (d - q);
+            u = fmaf(e, e == 0.f ? 0.f : f - q, u);
         }
     }
     // over `width` neighbouring lanes, all of which get the same bits
@@ -93,19 +98,20 @@ struct Sums {
     double policy = 0, kl = 0, entropy = 0, clipped = 0;
 };
 struct Coef {
-    bool known;
-    float pick, kl, ent, KL, H;  // the formula's
-    float m, log_s, inv_s, m2, log_s2;
+    float m, m2, cd, cq, c0, pick;
+    // from the formula's numbers, all of them times `scale`; without a known action everything is NaN
+    __device__ void set(bool known, float inv_s, float log_s, float log_s2, float H, float KL, float choice, float kl, float ent, float scale) {
+        cd = (ent + kl) * inv_s * scale;
+        cq = -kl * inv_s * scale;
+        c0 = known ? (ent * (H - log_s) + (kl != 0.f ? kl * ((log_s2 - log_s) - KL) : 0.f) - choice) * inv_s * scale : NAN;
+        pick = choice * scale;
+    }
     template <bool REF>
-    __device__ float gradient(float l, float r, bool taken) const {
-        const float d = l - m, p = __expf(d) * inv_s, log_p = d - log_s;
-        float g = (taken ? pick : 0.f) - pick * p;
-        if (p != 0.f) {
-            float f = ent * (log_p + H);
-            if (REF) f += kl * ((log_p - ((r - m2) - log_s2)) - KL);
-            g += p * f;
-        }
-        return known ? g : NAN;
+    __device__ float gradient(float l, float r) const {
+        const float d = l - m, e = __expf(d);
+        float f = fmaf(cd, floor_of(d), c0);
+        if (REF) f = fmaf(cq, e == 0.f ? 0.f : r - m2, f);
+        return e * f;
     }
 };
 
@@ -137,13 +143,9 @@ struct LogprobsBackward {  // of rows short enough to sum up again
     template <bool REF>
     __device__ bool finish(long long r, const Stats<REF> &x, bool known, float, bool, Coef &c, Sums &) const {
         if (x.empty()) return false;
-        c.known = known;
+        const float log_s = logf(x.s), inv_s = 1.f / x.s;
         c.m = Stats<REF>::safe(x.m);
-        c.log_s = logf(x.s);
-        c.inv_s = 1.f / x.s;
-        c.H = c.log_s - x.w / x.s;
-        c.pick = d_logp ? d_logp[r] : 0.f;
-        c.ent = d_entropy ? -d_entropy[r] : 0.f;
+        c.set(known, inv_s, log_s, 0.f, log_s - x.w * inv_s, 0.f, d_logp ? d_logp[r] : 0.f, 0.f, d_entropy ? -d_entropy[r] : 0.f, 1.f);
         return true;
     }
 };
@@ -169,19 +171,16 @@ struct Policy {
     template <bool REF>
     __device__ bool finish(long long r, const Stats<REF> &x, bool known, float l, bool first, Coef &c, Sums &sums) const {
         if (x.empty()) return false;
-        c.known = known;
         c.m = Stats<REF>::safe(x.m);
-        c.log_s = logf(x.s);
-        c.inv_s = 1.f / x.s;
-        c.H = c.log_s - x.w / x.s;
-        const float logp = known ? (l - c.m) - c.log_s : NAN, ratio = __expf(logp - q.old_logprobs[r]), adv = q.adv[r], lo = 1.f - q.clip_low, hi = 1.f + q.clip_high;
+        const float log_s = logf(x.s), inv_s = 1.f / x.s, H = log_s - x.w * inv_s, logp = known ? (l - c.m) - log_s : NAN;
+        const float ratio = __expf(logp - q.old_logprobs[r]), adv = q.adv[r], lo = 1.f - q.clip_low, hi = 1.f + q.clip_high;
         const float held = (ratio < lo ? lo : ratio > hi ? hi : ratio) * adv, plain = ratio * adv;
         const bool out = plain > held;  // the clipped side is the smaller one and its gradient is zero; never where something is NaN
-        float pick = out ? 0.f : -plain, KL = 0.f;
+        float pick = out ? 0.f : -plain, KL = 0.f, log_s2 = 0.f;
         if (REF) {
             c.m2 = Stats<REF>::safe(x.m2);
-            c.log_s2 = logf(x.s2);
-            KL = x.s2 == 0.f ? INFINITY : x.u / x.s + logf(x.s2 / x.s);
+            log_s2 = logf(x.s2);
+            KL = x.s2 == 0.f ? INFINITY : x.u * inv_s + logf(x.s2 * inv_s);
         } else if (q.ref_logprobs) {
             const float d = q.ref_logprobs[r] - logp, f = expm1f(d);
             KL = f - d;
@@ -190,13 +189,10 @@ struct Policy {
         if (first) {
             sums.policy -= out ? held : plain;
             sums.kl += KL;
-            sums.entropy += c.H;
+            sums.entropy += H;
             sums.clipped += ratio < lo || ratio > hi ? 1.0 : 0.0;
         }
-        c.KL = KL;
-        c.pick = pick * scale;
-        c.kl = q.kl_coef * scale;
-        c.ent = q.entropy_coef * scale;
+        c.set(known, inv_s, log_s, log_s2, H, KL, pick, REF ? q.kl_coef : 0.f, q.entropy_coef, scale);
         return true;
     }
 };
@@ -290,27 +286,45 @@ __global__ __launch_bounds__(BLOCK) void short_rows(procgen_amd_rows p, Op op, c
         bool some = false;
         Coef c;
         if (wanted) {
-            float l[MOST], l2[REF ? MOST : 1];
+            // more than MOST / 2 columns, the others -inf; l and l2 become the differences to the maxima, e their exponentials
+            float l[MOST], e[MOST], l2[REF ? MOST : 1];
             Stats<REF> x;
 #pragma unroll
-            for (int j = 0; j < MOST; j++)
-                if (j < columns) {
-                    l[j] = (float)row[j];
-                    x.m = fmaxf(x.m, l[j]);
-                    if (REF) {
-                        l2[j] = (float)row2[j];
-                        x.m2 = fmaxf(x.m2, l2[j]);
-                    }
+            for (int j = 0; j < MOST; j++) {
+                const bool real = MOST > 8 && j <= MOST / 2 ? true : j < columns;
+                l[j] = real ? (float)row[j] : -INFINITY;
+                x.m = fmaxf(x.m, l[j]);
+                if (REF) {
+                    l2[j] = real ? (float)row2[j] : -INFINITY;
+                    x.m2 = fmaxf(x.m2, l2[j]);
                 }
+            }
+            const float m = Stats<REF>::safe(x.m), m2 = Stats<REF>::safe(x.m2);
 #pragma unroll
-            for (int j = 0; j < MOST; j++)
-                if (j < columns) x.add(l[j], REF ? l2[j] : 0.f);
+            for (int j = 0; j < MOST; j++) {
+                const float d = l[j] - m;
+                e[j] = __expf(d);
+                l[j] = floor_of(d);
+                x.s += e[j];
+                x.w = fmaf(e[j], l[j], x.w);
+                if (REF) {
+                    const float q = l2[j] - m2;
+                    x.s2 += __expf(q);
+                    l2[j] = e[j] == 0.f ? 0.f : q;
+                    x.u = fmaf(e[j], l[j] - l2[j], x.u);
+                }
+            }
             const bool known = a >= 0 && a < columns;
             some = op.template finish<REF>(r, x, known, known ? (float)row[a] : 0.f, true, c, sums);
             if (Op::GRADIENT && some && p.d_logits) {
+                const float taken = known ? (float)row[a] : 0.f, taken2 = REF && known ? (float)row2[a] : 0.f;
 #pragma unroll
-                for (int j = 0; j < MOST; j++)
-                    if (j < columns) row[j] = (T)c.gradient<REF>(l[j], REF ? l2[j] : 0.f, j == a);
+                for (int j = 0; j < MOST; j++) {
+                    float f = fmaf(c.cd, l[j], c.c0);
+                    if (REF) f = fmaf(c.cq, l2[j], f);
+                    if ((MOST > 8 && j <= MOST / 2) || j < columns) row[j] = (T)(e[j] * f);
+                }
+                if (known) row[a] = (T)(c.gradient<REF>(taken, taken2) + c.pick);
             }
         }
         if (Op::GRADIENT && p.d_logits) {
@@ -425,7 +439,7 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
             for (int i = 0; i < CH; i++) {
                 const int j = min(at(b, i), columns - N), shared = at(b, i) - j;
                 Chunk<E> d;
-                for (int k = 0; k < N; k++) d.x[k] = some ? (T)c.gradient<REF>((float)l[i].x[k], REF ? (float)l2[i].x[k] : 0.f, j + k == a) : (T)0.f;
+                for (int k = 0; k < N; k++) d.x[k] = some ? (T)c.gradient<REF>((float)l[i].x[k], REF ? (float)l2[i].x[k] : 0.f) : (T)0.f;
                 if (shared == 0) {
                     d.store(out + j);
                 } else {
@@ -434,6 +448,8 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
                 }
             }
         }
+        if (some && a >= 0 && a < columns && (int)(a / N) % G == g)  // by the lane that wrote the column just now
+            out[a] = (T)(c.gradient<REF>((float)row[a], REF ? (float)row2[a] : 0.f) + c.pick);
     }
     if (Op::SUMS && partial) put_sums(sums, partial);
 }
@@ -450,15 +466,11 @@ __global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, c
         const T *const row = (const T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride);
         T *const out = (T *)p.d_logits + r * p.columns;
         const long long a = action_of(p, r);
+        const float pick = d_logp ? d_logp[r] : 0.f, ent = d_entropy ? -d_entropy[r] : 0.f, z = lse[r];
+        const bool known = a >= 0 && a < columns, some = !(pick == 0.f && ent == 0.f) && z != -INFINITY;
         Coef c;
-        c.known = a >= 0 && a < columns;
-        c.pick = d_logp ? d_logp[r] : 0.f;
-        c.ent = d_entropy ? -d_entropy[r] : 0.f;
-        c.H = entropy[r];
-        c.m = lse[r];
-        c.log_s = 0.f;
-        c.inv_s = 1.f;
-        const bool some = !(c.pick == 0.f && c.ent == 0.f) && c.m != -INFINITY;
+        c.m = z;
+        c.set(known, 1.f, 0.f, 0.f, entropy[r], 0.f, pick, 0.f, ent, 1.f);
         Chunk<E> x;
         const bool whole = j + N <= columns;
         if (whole) {
@@ -466,7 +478,7 @@ __global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, c
         } else {
             for (int k = 0; k < N; k++) x.x[k] = j + k < columns ? row[j + k] : (T)0.f;
         }
-        for (int k = 0; k < N; k++) x.x[k] = some ? (T)c.gradient<false>((float)x.x[k], 0.f, j + k == a) : (T)0.f;
+        for (int k = 0; k < N; k++) x.x[k] = some ? (T)(c.gradient<false>((float)x.x[k], 0.f) + (j + k == a ? pick : 0.f)) : (T)0.f;
         if (whole) {
             x.store(out + j);
         } else {
@@ -532,7 +544,8 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
     constexpr int N = Chunk<E>::N;
     if (p.columns <= 64) {
         const size_t lds = ((WAVE * p.columns * sizeof(typename E::T) + 15) & ~15ull) * (BLOCK / WAVE) * (REF ? 2 : 1);
-        if (p.columns <= 16) short_rows<E, 16, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        if (p.columns <= 8) short_rows<E, 8, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         else if (p.columns <= 32) short_rows<E, 32, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         else short_rows<E, 64, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.columns <= 16 * 2 * N) {
