@@ -24,7 +24,8 @@ namespace {
 
 constexpr int BLOCK = 256;
 constexpr int MAX_COUNT_BLOCKS = 256;
-constexpr int MAX_BLOCKS = 2048;
+constexpr int CUS = 256;
+constexpr int MAX_BLOCKS = 8 * CUS;
 
 __device__ inline long long action_of(const procgen_amd_rows &p, long long r) {
     return p.actions_are_64_bit ? ((const long long *)p.actions)[r] : (long long)((const int *)p.actions)[r];
@@ -115,16 +116,18 @@ struct Coef {
     }
 };
 
-// Each operator's rows: what it loads for a row, what it makes of the row's sums.  finish() is called once per row by one lane at least, with `first`
-// set in exactly one; it returns whether the row's gradient is anything but zero.
+// Each operator's rows: what it fetches for a row besides its logits, whether it wants the row at all, what it makes of the row's sums.  finish() is
+// called once per row by one lane at least, with `first` set in exactly one; it returns whether the row's gradient is anything but zero.
 struct Logprobs {
     static constexpr bool GRADIENT = false, SUMS = false;
     __device__ bool done() const { return false; }
     float *logp, *entropy, *lse;
+    struct In {};
     __device__ void begin(const procgen_amd_rows &) {}
-    __device__ bool wanted(long long) const { return true; }
+    __device__ In fetch(long long) const { return In(); }
+    __device__ bool wanted(const In &) const { return true; }
     template <bool REF>
-    __device__ bool finish(long long r, const Stats<REF> &x, bool known, float l, bool first, Coef &, Sums &) const {
+    __device__ bool finish(long long r, const In &, const Stats<REF> &x, bool known, float l, bool first, Coef &, Sums &) const {
         if (!first) return false;
         const float log_s = logf(x.s), m = Stats<REF>::safe(x.m);
         logp[r] = !known ? NAN : x.empty() ? -INFINITY : (l - m) - log_s;
@@ -138,14 +141,18 @@ struct LogprobsBackward {  // of rows short enough to sum up again
     static constexpr bool GRADIENT = true, SUMS = false;
     __device__ bool done() const { return false; }
     const float *d_logp, *d_entropy;
+    struct In {
+        float d_logp, d_entropy;
+    };
     __device__ void begin(const procgen_amd_rows &) {}
-    __device__ bool wanted(long long r) const { return (d_logp && d_logp[r] != 0.f) || (d_entropy && d_entropy[r] != 0.f); }
+    __device__ In fetch(long long r) const { return {d_logp ? d_logp[r] : 0.f, d_entropy ? d_entropy[r] : 0.f}; }
+    __device__ bool wanted(const In &in) const { return in.d_logp != 0.f || in.d_entropy != 0.f; }
     template <bool REF>
-    __device__ bool finish(long long r, const Stats<REF> &x, bool known, float, bool, Coef &c, Sums &) const {
+    __device__ bool finish(long long, const In &in, const Stats<REF> &x, bool known, float, bool, Coef &c, Sums &) const {
         if (x.empty()) return false;
         const float log_s = logf(x.s), inv_s = 1.f / x.s;
         c.m = Stats<REF>::safe(x.m);
-        c.set(known, inv_s, log_s, 0.f, log_s - x.w * inv_s, 0.f, d_logp ? d_logp[r] : 0.f, 0.f, d_entropy ? -d_entropy[r] : 0.f, 1.f);
+        c.set(known, inv_s, log_s, 0.f, log_s - x.w * inv_s, 0.f, in.d_logp, 0.f, -in.d_entropy, 1.f);
         return true;
     }
 };
@@ -167,13 +174,18 @@ struct Policy {
         }
         scale = (q.scale ? *q.scale : 1.f) * (n > 0 ? (float)(1.0 / (double)n) : 0.f);
     }
-    __device__ bool wanted(long long r) const { return !q.valid || q.valid[r]; }
+    struct In {
+        float old, adv, ref;
+        uint8_t valid;
+    };
+    __device__ In fetch(long long r) const { return {q.old_logprobs[r], q.adv[r], q.ref_logprobs ? q.ref_logprobs[r] : 0.f, q.valid ? q.valid[r] : (uint8_t)1}; }
+    __device__ bool wanted(const In &in) const { return in.valid; }
     template <bool REF>
-    __device__ bool finish(long long r, const Stats<REF> &x, bool known, float l, bool first, Coef &c, Sums &sums) const {
+    __device__ bool finish(long long, const In &in, const Stats<REF> &x, bool known, float l, bool first, Coef &c, Sums &sums) const {
         if (x.empty()) return false;
         c.m = Stats<REF>::safe(x.m);
         const float log_s = logf(x.s), inv_s = 1.f / x.s, H = log_s - x.w * inv_s, logp = known ? (l - c.m) - log_s : NAN;
-        const float ratio = __expf(logp - q.old_logprobs[r]), adv = q.adv[r], lo = 1.f - q.clip_low, hi = 1.f + q.clip_high;
+        const float ratio = __expf(logp - in.old), adv = in.adv, lo = 1.f - q.clip_low, hi = 1.f + q.clip_high;
         const float held = (ratio < lo ? lo : ratio > hi ? hi : ratio) * adv, plain = ratio * adv;
         const bool out = plain > held;  // the clipped side is the smaller one and its gradient is zero; never where something is NaN
         float pick = out ? 0.f : -plain, KL = 0.f, log_s2 = 0.f;
@@ -182,7 +194,7 @@ struct Policy {
             log_s2 = logf(x.s2);
             KL = x.s2 == 0.f ? INFINITY : x.u * inv_s + logf(x.s2 * inv_s);
         } else if (q.ref_logprobs) {
-            const float d = q.ref_logprobs[r] - logp, f = expm1f(d);
+            const float d = in.ref - logp, f = expm1f(d);
             KL = f - d;
             pick -= q.kl_coef * f;
         }
@@ -232,37 +244,64 @@ struct Chunk {
 
 // ---- up to 64 columns: a lane per row -------------------------------------------------------------------------------------------------------------
 
-// 64 rows between memory and LDS; `rows` of them exist.  Contiguous rows go 16 bytes a lane, others element by element.
-template <class E>
-__device__ inline void rows_to_lds(typename E::T *lds, const procgen_amd_rows &p, const void *from, long long outer, long long inner, long long r0, int rows, int lane) {
+// 64 rows on their way from memory to LDS (`rows` of them exist).  Contiguous rows go 16 bytes a lane and, where they are few registers, are fetched
+// while the 64 before them are worked on; others go element by element.
+template <class E, int MOST>
+struct Tile {
     typedef typename E::T T;
-    const int columns = (int)p.columns, n = rows * columns;
-    if (p.inner == 1 && outer == columns) {
-        const T *src = (const T *)from + r0 * columns;
-        constexpr int N = Chunk<E>::N;
-        for (int i = lane * N; i < n; i += WAVE * N) {
-            if (i + N <= n) {
-                Chunk<E> c;
-                c.load(src + i);
-                c.store_aligned(lds + i);
-            } else {
-                for (int k = i; k < n; k++) lds[k] = src[k];
-            }
-        }
-    } else {
-        for (int i = lane; i < n; i += WAVE) {
-            const int r = i / columns;
-            lds[i] = ((const T *)from)[row_offset(p, r0 + r, outer, inner) + (i - r * columns)];
+    static constexpr int N = Chunk<E>::N, CHUNKS = MOST * (int)sizeof(T) / 16;  // 64 rows of MOST columns: so many 16 bytes a lane
+    static constexpr bool AHEAD = CHUNKS <= 4;
+    typedef uint32_t Bits __attribute__((ext_vector_type(4)));
+    Bits c[AHEAD ? CHUNKS : 1];
+    __device__ void fetch(const procgen_amd_rows &p, const void *from, long long outer, long long r0, int rows, int lane) {
+        if (!AHEAD || p.inner != 1 || outer != p.columns) return;
+        const int n = rows * (int)p.columns;
+        const T *const src = (const T *)from + r0 * p.columns;
+#pragma unroll
+        for (int i = 0; i < (AHEAD ? CHUNKS : 0); i++) {
+            const int at = (i * WAVE + lane) * N;
+            if (at + N <= n) __builtin_memcpy(&c[i], src + at, 16);
         }
     }
-}
+    __device__ void put(T *lds, const procgen_amd_rows &p, const void *from, long long outer, long long inner, long long r0, int rows, int lane) const {
+        const int columns = (int)p.columns, n = rows * columns;
+        if (p.inner == 1 && outer == columns) {
+            const T *const src = (const T *)from + r0 * columns;
+            if (AHEAD) {
+#pragma unroll
+                for (int i = 0; i < (AHEAD ? CHUNKS : 0); i++) {
+                    const int at = (i * WAVE + lane) * N;
+                    if (at + N <= n) *(Bits *)(lds + at) = c[i];
+                }
+            } else {
+                for (int at = lane * N; at + N <= n; at += WAVE * N) {
+                    Chunk<E> k;
+                    k.load(src + at);
+                    k.store_aligned(lds + at);
+                }
+            }
+            if (n / N * N + lane < n) lds[n / N * N + lane] = src[n / N * N + lane];
+        } else {
+            for (int i = lane; i < n; i += WAVE) {
+                const int r = i / columns;
+                lds[i] = ((const T *)from)[row_offset(p, r0 + r, outer, inner) + (i - r * columns)];
+            }
+        }
+    }
+};
 __device__ inline void lds_settled() {  // a wave's own LDS is written and read in order; this holds the compiler to it
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
 
+// blocks of four waves that a compute unit holds: by registers (three, or four with a reference, for each of MOST columns) and by LDS
+template <class E, int MOST, bool REF>
+constexpr int short_residents() {
+    return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? 3 : sizeof(typename E::T) == 4 ? 4 : 5) : MOST <= 32 ? (REF ? 2 : 3) : REF ? 1 : 2;
+}
+
 template <class E, int MOST, bool REF, class Op>
-__global__ __launch_bounds__(BLOCK) void short_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
+__global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void short_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), columns = (int)p.columns;
@@ -272,15 +311,30 @@ __global__ __launch_bounds__(BLOCK) void short_rows(procgen_amd_rows p, Op op, c
     op.begin(p);
     Sums sums;
     const long long step = (long long)gridDim.x * (BLOCK / WAVE) * WAVE;
-    for (long long r0 = ((long long)blockIdx.x * (BLOCK / WAVE) + wave) * WAVE; r0 < p.rows; r0 += step) {
+    Tile<E, MOST> next;
+    Tile<E, REF ? MOST : 8> next2;
+    typename Op::In next_in;
+    long long next_a = 0;
+    auto fetch = [&](long long r0) {
+        const int rows = (int)min((long long)WAVE, p.rows - r0);
+        const long long r = r0 + min(lane, rows - 1);
+        next_in = op.fetch(r);
+        next_a = action_of(p, r);
+        next.fetch(p, p.logits, p.outer_stride, r0, rows, lane);
+        if (REF) next2.fetch(p, ref, ref_outer, r0, rows, lane);
+    };
+    long long r0 = ((long long)blockIdx.x * (BLOCK / WAVE) + wave) * WAVE;
+    if (r0 < p.rows) fetch(r0);
+    for (; r0 < p.rows; r0 += step) {
         const int rows = (int)min((long long)WAVE, p.rows - r0);
         const bool mine = lane < rows;
-        const long long r = mine ? r0 + lane : r0;
-        const bool wanted = mine && op.wanted(r);
-        const long long a = action_of(p, r);
-        rows_to_lds<E>(tile, p, p.logits, p.outer_stride, p.inner_stride, r0, rows, lane);
-        if (REF) rows_to_lds<E>(tile2, p, ref, ref_outer, ref_inner, r0, rows, lane);
+        const long long r = mine ? r0 + lane : r0, a = next_a;
+        const typename Op::In in = next_in;
+        const bool wanted = mine && op.wanted(in);
+        next.put(tile, p, p.logits, p.outer_stride, p.inner_stride, r0, rows, lane);
+        if (REF) next2.put(tile2, p, ref, ref_outer, ref_inner, r0, rows, lane);
         lds_settled();
+        if (r0 + step < p.rows) fetch(r0 + step);
         T *const row = tile + lane * columns;
         const T *const row2 = tile2 + lane * columns;
         bool some = false;
@@ -315,7 +369,7 @@ __global__ __launch_bounds__(BLOCK) void short_rows(procgen_amd_rows p, Op op, c
                 }
             }
             const bool known = a >= 0 && a < columns;
-            some = op.template finish<REF>(r, x, known, known ? (float)row[a] : 0.f, true, c, sums);
+            some = op.template finish<REF>(r, in, x, known, known ? (float)row[a] : 0.f, true, c, sums);
             if (Op::GRADIENT && some && p.d_logits) {
                 const float taken = known ? (float)row[a] : 0.f, taken2 = REF && known ? (float)row2[a] : 0.f;
 #pragma unroll
@@ -397,7 +451,8 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
         };
         Coef c;
         long long a = 0;
-        if (op.wanted(r)) {  // the same for the whole group
+        const typename Op::In in = op.fetch(r);
+        if (op.wanted(in)) {  // the same for the whole group
             a = action_of(p, r);
             const bool known = a >= 0 && a < columns;
             const float taken = (float)row[known ? a : 0];
@@ -429,7 +484,7 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
                 if (REF) x.m2 = __shfl(x.m2, 0, WAVE), x.s2 = __shfl(x.s2, 0, WAVE), x.u = __shfl(x.u, 0, WAVE);
                 odd ^= 1;
             }
-            some = op.template finish<REF>(r, x, known, taken, g == 0, c, sums);
+            some = op.template finish<REF>(r, in, x, known, taken, g == 0, c, sums);
             forget();
         }
         if (!Op::GRADIENT || !out) continue;
@@ -509,12 +564,13 @@ __global__ __launch_bounds__(BLOCK) void count_valid(const uint8_t *valid, long 
     if (threadIdx.x == 0) counts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
-__global__ __launch_bounds__(BLOCK) void policy_means(procgen_amd_policy q, long long rows, const long long *counts, int count_blocks, const double *partial, int blocks) {
+constexpr int MEANS = 1024;
+__global__ __launch_bounds__(MEANS) void policy_means(procgen_amd_policy q, long long rows, const long long *counts, int count_blocks, const double *partial, int blocks) {
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, k = lane % 4;  // four neighbouring lanes: a block's four sums
     double v = 0;
-    for (int i = threadIdx.x / 4; i < blocks; i += BLOCK / 4) v += partial[(long long)i * 4 + k];
+    for (int i = threadIdx.x / 4; i < blocks; i += MEANS / 4) v += partial[(long long)i * 4 + k];
     for (int d = WAVE / 2; d >= 4; d >>= 1) v += __shfl_xor(v, d, WAVE);
-    __shared__ double part[BLOCK / WAVE][4];
+    __shared__ double part[MEANS / WAVE][4];
     if (lane < 4) part[wave][lane] = v;
     __syncthreads();
     if (wave) return;
@@ -524,8 +580,11 @@ __global__ __launch_bounds__(BLOCK) void policy_means(procgen_amd_policy q, long
         for (int i = lane; i < count_blocks; i += WAVE) n += counts[i];
         n = wave_reduce(n, Sum());
     }
-    double mean[4];
-    for (int i = 0; i < 4; i++) mean[i] = n > 0 ? (part[0][i] + part[1][i] + part[2][i] + part[3][i]) / (double)n : 0.0;
+    double mean[4] = {0, 0, 0, 0};
+    for (int i = 0; i < 4 && n > 0; i++) {
+        for (int w = 0; w < MEANS / WAVE; w++) mean[i] += part[w][i];
+        mean[i] /= (double)n;
+    }
     if (lane == 0) *q.loss = (float)(mean[0] + (q.kl_coef != 0.f ? (double)q.kl_coef * mean[1] : 0.0) - (q.entropy_coef != 0.f ? (double)q.entropy_coef * mean[2] : 0.0));
     if (lane < 4) q.stats[lane] = (float)mean[lane];
 }
@@ -544,10 +603,10 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
     constexpr int N = Chunk<E>::N;
     if (p.columns <= 64) {
         const size_t lds = ((WAVE * p.columns * sizeof(typename E::T) + 15) & ~15ull) * (BLOCK / WAVE) * (REF ? 2 : 1);
-        if (p.columns <= 8) short_rows<E, 8, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if (p.columns <= 32) short_rows<E, 32, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else short_rows<E, 64, REF, Op><<<grid(BLOCK, MAX_BLOCKS), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        if (p.columns <= 8) short_rows<E, 8, REF, Op><<<grid(BLOCK, CUS * short_residents<E, 8, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<grid(BLOCK, CUS * short_residents<E, 16, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if (p.columns <= 32) short_rows<E, 32, REF, Op><<<grid(BLOCK, CUS * short_residents<E, 32, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else short_rows<E, 64, REF, Op><<<grid(BLOCK, CUS * short_residents<E, 64, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.columns <= 16 * 2 * N) {
         long_rows<E, 16, 2, REF, Op><<<grid(BLOCK / 16, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.columns <= 64 * 2 * N) {
@@ -636,7 +695,7 @@ LIBENV_API int procgen_amd_policy_loss(const struct procgen_amd_rows *p, const s
         if (blocks < 0) return -1 - blocks;
     }
     if (!q->loss) return 0;
-    policy_means<<<1, BLOCK, 0, (hipStream_t)stream>>>(*q, p->rows, counts, count_blocks, partial, blocks);
+    policy_means<<<1, MEANS, 0, (hipStream_t)stream>>>(*q, p->rows, counts, count_blocks, partial, blocks);
     return launched();
 }
 
