@@ -1,15 +1,18 @@
 // learner_rows.hip -- rows of logits, one column per action: log-probabilities and entropy of the actions taken (forward, backward) and the clipped
 // policy loss with its gradient.
 //
-// With m = max l, e[j] = exp(l[j] - m), s = sum e:  p[j] = e[j] / s,  log p[j] = (l[j] - m) - log s,  H = log s - (sum e (l - m)) / s, and against a
-// reference row r (m', s' alike)  KL = (sum e ((l - m) - (r - m'))) / s + log(s' / s): every term is of the size of the differences, so nothing of
-// the size of the logits cancels.  The gradients of all three operators have one form,
+// With m = max l and everything in powers of two, t[j] = (l[j] - m) log2 e as ONE FMA of l[j] (the rounding of m log2 e is the same in every column; `delta`,
+// what the maximum itself comes to, takes it out again), e[j] = 2^t[j], s = sum e:
+//     p[j] = e[j] / s,   log p[j] = ln 2 (t[j] - delta) - log s,   H = log s - ln 2 (sum e t / s - delta),
+// and against a reference row r (q, delta', s' alike)  KL = ln 2 (sum e (t - q) / s - delta + delta') + log s' - log s: every term is of the size of the
+// differences, so nothing of the size of the logits cancels.  The gradients of all three operators have one form,
 //     dl[j] = pick * (1[j = a] - p[j]) + p[j] * (kl * (log p[j] - log q[j] - KL) + ent * (log p[j] + H))
-//           = e[j] * (cd * (l[j] - m) + cq * (r[j] - m') + c0)  (+ pick at a)
-// with three coefficients of the row: an exponential, two FMAs and a product a column.
+//           = e[j] * (cd t[j] + cq q[j] + c0)  (+ pick at a)
+// with three coefficients of the row.  A column that is -inf (or too far below the maximum) has e = 0 and counts as 0 whatever it is multiplied with:
+// product() is the hardware's multiplication in which zero times anything is zero.
 // Partial sums of a row are taken against the largest value their lane or wave has seen and rescaled when they meet (Stats::join), so a row is read once.
 //
-// Bound by memory: a column costs some 20 operations for 4 to 12 bytes.  Three kernels by the number of columns, each reading and writing a row once
+// Bound by memory: a column costs 12 operations for 4 to 8 bytes, 23 for 6 to 12 with a reference.  Three kernels by the number of columns, each reading and writing a row once
 // and 16 bytes a lane:
 //   up to 64      a wave takes 64 rows through LDS, a lane per row: no reduction over lanes, coalesced although a row is no multiple of anything
 //   more          a group of 16, 64, 256 or 1024 lanes per row keeps the row in its registers between the sums and the gradient
@@ -34,15 +37,29 @@ __device__ inline long long row_offset(const procgen_amd_rows &p, long long r, l
     return p.inner == 1 ? r * outer : (r / p.inner) * outer + (r % p.inner) * inner;
 }
 
-// a difference whose exponential is 0 in 32 bits, as a number that a zero can be multiplied with
-__device__ inline float floor_of(float d) { return fmaxf(d, -1000.f); }
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
+__device__ inline float exp2_of(float t) { return __builtin_amdgcn_exp2f(t); }
+__device__ float multiply_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");  // v_mul_legacy_f32, which has no builtin function
+__device__ inline float product(float e, float x) { return multiply_legacy(e, x); }
+
+// the difference to a maximum in powers of two, t = scale * l - base.  Near the ends of float32 m log2 e would overflow; there two different numbers are
+// so far apart that any scale tells them apart, and a power of two is exact.
+struct Base {
+    float scale, base;
+    __device__ explicit Base(float m) {
+#pragma clang fp contract(off)  // base is this rounded number wherever it is used, or delta does not cancel
+        const bool far = fabsf(m) > 1e38f && fabsf(m) < INFINITY;
+        scale = far ? 0x1p-64f : LOG2E;
+        base = m == -INFINITY ? 0.f : m * scale;
+    }
+    __device__ float t(float l) const { return fmaf(l, scale, -base); }
+};
 
 // sums over the columns seen so far.  m = -inf: none that is finite; s is then 0, or NaN where a NaN was among them
 template <bool REF>
 struct Stats {
-    float m = -INFINITY, s = 0.f, w = 0.f;   // max, sum e, sum e (l - m)
-    float m2 = -INFINITY, s2 = 0.f, u = 0.f; // of the reference row, and sum e ((l - m) - (r - m2))
-    __device__ static float safe(float m) { return m == -INFINITY ? 0.f : m; }
+    float m = -INFINITY, s = 0.f, w = 0.f;   // max, sum e, sum e t
+    float m2 = -INFINITY, s2 = 0.f, u = 0.f; // of the reference row, and sum e (t - q)
     __device__ void put(float *to) const {
         to[0] = m, to[1] = s, to[2] = w;
         if (REF) to[3] = m2, to[4] = s2, to[5] = u;
@@ -54,24 +71,25 @@ struct Stats {
     __device__ bool empty() const { return m == -INFINITY && s == 0.f; }
     // the same sums against larger maxima
     __device__ void rescale(float to, float to2) {
-        const float d = m == -INFINITY ? 0.f : m - to, c = __expf(d), d2 = !REF || m2 == -INFINITY ? 0.f : m2 - to2;
+        const float d = m == -INFINITY ? 0.f : Base(m).base - Base(to).base, c = exp2_of(d), d2 = !REF || m2 == -INFINITY ? 0.f : Base(m2).base - Base(to2).base;
         if (REF) {
-            u = c == 0.f ? 0.f : c * (u + s * (d - d2));  // sums that vanish against the new maximum, far as it may be (s d overflows), are zero
-            s2 *= __expf(d2);
+            u = product(c, fmaf(s, d - d2, u));
+            s2 *= exp2_of(d2);
             m2 = to2;
         }
-        w = c == 0.f ? 0.f : c * (w + s * d);
+        w = product(c, fmaf(s, d, w));
         s *= c;
         m = to;
     }
-    __device__ void add(float l, float r) {  // against maxima that cover them
-        const float d = l - safe(m), e = __expf(d), f = floor_of(d);
+    // columns against maxima that cover them
+    __device__ void add(const Base &b, const Base &b2, float l, float r) {
+        const float t = b.t(l), e = exp2_of(t);
         s += e;
-        w = fmaf(e, f, w);
+        w += product(e, t);
         if (REF) {
-            const float q = r - safe(m2);
-            s2 += __expf(q);
-            u = fmaf(e, e == 0.f ? 0.f : f - q, u);
+            const float q = b2.t(r);
+            s2 += exp2_of(q);
+            u += product(e, t - q);
         }
     }
     // over `width` neighbouring lanes, all of which get the same bits
@@ -93,26 +111,51 @@ struct Stats {
         }
     }
 };
+// a row's own numbers: natural logarithms, the largest value taken out
+template <bool REF>
+struct Row {
+    float m, log_s, inv_s, H, delta, delta2, log_s2, KL;
+    __device__ explicit Row(const Stats<REF> &x) {
+        m = x.m == -INFINITY ? 0.f : x.m;
+        delta = Base(x.m).t(m);
+        inv_s = 1.f / x.s;
+        log_s = logf(x.s) - LN2 * delta;
+        H = log_s - LN2 * (x.w * inv_s - delta);
+        delta2 = log_s2 = KL = 0.f;
+        if (REF) {
+            delta2 = x.m2 == -INFINITY ? 0.f : Base(x.m2).t(x.m2);
+            log_s2 = logf(x.s2) - LN2 * delta2;
+            KL = x.s2 == 0.f ? INFINITY : fmaf(LN2, x.u * inv_s, logf(x.s2 * inv_s));  // the deltas are in both terms and cancel
+        }
+    }
+    __device__ float logp(float l) const { return (l - m) - log_s; }
+};
 
 // what the rows add up to, and the gradient's coefficients of one row
 struct Sums {
     double policy = 0, kl = 0, entropy = 0, clipped = 0;
 };
 struct Coef {
-    float m, m2, cd, cq, c0, pick;
-    // from the formula's numbers, all of them times `scale`; without a known action everything is NaN
-    __device__ void set(bool known, float inv_s, float log_s, float log_s2, float H, float KL, float choice, float kl, float ent, float scale) {
-        cd = (ent + kl) * inv_s * scale;
-        cq = -kl * inv_s * scale;
-        c0 = known ? (ent * (H - log_s) + (kl != 0.f ? kl * ((log_s2 - log_s) - KL) : 0.f) - choice) * inv_s * scale : NAN;
+    Base b, b2;
+    float cd, cq, c0, pick;
+    __device__ Coef() : b(0.f), b2(0.f) {}
+    // from the formula's numbers, all of them times `scale`.  Without a known action, or with a NaN among the logits, everything is NaN.
+    template <bool REF>
+    __device__ void set(bool known, const Stats<REF> &x, const Row<REF> &row, float choice, float kl, float ent, float scale) {
+        b = Base(x.m), b2 = Base(x.m2);
+        if (!known || x.s != x.s) b.base = NAN;
+        const float by = row.inv_s * scale;
+        cd = (ent + kl) * by * LN2;
+        cq = -kl * by * LN2;
+        c0 = (ent * (row.H - row.log_s) + (REF && kl != 0.f ? kl * ((row.log_s2 - row.log_s) - row.KL) : 0.f) - choice) * by - cd * row.delta - cq * row.delta2;
         pick = choice * scale;
     }
     template <bool REF>
     __device__ float gradient(float l, float r) const {
-        const float d = l - m, e = __expf(d);
-        float f = fmaf(cd, floor_of(d), c0);
-        if (REF) f = fmaf(cq, e == 0.f ? 0.f : r - m2, f);
-        return e * f;
+        const float t = b.t(l);
+        float f = fmaf(cd, t, c0);
+        if (REF) f = fmaf(cq, b2.t(r), f);
+        return product(exp2_of(t), f);
     }
 };
 
@@ -129,10 +172,10 @@ struct Logprobs {
     template <bool REF>
     __device__ bool finish(long long r, const In &, const Stats<REF> &x, bool known, float l, bool first, Coef &, Sums &) const {
         if (!first) return false;
-        const float log_s = logf(x.s), m = Stats<REF>::safe(x.m);
-        logp[r] = !known ? NAN : x.empty() ? -INFINITY : (l - m) - log_s;
-        entropy[r] = x.empty() ? 0.f : log_s - x.w / x.s;
-        if (lse) lse[r] = x.empty() ? -INFINITY : m + log_s;
+        const Row<REF> row(x);
+        logp[r] = !known ? NAN : x.empty() ? -INFINITY : row.logp(l);
+        entropy[r] = x.empty() ? 0.f : row.H;
+        if (lse) lse[r] = x.empty() ? -INFINITY : row.m + row.log_s;
         return false;
     }
 };
@@ -150,9 +193,7 @@ struct LogprobsBackward {  // of rows short enough to sum up again
     template <bool REF>
     __device__ bool finish(long long, const In &in, const Stats<REF> &x, bool known, float, bool, Coef &c, Sums &) const {
         if (x.empty()) return false;
-        const float log_s = logf(x.s), inv_s = 1.f / x.s;
-        c.m = Stats<REF>::safe(x.m);
-        c.set(known, inv_s, log_s, 0.f, log_s - x.w * inv_s, 0.f, in.d_logp, 0.f, -in.d_entropy, 1.f);
+        c.set(known, x, Row<REF>(x), in.d_logp, 0.f, -in.d_entropy, 1.f);
         return true;
     }
 };
@@ -183,17 +224,12 @@ struct Policy {
     template <bool REF>
     __device__ bool finish(long long, const In &in, const Stats<REF> &x, bool known, float l, bool first, Coef &c, Sums &sums) const {
         if (x.empty()) return false;
-        c.m = Stats<REF>::safe(x.m);
-        const float log_s = logf(x.s), inv_s = 1.f / x.s, H = log_s - x.w * inv_s, logp = known ? (l - c.m) - log_s : NAN;
-        const float ratio = __expf(logp - in.old), adv = in.adv, lo = 1.f - q.clip_low, hi = 1.f + q.clip_high;
+        const Row<REF> row(x);
+        const float logp = known ? row.logp(l) : NAN, ratio = __expf(logp - in.old), adv = in.adv, lo = 1.f - q.clip_low, hi = 1.f + q.clip_high;
         const float held = (ratio < lo ? lo : ratio > hi ? hi : ratio) * adv, plain = ratio * adv;
         const bool out = plain > held;  // the clipped side is the smaller one and its gradient is zero; never where something is NaN
-        float pick = out ? 0.f : -plain, KL = 0.f, log_s2 = 0.f;
-        if (REF) {
-            c.m2 = Stats<REF>::safe(x.m2);
-            log_s2 = logf(x.s2);
-            KL = x.s2 == 0.f ? INFINITY : x.u * inv_s + logf(x.s2 * inv_s);
-        } else if (q.ref_logprobs) {
+        float pick = out ? 0.f : -plain, KL = row.KL;
+        if (!REF && q.ref_logprobs) {
             const float d = in.ref - logp, f = expm1f(d);
             KL = f - d;
             pick -= q.kl_coef * f;
@@ -201,10 +237,10 @@ struct Policy {
         if (first) {
             sums.policy -= out ? held : plain;
             sums.kl += KL;
-            sums.entropy += H;
+            sums.entropy += row.H;
             sums.clipped += ratio < lo || ratio > hi ? 1.0 : 0.0;
         }
-        c.set(known, inv_s, log_s, log_s2, H, KL, pick, REF ? q.kl_coef : 0.f, q.entropy_coef, scale);
+        c.set(known, x, row, pick, REF ? q.kl_coef : 0.f, q.entropy_coef, scale);
         return true;
     }
 };
@@ -225,21 +261,46 @@ __device__ inline void put_sums(Sums x, double *partial) {
     }
 }
 
+// 16 bytes of a row in registers, as memory holds them
+typedef uint32_t Bits __attribute__((ext_vector_type(4)));
 template <class E>
 struct Chunk {
-    static constexpr int N = 16 / sizeof(typename E::T);
-    typename E::T x[N];
-    // forgets what the compiler has made of the values: they are widened again where they are used next, and not held in 32 bits in between
-    __device__ void forget() {
-        uint32_t w[4];
-        __builtin_memcpy(w, x, 16);
-        asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
-        __builtin_memcpy(x, w, 16);
+    typedef typename E::T T;
+    static constexpr int N = 16 / sizeof(T);
+    Bits w;
+    __device__ void load(const T *p) { __builtin_memcpy(&w, p, 16); }  // whatever the alignment
+    __device__ void store(T *p) const { __builtin_memcpy(p, &w, 16); }
+    __device__ float operator[](int k) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[k]);
+        else if constexpr (__is_same(T, __bf16)) return __builtin_bit_cast(float, k % 2 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16);
+        else return (float)__builtin_bit_cast(T, (uint16_t)(w[k / 2] >> k % 2 * 16));
     }
-    __device__ void load(const typename E::T *p) { __builtin_memcpy(x, p, 16); }  // from memory, whatever the alignment
-    __device__ void store(typename E::T *p) const { __builtin_memcpy(p, x, 16); }
-    __device__ void load_aligned(const typename E::T *p) { __builtin_memcpy(x, __builtin_assume_aligned(p, 16), 16); }  // from LDS
-    __device__ void store_aligned(typename E::T *p) const { __builtin_memcpy(__builtin_assume_aligned(p, 16), x, 16); }
+    __device__ void set(int d, float x, float y) {  // word d: value d, or values 2 d and 2 d + 1
+        if constexpr (sizeof(T) == 4) {
+            w[d] = __float_as_uint(x);
+        } else {
+            typedef T Two __attribute__((ext_vector_type(2)));
+            w[d] = __builtin_bit_cast(uint32_t, Two{(T)x, (T)y});
+        }
+    }
+    __device__ T piece(int k) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[k]);
+        else return __builtin_bit_cast(T, (uint16_t)(w[k / 2] >> k % 2 * 16));
+    }
+    // -inf for the first n values
+    __device__ void drop(int n) {
+        constexpr uint32_t INF = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __bf16) ? 0xff80u : 0xfc00u;
+        for (int d = 0; d < 4; d++) {
+            if constexpr (sizeof(T) == 4) {
+                if (d < n) w[d] = INF;
+            } else {
+                if (2 * d < n) w[d] = (w[d] & 0xffff0000u) | INF;
+                if (2 * d + 1 < n) w[d] = (w[d] & 0xffffu) | INF << 16;
+            }
+        }
+    }
+    // forgets what the compiler has made of the values: they are widened again where they are used next, and not held in 32 bits in between
+    __device__ void forget() { asm volatile("" : "+v"(w)); }
 };
 
 // ---- up to 64 columns: a lane per row -------------------------------------------------------------------------------------------------------------
@@ -251,7 +312,6 @@ struct Tile {
     typedef typename E::T T;
     static constexpr int N = Chunk<E>::N, CHUNKS = MOST * (int)sizeof(T) / 16;  // 64 rows of MOST columns: so many 16 bytes a lane
     static constexpr bool AHEAD = CHUNKS <= 4;
-    typedef uint32_t Bits __attribute__((ext_vector_type(4)));
     Bits c[AHEAD ? CHUNKS : 1];
     __device__ void fetch(const procgen_amd_rows &p, const void *from, long long outer, long long r0, int rows, int lane) {
         if (!AHEAD || p.inner != 1 || outer != p.columns) return;
@@ -275,9 +335,9 @@ struct Tile {
                 }
             } else {
                 for (int at = lane * N; at + N <= n; at += WAVE * N) {
-                    Chunk<E> k;
-                    k.load(src + at);
-                    k.store_aligned(lds + at);
+                    Bits k;
+                    __builtin_memcpy(&k, src + at, 16);
+                    *(Bits *)(lds + at) = k;
                 }
             }
             if (n / N * N + lane < n) lds[n / N * N + lane] = src[n / N * N + lane];
@@ -340,7 +400,7 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
         bool some = false;
         Coef c;
         if (wanted) {
-            // more than MOST / 2 columns, the others -inf; l and l2 become the differences to the maxima, e their exponentials
+            // more than MOST / 2 columns, the others -inf; l and l2 become t and q
             float l[MOST], e[MOST], l2[REF ? MOST : 1];
             Stats<REF> x;
 #pragma unroll
@@ -353,32 +413,32 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
                     x.m2 = fmaxf(x.m2, l2[j]);
                 }
             }
-            const float m = Stats<REF>::safe(x.m), m2 = Stats<REF>::safe(x.m2);
+            const Base b(x.m), b2(x.m2);
 #pragma unroll
             for (int j = 0; j < MOST; j++) {
-                const float d = l[j] - m;
-                e[j] = __expf(d);
-                l[j] = floor_of(d);
+                l[j] = b.t(l[j]);
+                e[j] = exp2_of(l[j]);
                 x.s += e[j];
-                x.w = fmaf(e[j], l[j], x.w);
+                x.w += product(e[j], l[j]);
                 if (REF) {
-                    const float q = l2[j] - m2;
-                    x.s2 += __expf(q);
-                    l2[j] = e[j] == 0.f ? 0.f : q;
-                    x.u = fmaf(e[j], l[j] - l2[j], x.u);
+                    l2[j] = b2.t(l2[j]);
+                    x.s2 += exp2_of(l2[j]);
+                    x.u += product(e[j], l[j] - l2[j]);
                 }
             }
             const bool known = a >= 0 && a < columns;
-            some = op.template finish<REF>(r, in, x, known, known ? (float)row[a] : 0.f, true, c, sums);
+            const float taken = known ? (float)row[a] : 0.f, taken2 = REF && known ? (float)row2[a] : 0.f;
+            some = op.template finish<REF>(r, in, x, known, taken, true, c, sums);
             if (Op::GRADIENT && some && p.d_logits) {
-                const float taken = known ? (float)row[a] : 0.f, taken2 = REF && known ? (float)row2[a] : 0.f;
 #pragma unroll
                 for (int j = 0; j < MOST; j++) {
                     float f = fmaf(c.cd, l[j], c.c0);
                     if (REF) f = fmaf(c.cq, l2[j], f);
-                    if ((MOST > 8 && j <= MOST / 2) || j < columns) row[j] = (T)(e[j] * f);
+                    if ((MOST > 8 && j <= MOST / 2) || j < columns) row[j] = (T)product(e[j], f);
                 }
                 if (known) row[a] = (T)(c.gradient<REF>(taken, taken2) + c.pick);
+                if (c.b.base != c.b.base)
+                    for (int j = 0; j < columns; j++) row[j] = (T)NAN;
             }
         }
         if (Op::GRADIENT && p.d_logits) {
@@ -391,7 +451,7 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
             for (int i = lane * N; i < n; i += WAVE * N) {
                 if (i + N <= n) {
                     Chunk<E> k;
-                    k.load_aligned(tile + i);
+                    k.w = *(const Bits *)(tile + i);
                     k.store(out + i);
                 } else {
                     for (int k = i; k < n; k++) out[k] = tile[k];
@@ -435,12 +495,10 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
 #pragma unroll
             for (int i = 0; i < CH; i++) {
                 const int shared = at(b, i) - (columns - N);
-                if (shared > 0)
-                    for (int k = 0; k < N; k++)
-                        if (k < shared) {
-                            l[i].x[k] = (T)-INFINITY;
-                            if (REF) l2[i].x[k] = (T)-INFINITY;
-                        }
+                if (shared > 0) {
+                    l[i].drop(shared);
+                    if (REF) l2[i].drop(shared);
+                }
             }
         };
         auto forget = [&] {
@@ -463,14 +521,15 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
 #pragma unroll
                 for (int i = 0; i < CH; i++)
                     for (int k = 0; k < N; k++) {
-                        to = fmaxf(to, (float)l[i].x[k]);
-                        if (REF) to2 = fmaxf(to2, (float)l2[i].x[k]);
+                        to = fmaxf(to, l[i][k]);
+                        if (REF) to2 = fmaxf(to2, l2[i][k]);
                     }
                 x.rescale(to, to2);
                 forget();
+                const Base base(to), base2(to2);
 #pragma unroll
                 for (int i = 0; i < CH; i++)
-                    for (int k = 0; k < N; k++) x.add((float)l[i].x[k], REF ? (float)l2[i].x[k] : 0.f);
+                    for (int k = 0; k < N; k++) x.add(base, base2, l[i][k], REF ? l2[i][k] : 0.f);
             }
             x.template join<(G < WAVE ? G : WAVE)>();
             if (G > WAVE) {
@@ -494,12 +553,16 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
             for (int i = 0; i < CH; i++) {
                 const int j = min(at(b, i), columns - N), shared = at(b, i) - j;
                 Chunk<E> d;
-                for (int k = 0; k < N; k++) d.x[k] = some ? (T)c.gradient<REF>((float)l[i].x[k], REF ? (float)l2[i].x[k] : 0.f) : (T)0.f;
+                constexpr int PER = N / 4;  // values of a word
+                for (int k = 0; k < N; k += PER) {
+                    const float y = c.gradient<REF>(l[i][k], REF ? l2[i][k] : 0.f), z = PER > 1 ? c.gradient<REF>(l[i][k + PER - 1], REF ? l2[i][k + PER - 1] : 0.f) : 0.f;
+                    d.set(k / PER, some ? y : 0.f, some ? z : 0.f);
+                }
                 if (shared == 0) {
                     d.store(out + j);
                 } else {
                     for (int k = 0; k < N; k++)
-                        if (k >= shared) out[j + k] = d.x[k];
+                        if (k >= shared) out[j + k] = d.piece(k);
                 }
             }
         }
@@ -515,7 +578,7 @@ __global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, c
     typedef typename E::T T;
     constexpr int N = Chunk<E>::N;
     const int columns = (int)p.columns;
-    const long long j = ((long long)blockIdx.x * BLOCK + threadIdx.x) * N;
+    const int j = (int)(((long long)blockIdx.x * BLOCK + threadIdx.x) * N);
     if (j >= columns) return;
     for (long long r = blockIdx.y; r < p.rows; r += gridDim.y) {
         const T *const row = (const T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride);
@@ -523,22 +586,24 @@ __global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, c
         const long long a = action_of(p, r);
         const float pick = d_logp ? d_logp[r] : 0.f, ent = d_entropy ? -d_entropy[r] : 0.f, z = lse[r];
         const bool known = a >= 0 && a < columns, some = !(pick == 0.f && ent == 0.f) && z != -INFINITY;
-        Coef c;
-        c.m = z;
-        c.set(known, 1.f, 0.f, 0.f, entropy[r], 0.f, pick, 0.f, ent, 1.f);
         Chunk<E> x;
-        const bool whole = j + N <= columns;
-        if (whole) {
-            x.load(row + j);
-        } else {
-            for (int k = 0; k < N; k++) x.x[k] = j + k < columns ? row[j + k] : (T)0.f;
+        const int at = min(j, columns - N), shared = j - at;  // the last one reaches back and writes only its own
+        x.load(row + at);
+        const float H = entropy[r];
+        constexpr int PER = N / 4;
+        auto gradient = [&](int k) {
+            const float log_p = x[k] - z, p = __expf(log_p);
+            return product(p, ent * (log_p + H) - pick) + (at + k == a ? pick : 0.f) + (known ? 0.f : NAN);
+        };
+        for (int k = 0; k < N; k += PER) {
+            const float y = some ? gradient(k) : 0.f, z1 = some && PER > 1 ? gradient(k + PER - 1) : 0.f;
+            x.set(k / PER, y, z1);
         }
-        for (int k = 0; k < N; k++) x.x[k] = some ? (T)(c.gradient<false>((float)x.x[k], 0.f) + (j + k == a ? pick : 0.f)) : (T)0.f;
-        if (whole) {
+        if (shared == 0) {
             x.store(out + j);
         } else {
             for (int k = 0; k < N; k++)
-                if (j + k < columns) out[j + k] = x.x[k];
+                if (k >= shared) out[at + k] = x.piece(k);
         }
     }
 }
