@@ -280,7 +280,9 @@ struct Chunk {
             w[d] = __float_as_uint(x);
         } else {
             typedef T Two __attribute__((ext_vector_type(2)));
-            w[d] = __builtin_bit_cast(uint32_t, Two{(T)x, (T)y});
+            typedef float TwoF __attribute__((ext_vector_type(2)));
+            const Two two = __builtin_convertvector((TwoF{x, y}), Two);
+            w[d] = __builtin_bit_cast(uint32_t, two);
         }
     }
     __device__ T piece(int k) const {
@@ -481,24 +483,37 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
         const T *const row2 = REF ? (const T *)ref + row_offset(p, r, ref_outer, ref_inner) : nullptr;
         T *const out = Op::GRADIENT && p.d_logits ? (T *)p.d_logits + r * p.columns : nullptr;
         bool some = false;
-        Chunk<E> l[CH], l2[REF ? CH : 1];
         // Columns [at(b, i), + N) are chunk i of batch b.  The last one of a row reaches back so that it ends with the row: what it shares with its
         // neighbour counts as -inf here and is not written.  Chunks behind the row are all -inf.
         auto at = [&](int b, int i) { return b * SPAN + (i * G + g) * N; };
+        Chunk<E> l[CH], l2[REF ? CH : 1], next[CH], next2[REF ? CH : 1];  // the batch that is worked on, and the one on its way
         auto load = [&](int b) {
 #pragma unroll
             for (int i = 0; i < CH; i++) {
                 const int j = min(at(b, i), columns - N);
-                l[i].load(row + j);
-                if (REF) l2[i].load(row2 + j);
+                next[i].load(row + j);
+                if (REF) next2[i].load(row2 + j);
             }
+        };
+        auto take = [&](int b) {
 #pragma unroll
             for (int i = 0; i < CH; i++) {
+                l[i] = next[i];
+                if (REF) l2[i] = next2[i];
                 const int shared = at(b, i) - (columns - N);
                 if (shared > 0) {
                     l[i].drop(shared);
                     if (REF) l2[i].drop(shared);
                 }
+            }
+        };
+        auto put = [&](T *to, int j, const Chunk<E> &d) {  // what is this lane's own of the chunk that is to begin at column j
+            const int own = min(j, columns - N);
+            if (own == j) {
+                d.store(to + j);
+            } else {
+                for (int k = 0; k < N; k++)
+                    if (own + k >= j) to[own + k] = d.piece(k);
             }
         };
         auto forget = [&] {
@@ -515,8 +530,11 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
             const bool known = a >= 0 && a < columns;
             const float taken = (float)row[known ? a : 0];
             Stats<REF> x;
+            Base base(x.m), base2(x.m2);
+            load(0);
             for (int b = 0; b < batches; b++) {
-                load(b);
+                take(b);
+                if (b + 1 < batches) load(b + 1);
                 float to = x.m, to2 = x.m2;
 #pragma unroll
                 for (int i = 0; i < CH; i++)
@@ -524,9 +542,13 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
                         to = fmaxf(to, l[i][k]);
                         if (REF) to2 = fmaxf(to2, l2[i][k]);
                     }
-                x.rescale(to, to2);
+                // m need not be the largest value, only near it: it is moved where it is left behind by more than 8, which after the first batches is rare
+                if (!(to <= x.m + 8.f) || (REF && !(to2 <= x.m2 + 8.f))) {
+                    x.rescale(to, to2);
+                    base = Base(to);
+                    base2 = Base(to2);
+                }
                 forget();
-                const Base base(to), base2(to2);
 #pragma unroll
                 for (int i = 0; i < CH; i++)
                     for (int k = 0; k < N; k++) x.add(base, base2, l[i][k], REF ? l2[i][k] : 0.f);
@@ -543,30 +565,35 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
                 if (REF) x.m2 = __shfl(x.m2, 0, WAVE), x.s2 = __shfl(x.s2, 0, WAVE), x.u = __shfl(x.u, 0, WAVE);
                 odd ^= 1;
             }
+            if (Op::GRADIENT && out && batches > 1) load(batches - 2);  // the first batch that is needed again
             some = op.template finish<REF>(r, in, x, known, taken, g == 0, c, sums);
             forget();
         }
         if (!Op::GRADIENT || !out) continue;
+        if (!some) {
+            for (int i = 0; i < batches * CH; i++) {
+                Chunk<E> zero;
+                zero.w = Bits{0, 0, 0, 0};
+                if (at(0, i) < columns) put(out, at(0, i), zero);
+            }
+            continue;
+        }
         for (int b = batches - 1; b >= 0; b--) {
-            if (some && b < batches - 1) load(b);
+            if (b < batches - 1) {
+                take(b);
+                if (b > 0) load(b - 1);
+            }
 #pragma unroll
             for (int i = 0; i < CH; i++) {
-                const int j = min(at(b, i), columns - N), shared = at(b, i) - j;
                 Chunk<E> d;
                 constexpr int PER = N / 4;  // values of a word
-                for (int k = 0; k < N; k += PER) {
-                    const float y = c.gradient<REF>(l[i][k], REF ? l2[i][k] : 0.f), z = PER > 1 ? c.gradient<REF>(l[i][k + PER - 1], REF ? l2[i][k + PER - 1] : 0.f) : 0.f;
-                    d.set(k / PER, some ? y : 0.f, some ? z : 0.f);
-                }
-                if (shared == 0) {
-                    d.store(out + j);
-                } else {
-                    for (int k = 0; k < N; k++)
-                        if (k >= shared) out[j + k] = d.piece(k);
-                }
+#pragma unroll
+                for (int k = 0; k < N; k += PER)
+                    d.set(k / PER, c.gradient<REF>(l[i][k], REF ? l2[i][k] : 0.f), PER > 1 ? c.gradient<REF>(l[i][k + PER - 1], REF ? l2[i][k + PER - 1] : 0.f) : 0.f);
+                if (at(b, i) < columns) put(out, at(b, i), d);
             }
         }
-        if (some && a >= 0 && a < columns && (int)(a / N) % G == g)  // by the lane that wrote the column just now
+        if (a >= 0 && a < columns && (int)(a / N) % G == g)  // by the lane that wrote the column just now
             out[a] = (T)(c.gradient<REF>((float)row[a], REF ? (float)row2[a] : 0.f) + c.pick);
     }
     if (Op::SUMS && partial) put_sums(sums, partial);
@@ -676,10 +703,10 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
         long_rows<E, 16, 2, REF, Op><<<grid(BLOCK / 16, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.columns <= 64 * 2 * N) {
         long_rows<E, 64, 2, REF, Op><<<grid(BLOCK / 64, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (p.columns <= 256 * 4 * N) {
-        long_rows<E, 256, 4, REF, Op><<<grid(1, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else {
-        long_rows<E, 1024, 4, REF, Op><<<grid(1, MAX_BLOCKS / 4), 1024, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (p.rows >= 2 * CUS || p.columns <= 256 * 4 * N) {
+        long_rows<E, 256, 2, REF, Op><<<grid(1, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else {  // too few rows to fill the card: more lanes for each
+        long_rows<E, 1024, 2, REF, Op><<<grid(1, CUS), 1024, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     }
     const int err = launched();
     return err ? -1 - err : blocks;
