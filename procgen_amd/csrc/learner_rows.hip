@@ -289,15 +289,16 @@ struct Chunk {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[k]);
         else return __builtin_bit_cast(T, (uint16_t)(w[k / 2] >> k % 2 * 16));
     }
-    // -inf for the first n values
+    // -inf for the first n values, or the last -n
     __device__ void drop(int n) {
         constexpr uint32_t INF = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __bf16) ? 0xff80u : 0xfc00u;
+        auto out = [&](int k) { return n > 0 ? k < n : k >= N + n; };
         for (int d = 0; d < 4; d++) {
             if constexpr (sizeof(T) == 4) {
-                if (d < n) w[d] = INF;
+                if (out(d)) w[d] = INF;
             } else {
-                if (2 * d < n) w[d] = (w[d] & 0xffff0000u) | INF;
-                if (2 * d + 1 < n) w[d] = (w[d] & 0xffffu) | INF << 16;
+                if (out(2 * d)) w[d] = (w[d] & 0xffff0000u) | INF;
+                if (out(2 * d + 1)) w[d] = (w[d] & 0xffffu) | INF << 16;
             }
         }
     }
@@ -476,21 +477,24 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
     if (op.done()) return;
     op.begin(p);
     Sums sums;
-    const int columns = (int)p.columns, batches = (columns + SPAN - 1) / SPAN;
+    const int columns = (int)p.columns;
     int odd = 0;
     for (long long r = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / G; r < p.rows; r += (long long)gridDim.x * PER_BLOCK) {
         const T *const row = (const T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride);
         const T *const row2 = REF ? (const T *)ref + row_offset(p, r, ref_outer, ref_inner) : nullptr;
         T *const out = Op::GRADIENT && p.d_logits ? (T *)p.d_logits + r * p.columns : nullptr;
         bool some = false;
-        // Columns [at(b, i), + N) are chunk i of batch b.  The last one of a row reaches back so that it ends with the row: what it shares with its
-        // neighbour counts as -inf here and is not written.  Chunks behind the row are all -inf.
-        auto at = [&](int b, int i) { return b * SPAN + (i * G + g) * N; };
+        // Chunk i of batch b are the columns [at(b, i), + N): 16 aligned bytes, whatever the row's own alignment (a row at an odd address costs an eighth
+        // more time otherwise).  The first and the last one of a row are moved so that they end in it: what they share with their neighbour counts as
+        // -inf here and is not written.  Chunks behind the row are all -inf.
+        const int ahead = (int)((uintptr_t)row / sizeof(T) % N), batches = (columns + ahead + SPAN - 1) / SPAN;
+        auto at = [&](int b, int i) { return b * SPAN + (i * G + g) * N - ahead; };
+        auto column = [&](int j) { return max(0, min(j, columns - N)); };
         Chunk<E> l[CH], l2[REF ? CH : 1], next[CH], next2[REF ? CH : 1];  // the batch that is worked on, and the one on its way
         auto load = [&](int b) {
 #pragma unroll
             for (int i = 0; i < CH; i++) {
-                const int j = min(at(b, i), columns - N);
+                const int j = column(at(b, i));
                 next[i].load(row + j);
                 if (REF) next2[i].load(row2 + j);
             }
@@ -500,20 +504,20 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
             for (int i = 0; i < CH; i++) {
                 l[i] = next[i];
                 if (REF) l2[i] = next2[i];
-                const int shared = at(b, i) - (columns - N);
-                if (shared > 0) {
-                    l[i].drop(shared);
-                    if (REF) l2[i].drop(shared);
+                const int moved = at(b, i) - column(at(b, i));
+                if (moved) {
+                    l[i].drop(moved);
+                    if (REF) l2[i].drop(moved);
                 }
             }
         };
         auto put = [&](T *to, int j, const Chunk<E> &d) {  // what is this lane's own of the chunk that is to begin at column j
-            const int own = min(j, columns - N);
-            if (own == j) {
+            const int from = column(j);
+            if (from == j) {
                 d.store(to + j);
             } else {
                 for (int k = 0; k < N; k++)
-                    if (own + k >= j) to[own + k] = d.piece(k);
+                    if (from + k >= j && from + k < j + N) to[from + k] = d.piece(k);
             }
         };
         auto forget = [&] {
@@ -593,7 +597,7 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
                 if (at(b, i) < columns) put(out, at(b, i), d);
             }
         }
-        if (a >= 0 && a < columns && (int)(a / N) % G == g)  // by the lane that wrote the column just now
+        if (a >= 0 && a < columns && (int)((a + ahead) / N) % G == g)  // by the lane that wrote the column just now
             out[a] = (T)(c.gradient<REF>((float)row[a], REF ? (float)row2[a] : 0.f) + c.pick);
     }
     if (Op::SUMS && partial) put_sums(sums, partial);
@@ -605,16 +609,16 @@ __global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, c
     typedef typename E::T T;
     constexpr int N = Chunk<E>::N;
     const int columns = (int)p.columns;
-    const int j = (int)(((long long)blockIdx.x * BLOCK + threadIdx.x) * N);
-    if (j >= columns) return;
     for (long long r = blockIdx.y; r < p.rows; r += gridDim.y) {
         const T *const row = (const T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride);
         T *const out = (T *)p.d_logits + r * p.columns;
+        const int ahead = (int)((uintptr_t)row / sizeof(T) % N), j = (int)(((long long)blockIdx.x * BLOCK + threadIdx.x) * N) - ahead;
+        if (j >= columns) continue;
         const long long a = action_of(p, r);
         const float pick = d_logp ? d_logp[r] : 0.f, ent = d_entropy ? -d_entropy[r] : 0.f, z = lse[r];
         const bool known = a >= 0 && a < columns, some = !(pick == 0.f && ent == 0.f) && z != -INFINITY;
         Chunk<E> x;
-        const int at = min(j, columns - N), shared = j - at;  // the last one reaches back and writes only its own
+        const int at = max(0, min(j, columns - N));  // aligned 16 bytes but for the first and the last, which write only their own
         x.load(row + at);
         const float H = entropy[r];
         constexpr int PER = N / 4;
@@ -626,11 +630,11 @@ __global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, c
             const float y = some ? gradient(k) : 0.f, z1 = some && PER > 1 ? gradient(k + PER - 1) : 0.f;
             x.set(k / PER, y, z1);
         }
-        if (shared == 0) {
+        if (at == j) {
             x.store(out + j);
         } else {
             for (int k = 0; k < N; k++)
-                if (k >= shared) out[at + k] = x.piece(k);
+                if (at + k >= j && at + k < j + N) out[at + k] = x.piece(k);
         }
     }
 }
@@ -744,7 +748,7 @@ LIBENV_API int procgen_amd_action_logprobs_backward(const struct procgen_amd_row
             const int got = launch_rows<E, false>(*p, LogprobsBackward{d_logp, d_entropy}, nullptr, 0, 0, nullptr, (hipStream_t)stream);
             return got < 0 ? -1 - got : 0;
         }
-        const long long chunks = (p->columns + Chunk<E>::N - 1) / Chunk<E>::N;
+        const long long chunks = (p->columns + Chunk<E>::N - 1) / Chunk<E>::N + 1;  // one more for rows that begin inside of 16 bytes
         const dim3 grid((unsigned)((chunks + BLOCK - 1) / BLOCK), (unsigned)std::min<long long>(p->rows, 65535));
         logprobs_gradient<E><<<grid, BLOCK, 0, (hipStream_t)stream>>>(*p, lse, entropy, d_logp, d_entropy);
         return launched();
