@@ -12,11 +12,12 @@
 // product() is the hardware's multiplication in which zero times anything is zero.
 // Partial sums of a row are taken against the largest value their lane or wave has seen and rescaled when they meet (Stats::join), so a row is read once.
 //
-// Bound by memory: a column costs 12 operations for 4 to 8 bytes, 23 for 6 to 12 with a reference.  Three kernels by the number of columns, each reading and writing a row once
-// and 16 bytes a lane:
+// Bound by memory: a column costs 12 operations for 4 to 8 bytes, 23 for 6 to 12 with a reference.  By the number of columns:
 //   up to 64      a wave takes 64 rows through LDS, a lane per row: no reduction over lanes, coalesced although a row is no multiple of anything
-//   more          a group of 16, 64, 256 or 1024 lanes per row keeps the row in its registers between the sums and the gradient
-//   very long     the same group in batches; the gradient goes through them backwards, so the last is still in registers and the others in cache
+//   more          a group of 16 to 1024 lanes per row, 16 or 32 bytes a lane at a time; a row of one such batch stays in registers between the sums
+//                 and the gradient
+//   very long     the same in several batches; the gradient goes through them backwards: the last is still in registers, those before it in LDS, and
+//                 only what is left is read from memory again
 #include "learner.h"
 
 #include <algorithm>
@@ -469,11 +470,14 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
 // ---- more columns: a group of G lanes per row -----------------------------------------------------------------------------------------------------
 
 template <class E, int G, int CH, bool REF, class Op>
-__global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
+__global__ __launch_bounds__(G > BLOCK ? G : BLOCK, 4) void long_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
     constexpr int N = Chunk<E>::N, THREADS = G > BLOCK ? G : BLOCK, PER_BLOCK = THREADS / G, SPAN = G * CH * N;  // columns of a batch
     const int g = threadIdx.x % G, lane = threadIdx.x % WAVE;
     __shared__ float wave_stats[2][G > WAVE ? G / WAVE : 1][6];
+    // a lane's own columns of the last batches but one stay in LDS, 128 bytes of it a lane, and are not read from memory again for the gradient
+    constexpr int KEPT = Op::GRADIENT && G >= 4 * WAVE ? 8 / (CH * (REF ? 2 : 1)) : 0;
+    __shared__ Bits kept[KEPT ? KEPT : 1][REF ? 2 : 1][KEPT ? CH : 1][KEPT ? G : 1];
     if (op.done()) return;
     op.begin(p);
     Sums sums;
@@ -539,6 +543,15 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
             for (int b = 0; b < batches; b++) {
                 take(b);
                 if (b + 1 < batches) load(b + 1);
+                if constexpr (KEPT > 0) {
+                    if (out && b < batches - 1 && b >= batches - 1 - KEPT) {
+#pragma unroll
+                        for (int i = 0; i < CH; i++) {
+                            kept[batches - 2 - b][0][i][g] = l[i].w;
+                            if constexpr (REF) kept[batches - 2 - b][1][i][g] = l2[i].w;
+                        }
+                    }
+                }
                 float to = x.m, to2 = x.m2;
 #pragma unroll
                 for (int i = 0; i < CH; i++)
@@ -569,7 +582,7 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
                 if (REF) x.m2 = __shfl(x.m2, 0, WAVE), x.s2 = __shfl(x.s2, 0, WAVE), x.u = __shfl(x.u, 0, WAVE);
                 odd ^= 1;
             }
-            if (Op::GRADIENT && out && batches > 1) load(batches - 2);  // the first batch that is needed again
+            if (Op::GRADIENT && out && batches > 1 + KEPT) load(batches - 2 - KEPT);  // the first batch that has to be read again
             some = op.template finish<REF>(r, in, x, known, taken, g == 0, c, sums);
             forget();
         }
@@ -583,7 +596,15 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK) void long_rows(procgen_amd_r
             continue;
         }
         for (int b = batches - 1; b >= 0; b--) {
-            if (b < batches - 1) {
+            if (KEPT && b < batches - 1 && b >= batches - 1 - KEPT) {
+                if constexpr (KEPT > 0) {
+#pragma unroll
+                    for (int i = 0; i < CH; i++) {
+                        l[i].w = kept[batches - 2 - b][0][i][g];
+                        if constexpr (REF) l2[i].w = kept[batches - 2 - b][1][i][g];
+                    }
+                }
+            } else if (b < batches - 1) {
                 take(b);
                 if (b > 0) load(b - 1);
             }
@@ -707,8 +728,10 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
         long_rows<E, 16, 2, REF, Op><<<grid(BLOCK / 16, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.columns <= 64 * 2 * N) {
         long_rows<E, 64, 2, REF, Op><<<grid(BLOCK / 64, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (p.rows >= 2 * CUS || p.columns <= 256 * 4 * N) {
+    } else if (p.columns <= 256 * 2 * N || (p.rows >= 2 * CUS && !(REF && p.d_logits))) {
         long_rows<E, 256, 2, REF, Op><<<grid(1, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (p.rows >= 2 * CUS) {  // 2048 x 50021 bf16 with a reference: 154 us, against 173 with 256 lanes and two chunks, 179 with 1024
+        long_rows<E, 512, 1, REF, Op><<<grid(1, CUS * 2), 512, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else {  // too few rows to fill the card: more lanes for each
         long_rows<E, 1024, 2, REF, Op><<<grid(1, CUS), 1024, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     }
