@@ -378,12 +378,13 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
     Tile<E, MOST> next;
     Tile<E, REF ? MOST : 8> next2;
     typename Op::In next_in;
-    long long next_a = 0;
+    int next_a = -1;  // -1: not one of the columns
     auto fetch = [&](long long r0) {
         const int rows = (int)min((long long)WAVE, p.rows - r0);
         const long long r = r0 + min(lane, rows - 1);
         next_in = op.fetch(r);
-        next_a = action_of(p, r);
+        const long long a = action_of(p, r);
+        next_a = a >= 0 && a < columns ? (int)a : -1;
         next.fetch(p, p.logits, p.outer_stride, r0, rows, lane);
         if (REF) next2.fetch(p, ref, ref_outer, r0, rows, lane);
     };
@@ -392,7 +393,8 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
     for (; r0 < p.rows; r0 += step) {
         const int rows = (int)min((long long)WAVE, p.rows - r0);
         const bool mine = lane < rows;
-        const long long r = mine ? r0 + lane : r0, a = next_a;
+        const long long r = mine ? r0 + lane : r0;
+        const int a = next_a;
         const typename Op::In in = next_in;
         const bool wanted = mine && op.wanted(in);
         next.put(tile, p, p.logits, p.outer_stride, p.inner_stride, r0, rows, lane);
@@ -430,7 +432,7 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
                     x.u += product(e[j], l[j] - l2[j]);
                 }
             }
-            const bool known = a >= 0 && a < columns;
+            const bool known = a >= 0;
             const float taken = known ? (float)row[a] : 0.f, taken2 = REF && known ? (float)row2[a] : 0.f;
             some = op.template finish<REF>(r, in, x, known, taken, true, c, sums);
             if (Op::GRADIENT && some && p.d_logits) {
