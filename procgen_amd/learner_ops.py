@@ -14,7 +14,9 @@ Tensors may be strided (batch-major windows, slices, expanded dimensions); argum
 before anything runs.  Element types: float32, float16, bfloat16; sums, states and statistics are held in 32 bits or more.
 """
 import ctypes as C
+import functools
 import os
+import struct
 from typing import NamedTuple
 
 import torch
@@ -24,35 +26,13 @@ from .env import DEFAULT_LIB_DIR
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # enum procgen_amd_dtype
 
-
-class _Array3(C.Structure):  # struct procgen_amd_array3
-    _fields_ = [("data", C.c_void_p), ("t_stride", C.c_longlong), ("n_stride", C.c_longlong), ("d_stride", C.c_longlong)]
-
-
-class _Recurrence(C.Structure):  # struct procgen_amd_recurrence
-    _fields_ = [("dtype", C.c_int), ("T", C.c_int), ("N", C.c_int), ("D", C.c_int), ("gate", _Array3), ("update", _Array3), ("h", _Array3),
-                ("first", C.c_void_p), ("first_t_stride", C.c_longlong), ("first_n_stride", C.c_longlong), ("state", C.c_void_p), ("state_out", C.c_void_p),
-                ("checkpoints", C.c_void_p), ("workspace", C.c_void_p), ("d_h", _Array3), ("d_gate", _Array3), ("d_update", _Array3),
-                ("d_state_out", C.c_void_p), ("d_state", C.c_void_p)]
-
-
-class _Advantage(C.Structure):  # struct procgen_amd_advantage
-    _fields_ = [("dtype", C.c_int), ("T", C.c_int), ("N", C.c_int), ("rew", C.c_void_p), ("rew_t_stride", C.c_longlong), ("rew_n_stride", C.c_longlong),
-                ("values", C.c_void_p), ("values_t_stride", C.c_longlong), ("values_n_stride", C.c_longlong),
-                ("first", C.c_void_p), ("first_t_stride", C.c_longlong), ("first_n_stride", C.c_longlong), ("gamma", C.c_float), ("lam", C.c_float),
-                ("adv", C.c_void_p), ("ret", C.c_void_p), ("workspace", C.c_void_p)]
-
-
-class _Rows(C.Structure):  # struct procgen_amd_rows
-    _fields_ = [("dtype", C.c_int), ("rows", C.c_longlong), ("columns", C.c_longlong), ("inner", C.c_longlong), ("logits", C.c_void_p),
-                ("outer_stride", C.c_longlong), ("inner_stride", C.c_longlong), ("actions", C.c_void_p), ("actions_are_64_bit", C.c_int),
-                ("d_logits", C.c_void_p), ("workspace", C.c_void_p)]
-
-
-class _Policy(C.Structure):  # struct procgen_amd_policy
-    _fields_ = [("old_logprobs", C.c_void_p), ("adv", C.c_void_p), ("valid", C.c_void_p), ("ref_logits", C.c_void_p), ("ref_outer_stride", C.c_longlong),
-                ("ref_inner_stride", C.c_longlong), ("ref_logprobs", C.c_void_p), ("clip_low", C.c_float), ("clip_high", C.c_float), ("kl_coef", C.c_float),
-                ("entropy_coef", C.c_float), ("scale", C.c_void_p), ("loss", C.c_void_p), ("stats", C.c_void_p), ("resume", C.c_int)]
+# the C structs, packed field by field (native sizes and alignment; the closing 0P pads the end): a third of the time that filling a ctypes.Structure takes
+_ARRAY3 = "Pqqq"  # struct procgen_amd_array3: data, t_stride, n_stride, d_stride
+_RECURRENCE = struct.Struct("@4i" + 3 * _ARRAY3 + "Pqq4P" + 3 * _ARRAY3 + "2P" + "0P")
+_ADVANTAGE = struct.Struct("@3iPqqPqqPqqff3P" + "0P")
+_ROWS = struct.Struct("@iqqqPqqPiPP" + "0P")
+_POLICY = struct.Struct("@4PqqP4f3Pi" + "0P")
+_NO_ARRAY = (0, 0, 0, 0)
 
 
 class _Library:
@@ -65,9 +45,11 @@ class _Library:
         if self.lib is None:
             lib = C.CDLL(os.path.join(DEFAULT_LIB_DIR, "libenv.so"))
             P, I, L = C.c_void_p, C.c_int, C.c_longlong
-            for fn, res, args in (("recurrence_checkpoints", L, [I]), ("recurrence_workspace", L, [I, I, I]), ("recurrence_forward", I, [P, I, P]),
-                                  ("recurrence_backward", I, [P, I, P]), ("advantages", I, [P, I, P]), ("rows_workspace", L, [L, L]),
-                                  ("action_logprobs", I, [P, P, P, P, I, P]), ("action_logprobs_backward", I, [P, P, P, P, P, I, P]), ("policy_loss", I, [P, P, I, P]), ("capture_id", L, [P])):
+            S = C.c_char_p  # a packed struct
+            for fn, res, args in (("recurrence_checkpoints", L, [I]), ("recurrence_workspace", L, [I, I, I]), ("recurrence_forward", I, [S, I, P]),
+                                  ("recurrence_backward", I, [S, I, P]), ("advantages", I, [S, I, P]), ("rows_workspace", L, [L, L]),
+                                  ("action_logprobs", I, [S, P, P, P, I, P]), ("action_logprobs_backward", I, [S, P, P, P, P, I, P]), ("policy_loss", I, [S, S, I, P]),
+                                  ("capture_id", L, [P])):
                 f = getattr(lib, "procgen_amd_" + fn)
                 f.restype, f.argtypes = res, args
                 setattr(self, fn, f)
@@ -77,10 +59,26 @@ class _Library:
 
 
 _lib = _Library()
+_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(device).cuda_stream without the Stream object
 
 
-def _run(fn, name, device, *args):
-    rc = fn(*args, device.index, torch.cuda.current_stream(device).cuda_stream)
+@functools.lru_cache(maxsize=1024)
+def _checkpoints(T):
+    return _lib.recurrence_checkpoints(T)
+
+
+@functools.lru_cache(maxsize=1024)
+def _recurrence_workspace(T, N, D):
+    return _lib.recurrence_workspace(T, N, D)
+
+
+@functools.lru_cache(maxsize=1024)
+def _rows_workspace(rows, columns):
+    return _lib.rows_workspace(rows, columns)
+
+
+def _run(fn, name, index, *args):
+    rc = fn(*args, index, _stream(index))
     if rc:
         raise RuntimeError(f"{name}: " + ("the library refused the arguments" if rc < 0 else f"HIP error {rc}"))
 
@@ -91,35 +89,53 @@ def _need(ok, message, kind=ValueError):
 
 
 def _tensor(x, what, dtypes, shape=None):
-    _need(isinstance(x, torch.Tensor), f"{what} has to be a tensor", TypeError)
-    _need(x.dtype in dtypes, f"{what} has to be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, not {x.dtype}", TypeError)
-    _need(shape is None or tuple(x.shape) == tuple(shape), f"{what} has to have the shape {tuple(shape) if shape is not None else ''}, not {tuple(x.shape)}")
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what} has to be a tensor")
+    if x.dtype not in dtypes:
+        raise TypeError(f"{what} has to be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, not {x.dtype}")
+    if shape is not None and x.shape != shape:
+        raise ValueError(f"{what} has to have the shape {tuple(shape)}, not {tuple(x.shape)}")
 
 
-def _on_gpu(*tensors):
+def _on_gpu(x, *others):
     """the one device all of them are on"""
-    device = tensors[0].device
-    _need(device.type == "cuda", f"the learner operators run on the GPU only: a tensor is on {device}")
-    for x in tensors:
-        _need(x is None or x.device == device, f"the tensors are on different devices ({device} and {x.device if x is not None else ''})")
+    device = x.device
+    if device.type != "cuda":
+        raise ValueError(f"the learner operators run on the GPU only: a tensor is on {device}")
+    for y in others:
+        if y is not None and y.device != device:
+            raise ValueError(f"the tensors are on different devices ({device} and {y.device})")
     return device
 
 
 def _constant(x, what):
-    _need(x is None or not (x.requires_grad and torch.is_grad_enabled()), f"{what} is a constant to this operator and gets no gradient: detach it")
+    if x is not None and x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} is a constant to this operator and gets no gradient: detach it")
 
 
 def _number(x, what, low=float("-inf"), high=float("inf")):
-    _need(isinstance(x, (int, float)) and not isinstance(x, bool), f"{what} has to be a number", TypeError)
-    _need(low <= x <= high, f"{what} has to lie in [{low}, {high}], not {x}")
+    if not isinstance(x, (int, float)) or isinstance(x, bool):
+        raise TypeError(f"{what} has to be a number")
+    if not low <= x <= high:
+        raise ValueError(f"{what} has to lie in [{low}, {high}], not {x}")
 
 
 _FLAGS = (torch.uint8, torch.bool)
 _F32 = (torch.float32,)
+_INTS = (torch.int32, torch.int64)
+_FLOATS = tuple(_DTYPES)
+
+
+def _wants_grad(*tensors):
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                return True
+    return False
 
 
 def _array3(x):
-    return _Array3(x.data_ptr(), *x.stride())
+    return (x.data_ptr(), *x.stride())
 
 
 def _bytes(n, device):
@@ -127,65 +143,51 @@ def _bytes(n, device):
 
 
 def _ptr(x):
-    return None if x is None else x.data_ptr()
+    return 0 if x is None else x.data_ptr()
 
 
 # ---- the memory of a policy ------------------------------------------------------------------------------------------------------------------
 
 
-def _recurrence_args(gate, update, first, state, checkpoints):
-    T, N, D = gate.shape
-    a = _Recurrence(dtype=_DTYPES[gate.dtype], T=T, N=N, D=D, gate=_array3(gate), update=_array3(update), state=_ptr(state), checkpoints=_ptr(checkpoints))
-    if first is not None:
-        a.first, a.first_t_stride, a.first_n_stride = first.data_ptr(), first.stride(0), first.stride(1)
-    work = _bytes(_lib.recurrence_workspace(T, N, D), gate.device)
-    a.workspace = _ptr(work)
-    return a, work
+def _recurrence_args(gate, update, h, first, state, state_out, checkpoints, work, backward=3 * _NO_ARRAY + (0, 0)):
+    flags = (first.data_ptr(), *first.stride()) if first is not None else (0, 0, 0)
+    return _RECURRENCE.pack(_DTYPES[gate.dtype], *gate.shape, *_array3(gate), *_array3(update), *h, *flags, _ptr(state), _ptr(state_out), _ptr(checkpoints), _ptr(work), *backward)
 
 
 def _recurrence_forward(gate, update, first, state, state_out, checkpoints=None):
     h = torch.empty_like(update)
-    last = state_out if state_out is not None else torch.empty(gate.shape[1:], dtype=torch.float32, device=gate.device)
-    a, work = _recurrence_args(gate, update, first, state, checkpoints)
-    a.h, a.state_out = _array3(h), last.data_ptr()
-    _run(_lib.recurrence_forward, "gated_recurrence", gate.device, C.addressof(a))
+    device = gate.device
+    last = state_out if state_out is not None else torch.empty(gate.shape[1:], dtype=torch.float32, device=device)
+    work = _bytes(_recurrence_workspace(*gate.shape), device)
+    _run(_lib.recurrence_forward, "gated_recurrence", device.index, _recurrence_args(gate, update, _array3(h), first, state, last, checkpoints, work))
     return h, last
 
 
 class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, update, first, state):
-        checkpoints = torch.empty((_lib.recurrence_checkpoints(gate.shape[0]), *gate.shape[1:]), dtype=torch.float32, device=gate.device)
+        T, N, D = gate.shape
+        checkpoints = torch.empty((_checkpoints(T), N, D), dtype=torch.float32, device=gate.device)
         h, last = _recurrence_forward(gate, update, first, state, None, checkpoints)
         ctx.save_for_backward(gate, update, first, state, checkpoints)
+        ctx.set_materialize_grads(False)
         return h, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_h, d_last):
         gate, update, first, state, checkpoints = ctx.saved_tensors
-        a, work = _recurrence_args(gate, update, first, state, checkpoints)
-        d_gate = d_update = d_state = None
-        if d_h is not None:
-            a.d_h = _array3(d_h)
+        wanted = ctx.needs_input_grad
+        d_gate = torch.empty_like(gate) if wanted[0] else None
+        d_update = torch.empty_like(update) if wanted[1] else None
+        d_state = torch.empty_like(state) if wanted[3] else None
         if d_last is not None:
             d_last = d_last.contiguous()
-            a.d_state_out = d_last.data_ptr()
-        if ctx.needs_input_grad[0]:
-            d_gate = torch.empty_like(gate)
-            a.d_gate = _array3(d_gate)
-        if ctx.needs_input_grad[1]:
-            d_update = torch.empty_like(update)
-            a.d_update = _array3(d_update)
-        if ctx.needs_input_grad[3]:
-            d_state = torch.empty_like(state)
-            a.d_state = d_state.data_ptr()
-        _run(_lib.recurrence_backward, "gated_recurrence", gate.device, C.addressof(a))
+        work = _bytes(_recurrence_workspace(*gate.shape), gate.device)
+        arrays = [_NO_ARRAY if x is None else _array3(x) for x in (d_h, d_gate, d_update)]
+        a = _recurrence_args(gate, update, _NO_ARRAY, first, state, None, checkpoints, work, (*arrays[0], *arrays[1], *arrays[2], _ptr(d_last), _ptr(d_state)))
+        _run(_lib.recurrence_backward, "gated_recurrence", gate.device.index, a)
         return d_gate, d_update, None, d_state
-
-
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors)
 
 
 def gated_recurrence(gate, update, first=None, state=None, state_out=None):
@@ -196,21 +198,21 @@ def gated_recurrence(gate, update, first=None, state=None, state_out=None):
     gate, update: [T, N, D] (or [T, N]) float32, float16 or bfloat16, any strides; first: [T, N] uint8 or bool, None: no episode begins; state:
     float32 [N, D] (or [N]), None: zeros.  state_out: a float32 buffer that takes the new state, `state` itself to move it on in place; only without
     gradients.  Differentiable in gate, update and state, once."""
-    _tensor(gate, "gate", tuple(_DTYPES))
-    _need(gate.dim() in (2, 3), f"gate has to be [T, N, D] or [T, N], not {tuple(gate.shape)}")
-    _tensor(update, "update", (gate.dtype,), gate.shape)
-    lead, per_env = gate.shape[:2], gate.shape[1:]
+    _tensor(gate, "gate", _FLOATS)
+    shape = gate.shape
+    if len(shape) not in (2, 3):
+        raise ValueError(f"gate has to be [T, N, D] or [T, N], not {tuple(shape)}")
+    _tensor(update, "update", (gate.dtype,), shape)
     if first is not None:
-        _tensor(first, "first", _FLAGS, lead)
+        _tensor(first, "first", _FLAGS, shape[:2])
     if state is not None:
-        _tensor(state, "state", _F32, per_env)
+        _tensor(state, "state", _F32, shape[1:])
     if state_out is not None:
-        _tensor(state_out, "state_out", _F32, per_env)
+        _tensor(state_out, "state_out", _F32, shape[1:])
         _need(state_out.is_contiguous(), "state_out has to be contiguous")
-        _need(not _wants_grad(gate, update, state, state_out),
-              "state_out overwrites a state: call under torch.no_grad(), or take the returned state")
+        _need(not _wants_grad(gate, update, state, state_out), "state_out overwrites a state: call under torch.no_grad(), or take the returned state")
     _on_gpu(gate, update, first, state, state_out)
-    flat = gate.dim() == 2
+    flat = len(shape) == 2
     if flat:
         gate, update = gate.unsqueeze(2), update.unsqueeze(2)
         state = state.unsqueeze(1) if state is not None else None
@@ -243,7 +245,7 @@ def advantages(rew, values, first, *, gamma, lam):
     _tensor(rew, "rew", _F32)
     _need(rew.dim() == 2, f"rew has to be [T, N], not {tuple(rew.shape)}")
     T, N = rew.shape
-    _tensor(values, "values", tuple(_DTYPES), (T + 1, N))
+    _tensor(values, "values", _FLOATS, (T + 1, N))
     _tensor(first, "first", _FLAGS, (T + 1, N))
     _number(gamma, "gamma", 0.0, 1.0)
     _number(lam, "lam", 0.0, 1.0)
@@ -253,11 +255,10 @@ def advantages(rew, values, first, *, gamma, lam):
     adv = torch.empty((T, N), dtype=torch.float32, device=device)
     ret = torch.empty((T, N), dtype=torch.float32, device=device)
     if T and N:
-        a = _Advantage(_DTYPES[values.dtype], T, N, rew.data_ptr(), *rew.stride(), values.data_ptr(), *values.stride(), first.data_ptr(), *first.stride(),
-                       gamma, lam, adv.data_ptr(), ret.data_ptr(), None)
-        work = _bytes(_lib.recurrence_workspace(T, N, 1), device)
-        a.workspace = _ptr(work)
-        _run(_lib.advantages, "advantages", device, C.addressof(a))
+        work = _bytes(_recurrence_workspace(T, N, 1), device)
+        a = _ADVANTAGE.pack(_DTYPES[values.dtype], T, N, rew.data_ptr(), *rew.stride(), values.data_ptr(), *values.stride(), first.data_ptr(), *first.stride(), gamma, lam,
+                            adv.data_ptr(), ret.data_ptr(), _ptr(work))
+        _run(_lib.advantages, "advantages", device.index, a)
     return adv, ret
 
 
@@ -266,49 +267,55 @@ def advantages(rew, values, first, *, gamma, lam):
 
 def _layout(x, what):
     """(inner, outer stride, inner stride) of the rows of x [..., columns]: the leading dimensions as at most two strided ones"""
+    if x.is_contiguous():
+        return 1, x.shape[-1], 0
+    *lead, columns = zip(x.shape, x.stride())
+    if columns[0] != 1 and columns[1] != 1:
+        raise ValueError(f"the columns of {what} have to be contiguous")
     dims = []
-    for size, stride in zip(x.shape[:-1], x.stride()[:-1]):
+    for size, stride in lead:
         if size == 1:
             continue
         if dims and dims[-1][1] == stride * size:
             dims[-1] = (dims[-1][0] * size, stride)
         else:
             dims.append((size, stride))
-    _need(x.shape[-1] == 1 or x.stride(-1) == 1, f"the columns of {what} have to be contiguous")
-    _need(len(dims) <= 2, f"the leading dimensions of {what} are strided in more than two ways: make it contiguous")
+    if len(dims) > 2:
+        raise ValueError(f"the leading dimensions of {what} are strided in more than two ways: make it contiguous")
     if len(dims) == 2:
         return dims[1][0], dims[0][1], dims[1][1]
     return 1, dims[0][1] if dims else 0, 0
 
 
-def _rows(logits, actions):
-    inner, outer_stride, inner_stride = _layout(logits, "logits")
+def _rows(logits, layout, actions, d_logits=None, work=None):
+    inner, outer_stride, inner_stride = layout
     columns = logits.shape[-1]
-    return _Rows(_DTYPES[logits.dtype], logits.numel() // columns, columns, max(1, inner), logits.data_ptr(), outer_stride, inner_stride, actions.data_ptr(), actions.dtype == torch.int64)
+    return _ROWS.pack(_DTYPES[logits.dtype], logits.numel() // columns, columns, inner or 1, logits.data_ptr(), outer_stride, inner_stride, actions.data_ptr(),
+                      actions.dtype == torch.int64, _ptr(d_logits), _ptr(work))
 
 
 def _check_rows(logits, actions):
-    _tensor(logits, "logits", tuple(_DTYPES))
-    _need(logits.dim() >= 1 and logits.shape[-1] >= 1, "logits have to be [..., columns] with one column at least")
-    _tensor(actions, "actions", (torch.int32, torch.int64), logits.shape[:-1])
+    _tensor(logits, "logits", _FLOATS)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits have to be [..., columns] with one column at least")
+    _tensor(actions, "actions", _INTS, logits.shape[:-1])
 
 
-def _action_logprobs(logits, actions, grad):
-    device = logits.device
-    logp, entropy = (torch.empty(logits.shape[:-1], dtype=torch.float32, device=device) for _ in range(2))
-    lse = torch.empty_like(logp) if grad else None
-    a = _rows(logits, actions)
-    work = _bytes(_lib.rows_workspace(a.rows, a.columns), device)
-    a.workspace = work.data_ptr()
-    _run(_lib.action_logprobs, "action_logprobs", device, C.addressof(a), logp.data_ptr(), entropy.data_ptr(), _ptr(lse))
+def _action_logprobs(logits, layout, actions, grad):
+    device, lead = logits.device, logits.shape[:-1]
+    logp = torch.empty(lead, dtype=torch.float32, device=device)
+    entropy = torch.empty(lead, dtype=torch.float32, device=device)
+    lse = torch.empty(lead, dtype=torch.float32, device=device) if grad else None
+    _run(_lib.action_logprobs, "action_logprobs", device.index, _rows(logits, layout, actions), logp.data_ptr(), entropy.data_ptr(), _ptr(lse))
     return logp, entropy, lse
 
 
 class _ActionLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, actions):
-        logp, entropy, lse = _action_logprobs(logits, actions, True)
+    def forward(ctx, logits, layout, actions):
+        logp, entropy, lse = _action_logprobs(logits, layout, actions, True)
         ctx.save_for_backward(logits, actions, lse, entropy)
+        ctx.set_materialize_grads(False)
         return logp, entropy
 
     @staticmethod
@@ -316,11 +323,11 @@ class _ActionLogprobs(torch.autograd.Function):
     def backward(ctx, d_logp, d_entropy):
         logits, actions, lse, entropy = ctx.saved_tensors
         d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        a = _rows(logits, actions)
-        a.d_logits = d_logits.data_ptr()
-        d_logp, d_entropy = (None if x is None else x.contiguous() for x in (d_logp, d_entropy))
-        _run(_lib.action_logprobs_backward, "action_logprobs", logits.device, C.addressof(a), lse.data_ptr(), entropy.data_ptr(), _ptr(d_logp), _ptr(d_entropy))
-        return d_logits, None
+        d_logp = None if d_logp is None else d_logp.contiguous()
+        d_entropy = None if d_entropy is None else d_entropy.contiguous()
+        _run(_lib.action_logprobs_backward, "action_logprobs", logits.device.index, _rows(logits, _layout(logits, "logits"), actions, d_logits), lse.data_ptr(), entropy.data_ptr(),
+             _ptr(d_logp), _ptr(d_entropy))
+        return d_logits, None, None
 
 
 def action_logprobs(logits, actions):
@@ -331,14 +338,14 @@ def action_logprobs(logits, actions):
     reset -- has no log-probability: NaN, and a NaN gradient unless its gradients coming in are zero.  Differentiable in logits, once."""
     _check_rows(logits, actions)
     _on_gpu(logits, actions)
-    _layout(logits, "logits")
+    layout = _layout(logits, "logits")
     if logits.numel() == 0:
         empty = logits.sum(-1, dtype=torch.float32)
         return empty, empty * 1
     actions = actions.contiguous()
     if _wants_grad(logits):
-        return _ActionLogprobs.apply(logits, actions)
-    return _action_logprobs(logits, actions, False)[:2]
+        return _ActionLogprobs.apply(logits, layout, actions)
+    return _action_logprobs(logits, layout, actions, False)[:2]
 
 
 class PolicyLoss(NamedTuple):
@@ -346,35 +353,32 @@ class PolicyLoss(NamedTuple):
     stats: torch.Tensor  # float32 [4]: the means of -objective, KL, entropy and of (ratio outside the clip range), constants
 
 
-def _policy_args(coefs, work, logits, actions, old, adv, valid, ref_logits, ref_logprobs):
-    a = _rows(logits, actions)
-    a.workspace = work.data_ptr()
-    clip, kl_coef, entropy_coef = coefs
-    q = _Policy(old.data_ptr(), adv.data_ptr(), _ptr(valid), _ptr(ref_logits), 0, 0, _ptr(ref_logprobs), *clip, kl_coef, entropy_coef)
-    if ref_logits is not None:
-        (a.inner, a.outer_stride, a.inner_stride), (_, q.ref_outer_stride, q.ref_inner_stride) = _common_layout(logits, ref_logits)
-    return a, q
+def _policy_args(coefs, work, d_logits, logits, actions, old, adv, valid, ref_logits, ref_logprobs, scale=None, loss=None, stats=None, resume=0):
+    if ref_logits is None:
+        layout, ref_strides = _layout(logits, "logits"), (0, 0)
+    else:
+        layout, (_, *ref_strides) = _common_layout(logits, ref_logits)
+    return (_rows(logits, layout, actions, d_logits, work),
+            _POLICY.pack(old.data_ptr(), adv.data_ptr(), _ptr(valid), _ptr(ref_logits), *ref_strides, _ptr(ref_logprobs), *coefs, _ptr(scale), _ptr(loss), _ptr(stats), resume))
 
 
 def _policy_forward(coefs, d_logits, *tensors):
     logits = tensors[0]
     device, columns = logits.device, logits.shape[-1]
     loss, stats = torch.empty((), dtype=torch.float32, device=device), torch.empty(4, dtype=torch.float32, device=device)
-    work = _bytes(_lib.rows_workspace(logits.numel() // columns, columns), device)
-    a, q = _policy_args(coefs, work, *tensors)
-    a.d_logits, q.loss, q.stats = _ptr(d_logits), loss.data_ptr(), stats.data_ptr()
-    _run(_lib.policy_loss, "policy_loss", device, C.addressof(a), C.addressof(q))
+    work = _bytes(_rows_workspace(logits.numel() // columns, columns), device)
+    _run(_lib.policy_loss, "policy_loss", device.index, *_policy_args(coefs, work, d_logits, *tensors, loss=loss, stats=stats))
     return loss, stats, work
 
 
 def _capture(device):
-    return _lib.capture_id(torch.cuda.current_stream(device).cuda_stream)
+    return _lib.capture_id(_stream(device.index))
 
 
 class _PolicyLoss(torch.autograd.Function):
     """The forward call writes the gradient too, from the row that it has in registers.  The first backward pass hands it out, after a kernel that goes
-    over the rows again only where the loss's own gradient is not 1; each further one (retain_graph)
-    computes its own, and so does a backward pass that is captured apart from its forward call."""
+    over the rows again only where the loss's own gradient is not 1; each further one (retain_graph) computes its own, and so does a backward pass that
+    is captured apart from its forward call."""
 
     @staticmethod
     def forward(ctx, coefs, *tensors):
@@ -389,21 +393,19 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss, _):
-        logits = ctx.saved_tensors[0]
-        d_logits, ctx.d_logits = ctx.d_logits, None
-        a, q = _policy_args(ctx.coefs, ctx.work, *ctx.saved_tensors)
-        q.resume = 1
-        if d_logits is not None and ctx.capture == _capture(logits.device) >= 0:
-            q.resume = 3
-        else:
-            d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        a.d_logits, q.scale = d_logits.data_ptr(), d_loss.data_ptr()
-        _run(_lib.policy_loss, "policy_loss", logits.device, C.addressof(a), C.addressof(q))
-        return (None, d_logits) + (None,) * 6
+        tensors = ctx.saved_tensors
+        logits = tensors[0]
+        d_logits, ctx.d_logits, resume = ctx.d_logits, None, 3
+        if d_logits is None or not ctx.capture == _capture(logits.device) >= 0:
+            d_logits, resume = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), 1
+        _run(_lib.policy_loss, "policy_loss", logits.device.index, *_policy_args(ctx.coefs, ctx.work, d_logits, *tensors, scale=d_loss, resume=resume))
+        return None, d_logits, None, None, None, None, None, None
 
 
 def _common_layout(x, y):
     """the rows of two equally shaped tensors under one split of their leading dimensions, or ValueError"""
+    if x.is_contiguous() and y.is_contiguous():
+        return (1, x.shape[-1], 0), (1, x.shape[-1], 0)
     lead = x.shape[:-1]
     for k in range(len(lead) + 1):
         got = []
@@ -436,10 +438,12 @@ def policy_loss(logits, actions, old_logprobs, advantages, *, clip=0.2, kl_coef=
     column counts, with nothing to add.  Only the logits get a gradient, once."""
     _check_rows(logits, actions)
     lead = logits.shape[:-1]
-    for x, what in ((old_logprobs, "old_logprobs"), (advantages, "advantages"), (ref_logprobs, "ref_logprobs")):
-        if x is not None or what != "ref_logprobs":
-            _tensor(x, what, _F32, lead)
+    for x, what in ((old_logprobs, "old_logprobs"), (advantages, "advantages")):
+        _tensor(x, what, _F32, lead)
         _constant(x, what)
+    if ref_logprobs is not None:
+        _tensor(ref_logprobs, "ref_logprobs", _F32, lead)
+        _constant(ref_logprobs, "ref_logprobs")
     if valid is not None:
         _tensor(valid, "valid", _FLAGS, lead)
     if ref_logits is not None:
@@ -456,8 +460,7 @@ def policy_loss(logits, actions, old_logprobs, advantages, *, clip=0.2, kl_coef=
     _layout(logits, "logits")
     if ref_logits is not None:
         _layout(ref_logits, "ref_logits")
-        _common_layout(logits, ref_logits)
     actions, old_logprobs, advantages, valid, ref_logprobs = (None if x is None else x.contiguous() for x in (actions, old_logprobs, advantages, valid, ref_logprobs))
-    coefs = (float(low), float(high)), float(kl_coef), float(entropy_coef)
+    coefs = float(low), float(high), float(kl_coef), float(entropy_coef)
     tensors = logits, actions, old_logprobs, advantages, valid, ref_logits, ref_logprobs
     return PolicyLoss(*(_PolicyLoss.apply(coefs, *tensors) if _wants_grad(logits) else _policy_forward(coefs, None, *tensors)[:2]))

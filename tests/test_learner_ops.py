@@ -29,15 +29,14 @@ def test_library_exports_every_declared_symbol():
         assert hasattr(lib, s), f"libenv.so does not export {s}"
 
 
-def test_struct_sizes_of_the_ctypes_mirror(tmp_path):
-    names = {"procgen_amd_array3": ops._Array3, "procgen_amd_recurrence": ops._Recurrence, "procgen_amd_advantage": ops._Advantage, "procgen_amd_rows": ops._Rows,
-             "procgen_amd_policy": ops._Policy}
+def test_struct_sizes_of_the_packed_mirrors(tmp_path):
+    names = {"procgen_amd_recurrence": ops._RECURRENCE, "procgen_amd_advantage": ops._ADVANTAGE, "procgen_amd_rows": ops._ROWS, "procgen_amd_policy": ops._POLICY}
     body = "".join('printf("%%zu\\n", sizeof(struct %s));' % n for n in names)
     src = tmp_path / "sizes.c"
     src.write_text('#include <stdio.h>\n#include "%s/include/procgen_amd_learner.h"\nint main(void) { %s return 0; }\n' % (REPO, body))
     subprocess.check_call(["gcc", str(src), "-o", str(tmp_path / "sizes")])
     got = [int(x) for x in subprocess.check_output([str(tmp_path / "sizes")]).split()]
-    assert got == [C.sizeof(t) for t in names.values()]
+    assert got == [t.size for t in names.values()]
 
 
 def test_c_entries_refuse_what_they_cannot_run():
@@ -45,21 +44,23 @@ def test_c_entries_refuse_what_they_cannot_run():
     if not os.path.exists(HIP_LIB):
         pytest.skip("libenv.so not built (run __graft_entry__.build())")
     lib = C.CDLL(HIP_LIB)
-    ref = C.byref
-    a = ops._Recurrence(dtype=7, T=1, N=1, D=1)
-    assert lib.procgen_amd_recurrence_forward(ref(a), 0, None) == -1
-    a = ops._Recurrence(dtype=0, T=0, N=1, D=1)
-    assert lib.procgen_amd_recurrence_forward(ref(a), 0, None) == -1 and lib.procgen_amd_recurrence_backward(ref(a), 0, None) == -1
-    a = ops._Recurrence(dtype=0, T=4, N=1, D=1)  # no arrays
-    assert lib.procgen_amd_recurrence_forward(ref(a), 0, None) == -1 and lib.procgen_amd_recurrence_backward(ref(a), 0, None) == -1
-    v = ops._Advantage(dtype=0, T=4, N=4)
-    assert lib.procgen_amd_advantages(ref(v), 0, None) == -1
-    r = ops._Rows(dtype=0, rows=4, columns=0, inner=1)
-    assert lib.procgen_amd_action_logprobs(ref(r), None, None, None, 0, None) == -1
-    r = ops._Rows(dtype=0, rows=4, columns=3, inner=1)
-    assert lib.procgen_amd_action_logprobs(ref(r), None, None, None, 0, None) == -1
-    assert lib.procgen_amd_action_logprobs_backward(ref(r), None, None, None, None, 0, None) == -1
-    assert lib.procgen_amd_policy_loss(ref(r), ref(ops._Policy()), 0, None) == -1
+    zeros = bytes(1024)
+
+    def recurrence(dtype, T):
+        return ops._RECURRENCE.pack(dtype, T, 1, 1, *[0] * 33)
+
+    assert lib.procgen_amd_recurrence_forward(recurrence(7, 1), 0, None) == -1
+    for T in (0, 4):  # no step; no arrays
+        assert lib.procgen_amd_recurrence_forward(recurrence(0, T), 0, None) == -1 and lib.procgen_amd_recurrence_backward(recurrence(0, T), 0, None) == -1
+    assert lib.procgen_amd_advantages(ops._ADVANTAGE.pack(0, 4, 4, *[0] * 14), 0, None) == -1
+
+    def rows(columns):
+        return ops._ROWS.pack(0, 4, columns, 1, *[0] * 7)
+
+    for columns in (0, 3):
+        assert lib.procgen_amd_action_logprobs(rows(columns), None, None, None, 0, None) == -1
+        assert lib.procgen_amd_action_logprobs_backward(rows(columns), None, None, None, None, 0, None) == -1
+        assert lib.procgen_amd_policy_loss(rows(columns), zeros, 0, None) == -1
     assert lib.procgen_amd_policy_loss(None, None, 0, None) == -1
 
 
@@ -106,11 +107,11 @@ def test_refusals(kind, call):
 
 def test_layouts():
     x = torch.zeros(6, 5, 4, 8)
-    assert ops._layout(x, "x") == (1, 8, 0)
+    assert ops._layout(x, "x") == (1, 8, 0)  # (rows per inner group, stride of the groups, stride inside)
     assert ops._layout(x[:, :3], "x") == (12, 160, 8)
     assert ops._layout(x.transpose(0, 1)[0], "x") == (4, 160, 8)
     assert ops._layout(torch.zeros(7, 3)[:, :2], "x") == (1, 3, 0)
-    assert ops._layout(torch.zeros(3), "x") == (1, 0, 0)
+    assert ops._layout(torch.zeros(3), "x") == (1, 3, 0)
     assert ops._layout(torch.zeros(1, 3).expand(5, 3), "x") == (1, 0, 0)
     with pytest.raises(ValueError):
         ops._layout(x[:, :3, :2], "x")
