@@ -163,7 +163,7 @@ struct Coef {
 // Each operator's rows: what it fetches for a row besides its logits, whether it wants the row at all, what it makes of the row's sums.  finish() is
 // called once per row by one lane at least, with `first` set in exactly one; it returns whether the row's gradient is anything but zero.
 struct Logprobs {
-    static constexpr bool GRADIENT = false, SUMS = false;
+    static constexpr bool GRADIENT = false;
     __device__ bool done() const { return false; }
     float *logp, *entropy, *lse;
     struct In {};
@@ -182,7 +182,7 @@ struct Logprobs {
 };
 
 struct LogprobsBackward {  // of rows short enough to sum up again
-    static constexpr bool GRADIENT = true, SUMS = false;
+    static constexpr bool GRADIENT = true;
     __device__ bool done() const { return false; }
     const float *d_logp, *d_entropy;
     struct In {
@@ -200,7 +200,7 @@ struct LogprobsBackward {  // of rows short enough to sum up again
 };
 
 struct Policy {
-    static constexpr bool GRADIENT = true, SUMS = true;
+    static constexpr bool GRADIENT = true;
     __device__ bool done() const { return (q.resume & 2) && *q.scale == 1.f; }  // the gradient that is there is the one that is wanted
     procgen_amd_policy q;
     const long long *counts;
@@ -246,8 +246,15 @@ struct Policy {
     }
 };
 
-// the block's sums, in a fixed order
-__device__ inline void put_sums(Sums x, double *partial) {
+// the loss and the four means, by one thread
+__device__ inline void put_means(const procgen_amd_policy &q, long long n, double *sum) {
+    for (int k = 0; k < 4; k++) sum[k] = n > 0 ? sum[k] / (double)n : 0.0;
+    *q.loss = (float)(sum[0] + (q.kl_coef != 0.f ? (double)q.kl_coef * sum[1] : 0.0) - (q.entropy_coef != 0.f ? (double)q.entropy_coef * sum[2] : 0.0));
+    for (int k = 0; k < 4; k++) q.stats[k] = (float)sum[k];
+}
+
+// the block's sums, in a fixed order; the only block of a launch makes the means of them
+__device__ inline void put_sums(Sums x, const Policy &op, double *partial) {
     __shared__ double part[BLOCK * 4 / WAVE][4];  // 1024 lanes at the most
     double v[4] = {x.policy, x.kl, x.entropy, x.clipped};
     for (int k = 0; k < 4; k++) v[k] = wave_reduce(v[k], Sum());
@@ -255,12 +262,17 @@ __device__ inline void put_sums(Sums x, double *partial) {
     if (threadIdx.x % WAVE == 0)
         for (int k = 0; k < 4; k++) part[threadIdx.x / WAVE][k] = v[k];
     __syncthreads();
-    if (threadIdx.x < 4) {
-        double y = 0;
-        for (unsigned w = 0; w < blockDim.x / WAVE; w++) y += part[w][threadIdx.x];
-        partial[(long long)blockIdx.x * 4 + threadIdx.x] = y;
+    if (threadIdx.x) return;
+    for (int k = 0; k < 4; k++) {
+        v[k] = 0;
+        for (unsigned w = 0; w < blockDim.x / WAVE; w++) v[k] += part[w][k];
     }
+    if (gridDim.x == 1) put_means(op.q, op.n, v);
+    else
+        for (int k = 0; k < 4; k++) partial[(long long)blockIdx.x * 4 + k] = v[k];
 }
+__device__ inline void put_sums(Sums, const Logprobs &, double *) {}
+__device__ inline void put_sums(Sums, const LogprobsBackward &, double *) {}
 
 // 16 bytes of a row in registers, as memory holds them
 typedef uint32_t Bits __attribute__((ext_vector_type(4)));
@@ -466,7 +478,7 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
             lds_settled();
         }
     }
-    if (Op::SUMS && partial) put_sums(sums, partial);
+    if (partial) put_sums(sums, op, partial);
 }
 
 // ---- more columns: a group of G lanes per row -----------------------------------------------------------------------------------------------------
@@ -623,7 +635,7 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK, 4) void long_rows(procgen_am
         if (a >= 0 && a < columns && (int)((a + ahead) / N) % G == g)  // by the lane that wrote the column just now
             out[a] = (T)(c.gradient<REF>((float)row[a], REF ? (float)row2[a] : 0.f) + c.pick);
     }
-    if (Op::SUMS && partial) put_sums(sums, partial);
+    if (partial) put_sums(sums, op, partial);
 }
 
 // the gradient of long rows' log-probabilities: lse and entropy are known, so every column stands for itself
@@ -699,13 +711,11 @@ __global__ __launch_bounds__(MEANS) void policy_means(procgen_amd_policy q, long
         for (int i = lane; i < count_blocks; i += WAVE) n += counts[i];
         n = wave_reduce(n, Sum());
     }
-    double mean[4] = {0, 0, 0, 0};
-    for (int i = 0; i < 4 && n > 0; i++) {
-        for (int w = 0; w < MEANS / WAVE; w++) mean[i] += part[w][i];
-        mean[i] /= (double)n;
-    }
-    if (lane == 0) *q.loss = (float)(mean[0] + (q.kl_coef != 0.f ? (double)q.kl_coef * mean[1] : 0.0) - (q.entropy_coef != 0.f ? (double)q.entropy_coef * mean[2] : 0.0));
-    if (lane < 4) q.stats[lane] = (float)mean[lane];
+    if (lane) return;
+    double sum[4] = {0, 0, 0, 0};
+    for (int i = 0; i < 4; i++)
+        for (int w = 0; w < MEANS / WAVE; w++) sum[i] += part[w][i];
+    put_means(q, n, sum);
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------------------------------------
@@ -719,13 +729,15 @@ template <class E, bool REF, class Op>
 int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long long ref_outer, long long ref_inner, double *partial, hipStream_t stream) {
     int blocks = 0;
     auto grid = [&](int per_block, int most) { return blocks = (int)std::min<long long>(most, (p.rows + per_block - 1) / per_block); };
+    // two rounds of one block, which ends with the means, cost less than a launch for them
+    auto short_grid = [&](int most) { return partial && p.rows <= 2 * BLOCK ? blocks = 1 : grid(BLOCK, most); };
     constexpr int N = Chunk<E>::N;
     if (p.columns <= 64) {
         const size_t lds = ((WAVE * p.columns * sizeof(typename E::T) + 15) & ~15ull) * (BLOCK / WAVE) * (REF ? 2 : 1);
-        if (p.columns <= 8) short_rows<E, 8, REF, Op><<<grid(BLOCK, CUS * short_residents<E, 8, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<grid(BLOCK, CUS * short_residents<E, 16, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if (p.columns <= 32) short_rows<E, 32, REF, Op><<<grid(BLOCK, CUS * short_residents<E, 32, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else short_rows<E, 64, REF, Op><<<grid(BLOCK, CUS * short_residents<E, 64, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        if (p.columns <= 8) short_rows<E, 8, REF, Op><<<short_grid(CUS * short_residents<E, 8, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<short_grid(CUS * short_residents<E, 16, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if (p.columns <= 32) short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else short_rows<E, 64, REF, Op><<<short_grid(CUS * short_residents<E, 64, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.columns <= 16 * 2 * N) {
         long_rows<E, 16, 2, REF, Op><<<grid(BLOCK / 16, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.columns <= 64 * 2 * N) {
@@ -815,7 +827,7 @@ LIBENV_API int procgen_amd_policy_loss(const struct procgen_amd_rows *p, const s
         });
         if (blocks < 0) return -1 - blocks;
     }
-    if (!q->loss) return 0;
+    if (!q->loss || blocks == 1) return 0;
     policy_means<<<1, MEANS, 0, (hipStream_t)stream>>>(*q, p->rows, counts, count_blocks, partial, blocks);
     return launched();
 }
