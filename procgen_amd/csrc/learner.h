@@ -50,6 +50,7 @@ struct OnDevice {
     int old = -1;
     hipError_t err;
     explicit OnDevice(int device) {
+        (void)hipGetLastError();  // what another call left behind (an event that was not ready, say) is not a launch's error
         err = hipGetDevice(&old);
         if (err == hipSuccess && old != device) err = hipSetDevice(device);
         else old = -1;

@@ -246,6 +246,14 @@ struct Policy {
     }
 };
 
+// lane 4 w + k of the first wave takes wave w's k-th sum; lanes 0 to 3 (and every fourth after them) return the totals
+__device__ inline double sum_of_waves(const double (*part)[4], int waves) {
+    const int lane = threadIdx.x;
+    double v = lane / 4 < waves ? part[lane / 4][lane % 4] : 0.0;
+    for (int d = WAVE / 2; d >= 4; d >>= 1) v += __shfl_xor(v, d, WAVE);
+    return v;
+}
+
 // the loss and the four means, by one thread
 __device__ inline void put_means(const procgen_amd_policy &q, long long n, double *sum) {
     for (int k = 0; k < 4; k++) sum[k] = n > 0 ? sum[k] / (double)n : 0.0;
@@ -262,11 +270,10 @@ __device__ inline void put_sums(Sums x, const Policy &op, double *partial) {
     if (threadIdx.x % WAVE == 0)
         for (int k = 0; k < 4; k++) part[threadIdx.x / WAVE][k] = v[k];
     __syncthreads();
+    if (threadIdx.x >= WAVE) return;
+    const double mine = sum_of_waves(part, blockDim.x / WAVE);
+    for (int k = 0; k < 4; k++) v[k] = __shfl(mine, k, WAVE);
     if (threadIdx.x) return;
-    for (int k = 0; k < 4; k++) {
-        v[k] = 0;
-        for (unsigned w = 0; w < blockDim.x / WAVE; w++) v[k] += part[w][k];
-    }
     if (gridDim.x == 1) put_means(op.q, op.n, v);
     else
         for (int k = 0; k < 4; k++) partial[(long long)blockIdx.x * 4 + k] = v[k];
@@ -681,6 +688,7 @@ __global__ __launch_bounds__(BLOCK) void count_valid(const uint8_t *valid, long 
     long long n = 0;
     const long long head = min(rows, (long long)(-(uintptr_t)valid & 15)), wide = (rows - head) / 16;  // bytes before the first aligned 16, and 16s
     const long long i = (long long)blockIdx.x * BLOCK + threadIdx.x, step = (long long)gridDim.x * BLOCK;
+#pragma unroll 4
     for (long long k = i; k < wide; k += step) {
         const uint4 v = ((const uint4 *)(valid + head))[k];
         const unsigned x[4] = {v.x, v.y, v.z, v.w};
@@ -699,6 +707,7 @@ constexpr int MEANS = 1024;
 __global__ __launch_bounds__(MEANS) void policy_means(procgen_amd_policy q, long long rows, const long long *counts, int count_blocks, const double *partial, int blocks) {
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, k = lane % 4;  // four neighbouring lanes: a block's four sums
     double v = 0;
+#pragma unroll 4
     for (int i = threadIdx.x / 4; i < blocks; i += MEANS / 4) v += partial[(long long)i * 4 + k];
     for (int d = WAVE / 2; d >= 4; d >>= 1) v += __shfl_xor(v, d, WAVE);
     __shared__ double part[MEANS / WAVE][4];
@@ -711,11 +720,10 @@ __global__ __launch_bounds__(MEANS) void policy_means(procgen_amd_policy q, long
         for (int i = lane; i < count_blocks; i += WAVE) n += counts[i];
         n = wave_reduce(n, Sum());
     }
-    if (lane) return;
-    double sum[4] = {0, 0, 0, 0};
-    for (int i = 0; i < 4; i++)
-        for (int w = 0; w < MEANS / WAVE; w++) sum[i] += part[w][i];
-    put_means(q, n, sum);
+    const double mine = sum_of_waves(part, MEANS / WAVE);
+    double sum[4];
+    for (int i = 0; i < 4; i++) sum[i] = __shfl(mine, i, WAVE);
+    if (lane == 0) put_means(q, n, sum);
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------------------------------------

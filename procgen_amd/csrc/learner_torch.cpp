@@ -70,6 +70,7 @@ std::pair<Tensor, Tensor> recurrence_forward(const Tensor &gate, const Tensor &u
     a.h = array3(h);
     a.state_out = data_as<float>(last);
     check(procgen_amd_recurrence_forward(&a, gate.get_device(), stream_of(gate)), "gated_recurrence");
+    if (state_out.defined()) torch::autograd::impl::bump_version(state_out);  // a graph that had saved it must not go on with the new values
     return {h, last};
 }
 

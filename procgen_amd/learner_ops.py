@@ -91,6 +91,16 @@ def _wants_grad(*tensors):
 # ---- the memory of a policy ------------------------------------------------------------------------------------------------------------------
 
 
+def _overlap(x, y):
+    """whether the memory that two tensors span has a part in common"""
+    spans = []
+    for z in (x, y):
+        if z.numel() == 0:
+            return False
+        spans.append((z.data_ptr(), z.data_ptr() + z.element_size() * (1 + sum((n - 1) * s for n, s in zip(z.shape, z.stride())))))
+    return spans[0][0] < spans[1][1] and spans[1][0] < spans[0][1]
+
+
 def gated_recurrence(gate, update, first=None, state=None, state_out=None):
     """h[t] = gate[t] * h[t-1] + update[t] along the steps of a window, each env and channel a chain of its own; where first[t] is set an episode
     begins and h[t] = update[t].  Returns (h, state): h [T, N, D] in the inputs' type, and the state behind the last step, float32 [N, D], to begin the
@@ -98,7 +108,10 @@ def gated_recurrence(gate, update, first=None, state=None, state_out=None):
 
     gate, update: [T, N, D] (or [T, N]) float32, float16 or bfloat16, any strides; first: [T, N] uint8 or bool, None: no episode begins; state:
     float32 [N, D] (or [N]), None: zeros.  state_out: a float32 buffer that takes the new state, `state` itself to move it on in place; only without
-    gradients.  Differentiable in gate, update and state, once."""
+    gradients.  Differentiable in gate, update and state, once.
+
+    Products of neighbouring gates are formed on the way (of 8 steps, and of up to the whole window where there are few chains): where such a product
+    passes float32's range -- gates larger than one over a long stretch -- h behind it is not finite, even if it began at zero."""
     _tensor(gate, "gate", _FLOATS)
     shape = gate.shape
     if len(shape) not in (2, 3):
@@ -113,6 +126,10 @@ def gated_recurrence(gate, update, first=None, state=None, state_out=None):
         _need(state_out.is_contiguous(), "state_out has to be contiguous")
         _need(not _wants_grad(gate, update, state, state_out), "state_out overwrites a state: call under torch.no_grad(), or take the returned state")
     _on_gpu(gate, update, first, state, state_out)
+    if state_out is not None:
+        for x, what in ((gate, "gate"), (update, "update"), (first, "first"), (state, "state")):
+            if x is not None and _overlap(x, state_out) and not (what == "state" and x.data_ptr() == state_out.data_ptr() and x.is_contiguous()):
+                raise ValueError(f"state_out lies inside of the memory of {what}")
     flat = len(shape) == 2
     if flat:
         gate, update = gate.unsqueeze(2), update.unsqueeze(2)

@@ -262,6 +262,39 @@ def test_gated_recurrence_in_place_single_steps_equal_the_window():
         check(state, want["last"], want["E_last"], "state")
 
 
+def test_gated_recurrence_refuses_a_state_out_inside_of_its_inputs():
+    x = torch.zeros((6, 2, 4), device="cuda")
+    state = torch.zeros((3, 4), device="cuda")
+    with torch.no_grad():
+        for out, kw in ((x[0], {}), (x[5], {}), (state[1:], {"state": state[:2]}), (state.view(-1)[:8].view(2, 4), {"state": state.view(-1)[:8].view(4, 2).T})):
+            with pytest.raises(ValueError):
+                ops().gated_recurrence(x, x, state_out=out, **kw)
+        rows = torch.zeros((2, 2, 4), device="cuda")
+        ops().gated_recurrence(x, x, state=rows[0], state_out=rows[1])  # neighbours in one buffer are no overlap
+
+
+def test_a_state_that_was_moved_on_in_place_is_not_used_by_an_older_graph():
+    g = gen(3)
+    gate, update, state = torch.rand((4, 2, 8), generator=g).cuda().requires_grad_(), rand((4, 2, 8), g).cuda(), rand((2, 8), g).cuda()
+    h, _ = ops().gated_recurrence(gate, update, None, state)
+    with torch.no_grad():
+        ops().gated_recurrence(gate, update, None, state, state_out=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+
+
+def test_gated_recurrence_reaches_beyond_32_bits():
+    """3 x 2^30 elements of output: gates and updates are expanded scalars, so that h[t] = 2 - 2^-t"""
+    T, D = 3 << 20, 1024
+    one = torch.ones((), dtype=torch.bfloat16, device="cuda")
+    with torch.no_grad():
+        h, last = ops().gated_recurrence((one * 0.5).expand(T, 1, D), one.expand(T, 1, D))
+    assert h.numel() * 2 > 1 << 32 and (last == 2).all()
+    for t in (0, 1, 2, 100, T // 2, T - 1):
+        assert (h[t] == 2 - 2.0 ** -min(t, 100)).all(), t
+    assert (h[1 << 20:, 0, ::257] == 2).all()
+
+
 # ---- advantages -------------------------------------------------------------------------------------------------------------------------------
 
 
@@ -433,6 +466,75 @@ def test_action_logprobs_where_little_is_left():
         assert d[1:3].isfinite().all()
 
 
+@pytest.mark.parametrize("A", [5, 40, 200, 9000])
+def test_rows_with_nan_and_infinities(A):
+    """NaN wherever a NaN or +inf is among the logits, as log_softmax has it; the rows beside them are as without"""
+    inf, nan = float("inf"), float("nan")
+    g, x, actions = row_inputs(6, A, "f32", A)
+    clean = x.clone()
+    x[1] = nan
+    x[2, A - 1] = nan
+    x[3, 0] = inf
+    x[4] = -inf
+    x[4, 1] = nan
+    t = x.cuda().requires_grad_()
+    logp, entropy = ops().action_logprobs(t, actions.cuda())
+    out = ops().policy_loss(t, actions.cuda(), logp.detach(), torch.ones(6, device="cuda"), entropy_coef=0.1)
+    (d,) = torch.autograd.grad([logp.sum() + entropy.sum()], t, retain_graph=True)
+    (e,) = torch.autograd.grad(out.loss, t)
+    for r in (1, 2, 3, 4):
+        assert logp[r].isnan() and entropy[r].isnan() and d[r].isnan().all() and e[r].isnan().all(), r
+    assert out.loss.isnan()
+    w = Rows64(clean)
+    for r in (0, 5):
+        check(logp[r], pick(w.logp, actions)[r], pick(w.T_logp, actions)[r], "log-probability")
+        assert d[r].isfinite().all() and e[r].isfinite().all()
+
+
+def test_policy_loss_against_a_reference_that_excludes_an_action():
+    """KL is infinite where the reference has no probability and the policy has; not where the policy has none either"""
+    inf = float("inf")
+    for A in (6, 500):
+        g, x, actions, old, adv = policy_inputs(4, A, "f32", 5)
+        ref = x + rand((4, A), g, scale=0.3)
+        x[1, 3] = ref[1, 3] = -inf
+        actions[1] = 0
+        old[1] = float(Rows64(x).logp[1, 0])
+        want = policy_64(x, actions, old, adv, 0.2, 0.2, 0.2, 0.0, None, ref)
+        out = ops().policy_loss(x.cuda(), actions.cuda(), old.cuda(), adv.cuda(), kl_coef=0.2, ref_logits=ref.cuda())
+        check(out.loss, want[0], want[1], "loss")
+        check(out.stats, want[2], want[3], "stats")
+        ref[2, 1] = -inf
+        out = ops().policy_loss(x.cuda(), actions.cuda(), old.cuda(), adv.cuda(), kl_coef=0.2, ref_logits=ref.cuda())
+        assert out.stats[1].item() == inf and out.loss.item() == inf
+        out = ops().policy_loss(x.cuda(), actions.cuda(), old.cuda(), adv.cuda(), kl_coef=0.0, ref_logits=ref.cuda())
+        assert out.stats[1].item() == inf and out.loss.isfinite()
+
+
+def test_rows_reach_beyond_32_bits():
+    """70 000 rows of 32 768 columns: the last rows against the same rows alone"""
+    B, A = 70000, 32768
+    x = torch.zeros((B, A), dtype=torch.bfloat16, device="cuda")
+    g, tail, actions = row_inputs(5, A, "bf16", 1)
+    x[-5:] = tail.cuda()
+    a = torch.zeros(B, dtype=torch.int32, device="cuda")
+    a[-5:] = actions.cuda()
+    alone = tail.cuda().requires_grad_()
+    logp, entropy = ops().action_logprobs(x, a)
+    w = Rows64(tail)
+    check(logp[-5:], pick(w.logp, actions), pick(w.T_logp, actions), "log-probabilities")
+    check(logp[:-5], torch.full((B - 5,), -np.log(A), dtype=torch.float64), torch.tensor(64 * U + 8 * U * np.log(A) + A / 64 * U), "uniform rows")
+    x.requires_grad_()
+    ones, valid = torch.ones(B, device="cuda"), torch.zeros(B, dtype=torch.uint8, device="cuda")
+    valid[-5:] = 1
+    (d,) = torch.autograd.grad(ops().policy_loss(x, a, logp, ones, valid=valid).loss, x)
+    (e,) = torch.autograd.grad(ops().policy_loss(alone, actions.cuda(), logp[-5:], ones[-5:]).loss, alone)
+    # another number of lanes for a row: sums in another order, bounded as ever; then half a step of bfloat16 each
+    tol = 2 * (w.rel_p * w.p / 5 + 16 * U * (1 + w.p) / 5) + rounding(e.double().cpu(), torch.bfloat16) * 2
+    check(d[-5:], e.double().cpu(), tol, "gradient of the last rows")
+    assert not d[:-5].any()
+
+
 @pytest.mark.parametrize("shape", [(0, 5), (3, 0, 5)])
 def test_rows_of_nothing(shape):
     x = torch.zeros(shape, device="cuda", requires_grad=True)
@@ -450,7 +552,7 @@ def policy_64(x, actions, old, adv, low, high, kl_coef, entropy_coef, valid=None
     """loss, stats, gradient and their tolerances, from the definition"""
     w = Rows64(x)
     A, B = x.shape[1], x.shape[0]
-    use = torch.ones(B, dtype=torch.bool) if valid is None else valid.bool()
+    use = torch.ones(B, dtype=torch.bool, device=x.device) if valid is None else valid.bool()
     n = max(1, int(use.sum()))
     use = use & ~w.empty
     logp, T = pick(w.logp, actions), pick(w.T_logp, actions)
@@ -492,7 +594,7 @@ def policy_64(x, actions, old, adv, low, high, kl_coef, entropy_coef, valid=None
 
     clipped = ((ratio < 1 - low) | (ratio > 1 + high)).double()
     stats = torch.stack([mean(policy), mean(kl), mean(w.H), mean(clipped)])
-    T_stats = torch.stack([mean(T_policy), mean(T_kl), mean(w.T_H), torch.zeros((), dtype=torch.float64)]) + 2 * U * stats.abs() + TINY[torch.float32]
+    T_stats = torch.stack([mean(T_policy), mean(T_kl), mean(w.T_H), torch.zeros((), dtype=torch.float64, device=x.device)]) + 2 * U * stats.abs() + TINY[torch.float32]
     loss = stats[0] + kl_coef * stats[1] - entropy_coef * stats[2]
     T_loss = T_stats[0] + kl_coef * T_stats[1] + abs(entropy_coef) * T_stats[2] + 4 * U * (stats[0].abs() + kl_coef * stats[1].abs() + abs(entropy_coef) * stats[2].abs())
     return loss, T_loss, stats, T_stats, d, T_d
@@ -542,6 +644,32 @@ def test_policy_loss(B, A, dtype, layout, ref):
     with torch.no_grad():
         again = ops().policy_loss(t, flat(actions), flat(old), flat(adv), **kw)
     assert torch.equal(again.loss, out.loss.detach()) and torch.equal(again.stats, out.stats)
+
+
+@pytest.mark.parametrize("B,A,dtype,ref", [(513, 20011, "f32", True), (515, 40003, "bf16", True), (600, 5000, "f16", True), (520, 33333, "bf16", False), (1030, 2500, "f32", False)])
+def test_policy_loss_of_many_long_rows(B, A, dtype, ref):
+    """rows of several batches, enough of them to fill the card; the 64-bit loss on the GPU for its time"""
+    g = torch.Generator(device="cuda").manual_seed(A)
+    x = (3 * torch.randn((B, A), generator=g, device="cuda")).to(DTYPES[dtype])
+    r = (x.float() + 0.5 * torch.randn((B, A), generator=g, device="cuda")).to(x.dtype) if ref else None
+    actions = torch.randint(0, A, (B,), generator=g, device="cuda")
+    actions[:4] = torch.tensor([0, 1, A - 2, A - 1])
+    step = 0.15 * torch.randn(B, generator=g, device="cuda").double()
+    for border in (np.log(0.8), np.log(1.2)):
+        step = torch.where((step - border).abs() < 1e-3, step + 4e-3, step)
+    old, adv = (pick(Rows64(x).logp, actions) - step).float(), torch.randn(B, generator=g, device="cuda")
+    valid = torch.rand(B, generator=g, device="cuda") < 0.9
+    want = [v.cpu() for v in policy_64(x, actions, old, adv, 0.2, 0.2, 0.3 if ref else 0.0, 0.02, valid, r)]
+    wide = torch.full((B, A + 5), float("nan"), dtype=x.dtype, device="cuda")
+    wide[:, 2:2 + A] = x
+    t = wide[:, 2:2 + A].requires_grad_()
+    out = ops().policy_loss(t, actions, old, adv, kl_coef=0.3 if ref else 0.0, ref_logits=r, entropy_coef=0.02, valid=valid)
+    check(out.loss, want[0], want[1], "loss")
+    check(out.stats, want[2], want[3], "stats")
+    (d,) = torch.autograd.grad(out.loss, t, retain_graph=True)
+    check(d, want[4], want[5] + rounding(want[4], x.dtype), "gradient")
+    (d,) = torch.autograd.grad(out.loss * 4, t)
+    check(d, want[4] * 4, want[5] * 4 + rounding(want[4] * 4, x.dtype), "gradient of 4 times the loss")
 
 
 @pytest.mark.parametrize("A", [6, 300])
@@ -721,6 +849,66 @@ def test_single_steps_in_a_captured_graph_move_the_state_on():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(graph_state, eager_state) and torch.equal(logp, want[0]) and torch.equal(entropy, want[1]), k
+
+
+def test_forward_and_backward_in_graphs_of_their_own():
+    """as torch.cuda.make_graphed_callables captures them: the backward graph cannot know what the forward one wrote, and serves every scale"""
+    g, x, actions, old, adv = policy_inputs(300, 15, "f32", 21)
+    args = actions.cuda(), old.cuda(), adv.cuda()
+
+    class Loss(torch.nn.Module):
+        def forward(self, logits):
+            return ops().policy_loss(logits, *args, entropy_coef=0.05).loss
+
+    graphed = torch.cuda.make_graphed_callables(Loss(), (torch.zeros((300, 15), device="cuda", requires_grad=True),))
+    for k, scale in enumerate((3.0, 1.0, 0.5, 1.0)):
+        values = x + 0.01 * k
+        t = values.cuda().requires_grad_()
+        (d,) = torch.autograd.grad(graphed(t) * scale, t)
+        torch.cuda.synchronize()
+        u = values.cuda().requires_grad_()
+        (e,) = torch.autograd.grad(Loss()(u) * scale, u)
+        assert torch.equal(d, e), scale
+
+
+def test_gradients_of_gradients_are_refused():
+    x, w = window_inputs(8, 3, 4, 15, 7)
+    logits = torch.zeros((8, 3, 15), device="cuda", requires_grad=True)
+    h, _ = ops().gated_recurrence(x["gate"], x["update"], x["first"][:-1], x["state"])
+    logp, _ = ops().action_logprobs(logits, x["actions"])
+    for y, leaf in ((h.sum(), x["gate"]), (logp.sum(), logits), (ops().policy_loss(logits, x["actions"], x["old"], x["rew"]).loss, logits)):
+        (d,) = torch.autograd.grad(y, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once"):
+            d.sum().backward()
+
+
+def test_two_host_threads_and_streams():
+    """each with a stream of its own, the same work at the same time: the results are those of one after the other"""
+    import threading
+
+    sets = [window_inputs(60, 4, 16, 15, 300 + k) for k in range(3)]
+    alone = [window_step(*s) for s in sets]
+    torch.cuda.synchronize()
+    got, errors = [None] * 3, []
+
+    def work(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    got[k] = window_step(*sets[k])
+            stream.synchronize()
+        except Exception as e:  # handed to the test's own thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for a, b in zip(got, alone):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 def test_repeated_calls_give_the_same_bits():
