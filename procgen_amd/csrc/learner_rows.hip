@@ -13,10 +13,9 @@
 // Partial sums of a row are taken against the largest value their lane or wave has seen and rescaled when they meet (Stats::join), so a row is read once.
 //
 // Bound by memory: a column costs 12 operations for 4 to 8 bytes, 23 for 6 to 12 with a reference.  By the number of columns:
-//   up to 64      a wave takes 64 rows through LDS, a lane per row: no reduction over lanes, coalesced although a row is no multiple of anything
-//   more          a group of 16 to 1024 lanes per row, 16 or 32 bytes a lane at a time; a row of one such batch stays in registers between the sums
-//                 and the gradient
-//   very long     the same in several batches; the gradient goes through them backwards: the last is still in registers, those before it in LDS, and
+//   up to 32      a wave takes 64 rows through LDS, a lane per row: no reduction over lanes, coalesced although a row is no multiple of anything
+//   up to 4096    a group of 4 to 64 lanes per row, the whole row in their registers between the sums and the gradient (2048 in float32)
+//   more          a block per row, in batches; the gradient goes through them backwards: the last is still in registers, those before it in LDS, and
 //                 only what is left is read from memory again
 #include "learner.h"
 
@@ -35,7 +34,9 @@ __device__ inline long long action_of(const procgen_amd_rows &p, long long r) {
     return p.actions_are_64_bit ? ((const long long *)p.actions)[r] : (long long)((const int *)p.actions)[r];
 }
 __device__ inline long long row_offset(const procgen_amd_rows &p, long long r, long long outer, long long inner) {
-    return p.inner == 1 ? r * outer : (r / p.inner) * outer + (r % p.inner) * inner;
+    if (p.inner == 1) return r * outer;
+    const uint32_t per = (uint32_t)p.inner, group = (uint32_t)r / per;  // rows fit 32 bits
+    return group * outer + ((uint32_t)r - group * per) * inner;
 }
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
@@ -326,7 +327,7 @@ struct Chunk {
     __device__ void forget() { asm volatile("" : "+v"(w)); }
 };
 
-// ---- up to 64 columns: a lane per row -------------------------------------------------------------------------------------------------------------
+// ---- up to 32 columns: a lane per row -------------------------------------------------------------------------------------------------------------
 
 // 64 rows on their way from memory to LDS (`rows` of them exist).  Contiguous rows go 16 bytes a lane and, where they are few registers, are fetched
 // while the 64 before them are worked on; others go element by element.
@@ -380,7 +381,7 @@ __device__ inline void lds_settled() {  // a wave's own LDS is written and read 
 // blocks of four waves that a compute unit holds: by registers (three, or four with a reference, for each of MOST columns) and by LDS
 template <class E, int MOST, bool REF>
 constexpr int short_residents() {
-    return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? 3 : sizeof(typename E::T) == 4 ? 4 : 5) : MOST <= 32 ? (REF ? 2 : 3) : REF ? 1 : 2;
+    return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? 3 : sizeof(typename E::T) == 4 ? 4 : 5) : REF ? 2 : 3;
 }
 
 template <class E, int MOST, bool REF, class Op>
@@ -490,36 +491,164 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
 
 // ---- more columns: a group of G lanes per row -----------------------------------------------------------------------------------------------------
 
-template <class E, int G, int CH, bool REF, class Op>
-__global__ __launch_bounds__(G > BLOCK ? G : BLOCK, 4) void long_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
+// Where a row's columns are among the lanes of a group.  Chunk c is the 16 aligned bytes of columns [c N - ahead, + N), whatever the row's own alignment
+// (a row at an odd address costs an eighth more time otherwise); lane g has the chunks g, g + G, ...  The first and the last chunk of a row are moved so
+// that they end in it: what they share with their neighbour counts as -inf and is not written.  Chunks behind the row are all -inf.
+template <class E>
+struct Place {
     typedef typename E::T T;
-    constexpr int N = Chunk<E>::N, THREADS = G > BLOCK ? G : BLOCK, PER_BLOCK = THREADS / G, SPAN = G * CH * N;  // columns of a batch
-    const int g = threadIdx.x % G, lane = threadIdx.x % WAVE;
-    __shared__ float wave_stats[2][G > WAVE ? G / WAVE : 1][6];
+    static constexpr int N = Chunk<E>::N;
+    int columns, ahead;
+    __device__ Place(const T *row, int columns_) : columns(columns_), ahead((int)((uintptr_t)row / sizeof(T) % N)) {}
+    __device__ int wanted(int chunk) const { return chunk * N - ahead; }
+    __device__ int column(int chunk) const { return max(0, min(wanted(chunk), columns - N)); }
+    __device__ void drop(Chunk<E> &x, int chunk) const {
+        const int moved = wanted(chunk) - column(chunk);
+        if (moved) x.drop(moved);
+    }
+    __device__ void put(T *out, int chunk, const Chunk<E> &x) const {
+        const int j = wanted(chunk), from = column(chunk);
+        if (j >= columns) return;
+        if (from == j) {
+            x.store(out + j);
+        } else {
+            for (int k = 0; k < N; k++)
+                if (from + k >= j && from + k < j + N) out[from + k] = x.piece(k);
+        }
+    }
+    __device__ int chunk_of(int column) const { return (column + ahead) / N; }
+};
+
+// Rows that fit the registers of a group inside of a wave: the next rows are on their way while these are worked on.
+template <class E, int G, int CH, bool REF, class Op>
+__global__ __launch_bounds__(BLOCK) void group_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
+    typedef typename E::T T;
+    constexpr int N = Chunk<E>::N, PER = N / 4, PER_BLOCK = BLOCK / G;
+    const int g = threadIdx.x % G, columns = (int)p.columns;
+    if (op.done()) return;
+    op.begin(p);
+    Sums sums;
+    Bits next[CH], next2[REF ? CH : 1];
+    typename Op::In next_in;
+    int next_a = -1;
+    auto row_of = [&](long long r) { return (const T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride); };
+    auto row2_of = [&](long long r) { return (const T *)ref + row_offset(p, r, ref_outer, ref_inner); };
+    auto fetch = [&](long long r) {
+        r = min(r, p.rows - 1);
+        const T *const row = row_of(r), *const row2 = REF ? row2_of(r) : nullptr;
+        const Place<E> at(row, columns);
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const int j = at.column(i * G + g);
+            __builtin_memcpy(&next[i], row + j, 16);
+            if (REF) __builtin_memcpy(&next2[i], row2 + j, 16);
+        }
+        next_in = op.fetch(r);
+        const long long a = action_of(p, r);
+        next_a = a >= 0 && a < columns ? (int)a : -1;
+    };
+    const long long step = (long long)gridDim.x * PER_BLOCK;
+    long long r = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / G;
+    fetch(r);
+    for (long long first = (long long)blockIdx.x * PER_BLOCK; first < p.rows; first += step, r += step) {
+        const bool mine = r < p.rows;
+        const long long here = mine ? r : p.rows - 1;
+        const T *const row = row_of(here), *const row2 = REF ? row2_of(here) : nullptr;
+        const Place<E> at(row, columns);
+        Chunk<E> l[CH], l2[REF ? CH : 1];
+        const typename Op::In in = next_in;
+        const int a = next_a;
+        const float taken = (float)row[max(a, 0)], taken2 = REF ? (float)row2[max(a, 0)] : 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            l[i].w = next[i];
+            at.drop(l[i], i * G + g);
+            if (REF) {
+                l2[i].w = next2[i];
+                at.drop(l2[i], i * G + g);
+            }
+        }
+        if (first + step < p.rows) fetch(r + step);
+        Stats<REF> x;
+        float to = -INFINITY, to2 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < CH; i++)
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                to = fmaxf(to, l[i][k]);
+                if (REF) to2 = fmaxf(to2, l2[i][k]);
+            }
+        for (int d = G / 2; d > 0; d >>= 1) {
+            to = fmaxf(to, __shfl_xor(to, d, WAVE));
+            if (REF) to2 = fmaxf(to2, __shfl_xor(to2, d, WAVE));
+        }
+        x.m = to, x.m2 = to2;
+        const Base b(to), b2(to2);
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            l[i].forget();
+            if (REF) l2[i].forget();
+#pragma unroll
+            for (int k = 0; k < N; k++) x.add(b, b2, l[i][k], REF ? l2[i][k] : 0.f);
+        }
+        for (int d = G / 2; d > 0; d >>= 1) {
+            x.s += __shfl_xor(x.s, d, WAVE);
+            x.w += __shfl_xor(x.w, d, WAVE);
+            if (REF) {
+                x.s2 += __shfl_xor(x.s2, d, WAVE);
+                x.u += __shfl_xor(x.u, d, WAVE);
+            }
+        }
+        Coef c;
+        const bool some = mine && op.wanted(in) && op.template finish<REF>(here, in, x, a >= 0, taken, g == 0, c, sums);
+        if (!Op::GRADIENT || !p.d_logits || !mine) continue;
+        T *const out = (T *)p.d_logits + r * p.columns;
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            l[i].forget();
+            if (REF) l2[i].forget();
+            Chunk<E> d;
+            d.w = Bits{0, 0, 0, 0};
+            if (some) {
+#pragma unroll
+                for (int k = 0; k < N; k += PER)
+                    d.set(k / PER, c.gradient<REF>(l[i][k], REF ? l2[i][k] : 0.f), PER > 1 ? c.gradient<REF>(l[i][k + PER - 1], REF ? l2[i][k + PER - 1] : 0.f) : 0.f);
+            }
+            at.put(out, i * G + g, d);
+        }
+        if (some && a >= 0 && at.chunk_of(a) % G == g) out[a] = (T)(c.gradient<REF>(taken, taken2) + c.pick);  // by the lane that wrote the column just now
+    }
+    if (partial) put_sums(sums, op, partial);
+}
+
+// A block per row, in batches of G lanes times CH chunks; the next batch is on its way while one is summed up.
+template <class E, int G, int CH, bool REF, class Op>
+__global__ __launch_bounds__(G, 4) void long_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
+    typedef typename E::T T;
+    constexpr int N = Chunk<E>::N, SPAN = G * CH * N;  // columns of a batch
+    const int g = threadIdx.x, lane = threadIdx.x % WAVE;
+    __shared__ float wave_stats[2][G / WAVE][6];
     // a lane's own columns of the last batches but one stay in LDS, 128 bytes of it a lane, and are not read from memory again for the gradient
-    constexpr int KEPT = Op::GRADIENT && G >= 4 * WAVE ? 8 / (CH * (REF ? 2 : 1)) : 0;
+    constexpr int KEPT = Op::GRADIENT ? 8 / (CH * (REF ? 2 : 1)) : 0;
     __shared__ Bits kept[KEPT ? KEPT : 1][REF ? 2 : 1][KEPT ? CH : 1][KEPT ? G : 1];
     if (op.done()) return;
     op.begin(p);
     Sums sums;
     const int columns = (int)p.columns;
     int odd = 0;
-    for (long long r = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / G; r < p.rows; r += (long long)gridDim.x * PER_BLOCK) {
+    for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const T *const row = (const T *)p.logits + row_offset(p, r, p.outer_stride, p.inner_stride);
         const T *const row2 = REF ? (const T *)ref + row_offset(p, r, ref_outer, ref_inner) : nullptr;
         T *const out = Op::GRADIENT && p.d_logits ? (T *)p.d_logits + r * p.columns : nullptr;
         bool some = false;
-        // Chunk i of batch b are the columns [at(b, i), + N): 16 aligned bytes, whatever the row's own alignment (a row at an odd address costs an eighth
-        // more time otherwise).  The first and the last one of a row are moved so that they end in it: what they share with their neighbour counts as
-        // -inf here and is not written.  Chunks behind the row are all -inf.
-        const int ahead = (int)((uintptr_t)row / sizeof(T) % N), batches = (columns + ahead + SPAN - 1) / SPAN;
-        auto at = [&](int b, int i) { return b * SPAN + (i * G + g) * N - ahead; };
-        auto column = [&](int j) { return max(0, min(j, columns - N)); };
+        const Place<E> at(row, columns);
+        const int batches = (columns + at.ahead + SPAN - 1) / SPAN;
+        auto chunk = [&](int b, int i) { return (b * CH + i) * G + g; };
         Chunk<E> l[CH], l2[REF ? CH : 1], next[CH], next2[REF ? CH : 1];  // the batch that is worked on, and the one on its way
         auto load = [&](int b) {
 #pragma unroll
             for (int i = 0; i < CH; i++) {
-                const int j = column(at(b, i));
+                const int j = at.column(chunk(b, i));
                 next[i].load(row + j);
                 if (REF) next2[i].load(row2 + j);
             }
@@ -529,20 +658,8 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK, 4) void long_rows(procgen_am
             for (int i = 0; i < CH; i++) {
                 l[i] = next[i];
                 if (REF) l2[i] = next2[i];
-                const int moved = at(b, i) - column(at(b, i));
-                if (moved) {
-                    l[i].drop(moved);
-                    if (REF) l2[i].drop(moved);
-                }
-            }
-        };
-        auto put = [&](T *to, int j, const Chunk<E> &d) {  // what is this lane's own of the chunk that is to begin at column j
-            const int from = column(j);
-            if (from == j) {
-                d.store(to + j);
-            } else {
-                for (int k = 0; k < N; k++)
-                    if (from + k >= j && from + k < j + N) to[from + k] = d.piece(k);
+                at.drop(l[i], chunk(b, i));
+                if (REF) at.drop(l2[i], chunk(b, i));
             }
         };
         auto forget = [&] {
@@ -591,18 +708,16 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK, 4) void long_rows(procgen_am
                 for (int i = 0; i < CH; i++)
                     for (int k = 0; k < N; k++) x.add(base, base2, l[i][k], REF ? l2[i][k] : 0.f);
             }
-            x.template join<(G < WAVE ? G : WAVE)>();
-            if (G > WAVE) {
-                if (lane == 0) x.put(wave_stats[odd][threadIdx.x / WAVE]);
-                __syncthreads();
-                x = Stats<REF>();
-                if (lane < G / WAVE) x.get(wave_stats[odd][lane]);
-                x.template join<(G > WAVE ? G / WAVE : 1)>();
-                // lanes beyond the first G / WAVE hold no wave's sums: they take the first one's
-                x.m = __shfl(x.m, 0, WAVE), x.s = __shfl(x.s, 0, WAVE), x.w = __shfl(x.w, 0, WAVE);
-                if (REF) x.m2 = __shfl(x.m2, 0, WAVE), x.s2 = __shfl(x.s2, 0, WAVE), x.u = __shfl(x.u, 0, WAVE);
-                odd ^= 1;
-            }
+            x.template join<WAVE>();
+            if (lane == 0) x.put(wave_stats[odd][threadIdx.x / WAVE]);
+            __syncthreads();
+            x = Stats<REF>();
+            if (lane < G / WAVE) x.get(wave_stats[odd][lane]);
+            x.template join<G / WAVE>();
+            // lanes beyond the first G / WAVE hold no wave's sums: they take the first one's
+            x.m = __shfl(x.m, 0, WAVE), x.s = __shfl(x.s, 0, WAVE), x.w = __shfl(x.w, 0, WAVE);
+            if (REF) x.m2 = __shfl(x.m2, 0, WAVE), x.s2 = __shfl(x.s2, 0, WAVE), x.u = __shfl(x.u, 0, WAVE);
+            odd ^= 1;
             if (Op::GRADIENT && out && batches > 1 + KEPT) load(batches - 2 - KEPT);  // the first batch that has to be read again
             some = op.template finish<REF>(r, in, x, known, taken, g == 0, c, sums);
             forget();
@@ -612,7 +727,7 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK, 4) void long_rows(procgen_am
             for (int i = 0; i < batches * CH; i++) {
                 Chunk<E> zero;
                 zero.w = Bits{0, 0, 0, 0};
-                if (at(0, i) < columns) put(out, at(0, i), zero);
+                at.put(out, chunk(0, i), zero);
             }
             continue;
         }
@@ -636,10 +751,10 @@ __global__ __launch_bounds__(G > BLOCK ? G : BLOCK, 4) void long_rows(procgen_am
 #pragma unroll
                 for (int k = 0; k < N; k += PER)
                     d.set(k / PER, c.gradient<REF>(l[i][k], REF ? l2[i][k] : 0.f), PER > 1 ? c.gradient<REF>(l[i][k + PER - 1], REF ? l2[i][k + PER - 1] : 0.f) : 0.f);
-                if (at(b, i) < columns) put(out, at(b, i), d);
+                at.put(out, chunk(b, i), d);
             }
         }
-        if (a >= 0 && a < columns && (int)((a + ahead) / N) % G == g)  // by the lane that wrote the column just now
+        if (a >= 0 && a < columns && at.chunk_of((int)a) % G == g)  // by the lane that wrote the column just now
             out[a] = (T)(c.gradient<REF>((float)row[a], REF ? (float)row2[a] : 0.f) + c.pick);
     }
     if (partial) put_sums(sums, op, partial);
@@ -740,16 +855,36 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
     // two rounds of one block, which ends with the means, cost less than a launch for them
     auto short_grid = [&](int most) { return partial && p.rows <= 2 * BLOCK ? blocks = 1 : grid(BLOCK, most); };
     constexpr int N = Chunk<E>::N;
-    if (p.columns <= 64) {
-        const size_t lds = ((WAVE * p.columns * sizeof(typename E::T) + 15) & ~15ull) * (BLOCK / WAVE) * (REF ? 2 : 1);
+    constexpr long long SIZE = sizeof(typename E::T);
+    // as many columns as a row can span in aligned chunks
+    const bool aligned = ((uintptr_t)p.logits | (uintptr_t)(p.outer_stride * SIZE) | (uintptr_t)(p.inner_stride * SIZE)) % 16 == 0;
+    const long long padded = p.columns + (aligned ? 0 : N - 1);
+    // A lane per row, where its registers leave enough waves.  Over 64 M columns in all, against the
+    // groups: 16-bit 17 columns 102 : 190 us, 24 80 : 122, 32 88 : 96, 33 127 : 152, 48 112 : 87; float32 16 149 : 171, 24 137 : 143, 32
+    // 276 : 127; float32 with a reference 16 227 : 203, 24 252 : 168.
+    const bool lane_per_row = SIZE == 2 ? p.columns <= 32 : p.columns <= (REF ? 15 : 24);
+    if (lane_per_row) {
+        const size_t lds = ((WAVE * p.columns * SIZE + 15) & ~15ull) * (BLOCK / WAVE) * (REF ? 2 : 1);
         if (p.columns <= 8) short_rows<E, 8, REF, Op><<<short_grid(CUS * short_residents<E, 8, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<short_grid(CUS * short_residents<E, 16, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if (p.columns <= 32) short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else short_rows<E, 64, REF, Op><<<short_grid(CUS * short_residents<E, 64, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (p.columns <= 16 * 2 * N) {
-        long_rows<E, 16, 2, REF, Op><<<grid(BLOCK / 16, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (p.columns <= 64 * 2 * N) {
-        long_rows<E, 64, 2, REF, Op><<<grid(BLOCK / 64, MAX_BLOCKS), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if constexpr (SIZE == 2 || !REF)
+            short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (padded <= 4 * 1 * N) {
+        group_rows<E, 4, 1, REF, Op><<<grid(BLOCK / 4, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (padded <= 4 * 2 * N) {
+        group_rows<E, 4, 2, REF, Op><<<grid(BLOCK / 4, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (padded <= 4 * 4 * N) {
+        group_rows<E, 4, 4, REF, Op><<<grid(BLOCK / 4, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (padded <= 8 * 4 * N) {
+        group_rows<E, 8, 4, REF, Op><<<grid(BLOCK / 8, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (padded <= 16 * 4 * N) {
+        group_rows<E, 16, 4, REF, Op><<<grid(BLOCK / 16, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (padded <= 32 * 4 * N) {
+        group_rows<E, 32, 4, REF, Op><<<grid(BLOCK / 32, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (padded <= 64 * 4 * N) {
+        group_rows<E, 64, 4, REF, Op><<<grid(BLOCK / 64, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (padded <= 64 * 8 * N) {
+        group_rows<E, 64, 8, REF, Op><<<grid(BLOCK / 64, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.columns <= 256 * 2 * N || (p.rows >= 2 * CUS && !(REF && p.d_logits))) {
         long_rows<E, 256, 2, REF, Op><<<grid(1, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.rows >= 2 * CUS) {  // 2048 x 50021 bf16 with a reference: 154 us, against 173 with 256 lanes and two chunks, 179 with 1024
@@ -789,7 +924,7 @@ LIBENV_API int procgen_amd_action_logprobs_backward(const struct procgen_amd_row
     if (on.err != hipSuccess) return (int)on.err;
     return by_dtype(p->dtype, [&](auto e) {
         typedef decltype(e) E;
-        if (p->columns <= 64) {
+        if (p->columns <= 256 * Chunk<E>::N) {
             const int got = launch_rows<E, false>(*p, LogprobsBackward{d_logp, d_entropy}, nullptr, 0, 0, nullptr, (hipStream_t)stream);
             return got < 0 ? -1 - got : 0;
         }
