@@ -3,9 +3,10 @@
 //
 // A step is the affine map x -> a x + b, or x -> b where an episode begins (`cut`: a select, so that nothing of the other episode, NaN or infinite,
 // passes).  Maps compose to maps of the same kind, so a chain is cut into pieces that are summed up at the same time and joined afterwards:
-//   wave     K = 8 consecutive steps in registers, their composition (A, B, cut) by 8 FMAs
-//   block    W <= 8 waves take consecutive pieces of a tile of 64 steps; the pieces' maps meet in LDS, every wave runs its value at the tile's start
-//            through the pieces before its own, and does its steps again from there: one read and one write of the data, one barrier a tile
+//   wave     8 consecutive steps in registers (4 backwards), their composition (A, B, cut) by an FMA each
+//   block    four waves (eight where a window is in segments) take consecutive pieces of a tile; the pieces' maps meet in LDS, every wave runs its value
+//            at the tile's start through the pieces before its own, and does its steps again from there: one read and one write of the data, one barrier
+//            a tile
 //   segment  where there are too few chains to fill the card, the window is cut into segments for blocks of their own: a first kernel composes each
 //            segment's map, the second begins each segment with the maps of those before it (the data is read twice)
 // Lanes are chains (VEC neighbouring channels each), so that every load of a step is one coalesced row piece.
@@ -17,10 +18,10 @@ namespace pgamd {
 namespace learner {
 namespace {
 
-constexpr int W_MAX = 4;          // waves of a block
+constexpr int W1 = 4, WS = 8;     // waves of a block: where there are chains enough, and where a window is cut into segments
 constexpr int KF = 8, KB = 4;     // steps of a wave in a tile: forwards (and advantages), backwards
-constexpr int TILE = KF * W_MAX;  // a segment is a whole number of these
-constexpr int CHECK = KB * W_MAX; // steps from one checkpoint to the next: a tile of the backward pass
+constexpr int UNIT = KF * WS;     // a segment is a whole number of these: of the tiles of either direction
+constexpr int CHECK = KB * W1;    // steps from one checkpoint to the next: a tile of the backward pass, or half of one
 
 // VEC neighbouring channels of a step, as memory holds them.  Loads are unconditional (addresses are clamped into the arrays and values selected
 // afterwards): a load behind a branch of its own would be waited for before the next is issued.
@@ -49,13 +50,13 @@ struct Map {
 };
 
 // the pieces' maps of a tile, by wave and lane
-template <int VEC>
+template <int VEC, int WAVES>
 struct Pieces {
     struct alignas(4 * VEC) Vec {
         float x[VEC];
     };
-    Vec A[W_MAX][WAVE], B[W_MAX][WAVE];
-    int cut[W_MAX][WAVE];
+    Vec A[WAVES][WAVE], B[WAVES][WAVE];
+    int cut[WAVES][WAVE];
     __device__ void put(int w, int lane, const Map<VEC> &m) {
         Vec a, b;
         for (int v = 0; v < VEC; v++) a.x[v] = m.A[v], b.x[v] = m.B[v];
@@ -114,8 +115,8 @@ __device__ inline Map<VEC> get_segment(const Segments &g, int s, long long chain
 }
 
 // x[] run through the segments [from, to) in order (to < from: downwards): the waves take a part each and join in LDS
-template <int VEC>
-__device__ inline void run_segments(float *x, const Segments &g, int from, int to, long long chains, const Chain<VEC> &ch, Pieces<VEC> &pieces, int w, int W, int lane) {
+template <int VEC, int WAVES>
+__device__ inline void run_segments(float *x, const Segments &g, int from, int to, long long chains, const Chain<VEC> &ch, Pieces<VEC, WAVES> &pieces, int w, int W, int lane) {
     const int n = abs(to - from), way = to < from ? -1 : 1, first = (int)((long long)n * w / W), last = (int)((long long)n * (w + 1) / W);
     Map<VEC> m;
     m.identity();
@@ -204,15 +205,15 @@ __device__ inline void convert(bool (&cut)[K], const uint8_t (&raw)[K], uint8_t 
 }
 
 // the map of every segment (blockIdx.y): forwards of gate and update, backwards of gate and d_h.  The waves take a part of the segment each.
-template <class E, int VEC, bool REVERSE>
-__global__ __launch_bounds__(W_MAX *WAVE) void recurrence_segments(procgen_amd_recurrence p, Segments g) {
+template <class E, int VEC, int WAVES, bool REVERSE>
+__global__ __launch_bounds__(WAVES *WAVE) void recurrence_segments(procgen_amd_recurrence p, Segments g) {
     constexpr int K = KF;
-    __shared__ Pieces<VEC> pieces;
+    __shared__ Pieces<VEC, WAVES> pieces;
     const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
     const Chain<VEC> ch(blockIdx.x * WAVE + lane, p.N, p.D);
     const long long chains = (long long)p.N * p.D;
-    const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE);
-    const int part = (g.tiles * TILE + W * K - 1) / (W * K) * K;  // steps of a wave
+    const int begin = s * g.tiles * UNIT, end = min((long long)p.T, (long long)begin + (long long)g.tiles * UNIT);
+    const int part = (g.tiles * UNIT + W * K - 1) / (W * K) * K;  // steps of a wave
     const int from = min((long long)end, (long long)begin + (long long)w * part), to = min((long long)end, (long long)from + part);
     const bool any = !REVERSE || p.d_h.data;
     const Column<E, VEC, K> gate(p.gate, ch), other(REVERSE ? (any ? p.d_h : p.gate) : p.update, ch);
@@ -246,14 +247,14 @@ __global__ __launch_bounds__(W_MAX *WAVE) void recurrence_segments(procgen_amd_r
     }
 }
 
-template <class E, int VEC>
-__global__ __launch_bounds__(W_MAX *WAVE) void recurrence_forward(procgen_amd_recurrence p, Segments g) {
-    constexpr int K = KF;
-    __shared__ Pieces<VEC> pieces[2];
+template <class E, int VEC, int WAVES>
+__global__ __launch_bounds__(WAVES *WAVE) void recurrence_forward(procgen_amd_recurrence p, Segments g) {
+    constexpr int K = KF, TILE = K * WAVES;
+    __shared__ Pieces<VEC, WAVES> pieces[2];
     const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
     const Chain<VEC> ch(blockIdx.x * WAVE + lane, p.N, p.D);
     const long long chains = (long long)p.N * p.D;
-    const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE), last = end - 1;
+    const int begin = s * g.tiles * UNIT, end = min((long long)p.T, (long long)begin + (long long)g.tiles * UNIT), last = end - 1;
     const Column<E, VEC, K> gate(p.gate, ch), update(p.update, ch), out(p.h, ch);
     const Flags first(p.first, p.first_t_stride, p.first_n_stride, ch.n, gate.base);
     Raw<E, VEC> ra[K], rb[K];
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(W_MAX *WAVE) void recurrence_forward(procgen_amd_re
     load(begin + w * K);
     float x[VEC];
     load_state<VEC>(x, p.state && g.count > 1 ? g.state : p.state, ch);
-    if (s) run_segments<VEC>(x, g, 0, s, chains, ch, pieces[0], w, W, lane);
+    if (s) run_segments(x, g, 0, s, chains, ch, pieces[0], w, W, lane);
     for (int t0 = begin, odd = 0; t0 < end; t0 += TILE, odd ^= 1) {
         const int t = t0 + w * K;
         float a[K][VEC], b[K][VEC];
@@ -298,14 +299,14 @@ __global__ __launch_bounds__(W_MAX *WAVE) void recurrence_forward(procgen_amd_re
 
 // Backwards over the tiles.  h is not read: its 32-bit value before every step comes from the checkpoint at the tile's start and the same joins as in
 // the forward pass (update is read in its place, so the bytes are the same and 16-bit rounding of h does not reach d_gate).
-template <class E, int VEC>
-__global__ __launch_bounds__(W_MAX *WAVE) void recurrence_backward(procgen_amd_recurrence p, Segments g) {
-    constexpr int K = KB;
-    __shared__ Pieces<VEC> fore[2], back[2];
+template <class E, int VEC, int WAVES>
+__global__ __launch_bounds__(WAVES *WAVE) void recurrence_backward(procgen_amd_recurrence p, Segments g) {
+    constexpr int K = KB, TILE = K * WAVES;
+    __shared__ Pieces<VEC, WAVES> fore[2], back[2];
     const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
     const Chain<VEC> ch(blockIdx.x * WAVE + lane, p.N, p.D);
     const long long chains = (long long)p.N * p.D;
-    const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE), last = end - 1;
+    const int begin = s * g.tiles * UNIT, end = min((long long)p.T, (long long)begin + (long long)g.tiles * UNIT), last = end - 1;
     const bool any = p.d_h.data;
     const Column<E, VEC, K> gate(p.gate, ch), update(p.update, ch), d_h(any ? p.d_h : p.gate, ch), d_gate(p.d_gate, ch), d_update(p.d_update, ch);
     const Flags first(p.first, p.first_t_stride, p.first_n_stride, ch.n, gate.base);
@@ -320,12 +321,12 @@ __global__ __launch_bounds__(W_MAX *WAVE) void recurrence_backward(procgen_amd_r
         first.load(rf, t, last);
         load_state<VEC>(start, p.checkpoints + (long long)(t0 / CHECK) * chains, ch);
     };
-    const int top = begin + (end - begin - 1) / CHECK * CHECK;
+    const int top = begin + (end - begin - 1) / TILE * TILE;
     load(top);
     float y[VEC];  // what reaches h from the steps behind the tile
     load_state<VEC>(y, p.d_state_out, ch);
-    if (s < g.count - 1) run_segments<VEC>(y, g, g.count, s + 1, chains, ch, fore[0], w, W, lane);
-    for (int t0 = top, odd = 0; t0 >= begin; t0 -= CHECK, odd ^= 1) {
+    if (s < g.count - 1) run_segments(y, g, g.count, s + 1, chains, ch, fore[0], w, W, lane);
+    for (int t0 = top, odd = 0; t0 >= begin; t0 -= TILE, odd ^= 1) {
         const int t = t0 + w * K;
         float a[K][VEC], b[K][VEC], d[K][VEC], x[VEC], before[VEC], behind[VEC];
         bool cut[K];
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(W_MAX *WAVE) void recurrence_backward(procgen_amd_r
         convert<E, VEC, K>(d, rd, t, any ? end : 0, 0.f);
         convert(cut, rf, first.mask, t, end);
         for (int v = 0; v < VEC; v++) x[v] = start[v];
-        if (t0 > begin) load(t0 - CHECK);
+        if (t0 > begin) load(t0 - TILE);
         fore[odd].put(w, lane, compose<VEC, false, K>(a, b, cut));
         back[odd].put(w, lane, compose<VEC, true, K>(a, d, cut));
         __syncthreads();
@@ -427,14 +428,14 @@ __device__ inline Map<1> compose_back(const bool (&cut)[K], const float (&a)[K],
     return m;
 }
 
-template <class E>
-__global__ __launch_bounds__(W_MAX *WAVE) void advantage_segments(procgen_amd_advantage p, Segments g) {
+template <class E, int WAVES>
+__global__ __launch_bounds__(WAVES *WAVE) void advantage_segments(procgen_amd_advantage p, Segments g) {
     constexpr int K = KF;
-    __shared__ Pieces<1> pieces;
+    __shared__ Pieces<1, WAVES> pieces;
     const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
     Advantage<E> r(p);
-    const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE);
-    const int part = (g.tiles * TILE + W * K - 1) / (W * K) * K;
+    const int begin = s * g.tiles * UNIT, end = min((long long)p.T, (long long)begin + (long long)g.tiles * UNIT);
+    const int part = (g.tiles * UNIT + W * K - 1) / (W * K) * K;
     const int from = min((long long)end, (long long)begin + (long long)w * part), to = min((long long)end, (long long)from + part);
     Map<1> m;
     m.identity();
@@ -453,17 +454,17 @@ __global__ __launch_bounds__(W_MAX *WAVE) void advantage_segments(procgen_amd_ad
     put_segment<1>(g, s, p.N, r.ch, m);
 }
 
-template <class E>
-__global__ __launch_bounds__(W_MAX *WAVE) void advantages(procgen_amd_advantage p, Segments g) {
-    constexpr int K = KF;
-    __shared__ Pieces<1> pieces[2];
+template <class E, int WAVES>
+__global__ __launch_bounds__(WAVES *WAVE) void advantages(procgen_amd_advantage p, Segments g) {
+    constexpr int K = KF, TILE = K * WAVES;
+    __shared__ Pieces<1, WAVES> pieces[2];
     const int lane = threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.y), W = blockDim.y, s = blockIdx.y;
     Advantage<E> r(p);
-    const int begin = s * g.tiles * TILE, end = min((long long)p.T, (long long)begin + (long long)g.tiles * TILE);
+    const int begin = s * g.tiles * UNIT, end = min((long long)p.T, (long long)begin + (long long)g.tiles * UNIT);
     const int top = begin + (end - begin - 1) / TILE * TILE;
     r.load(top + w * K, end - 1);
     float y = 0.f;
-    if (s < g.count - 1) run_segments<1>(&y, g, g.count, s + 1, p.N, r.ch, pieces[0], w, W, lane);
+    if (s < g.count - 1) run_segments(&y, g, g.count, s + 1, p.N, r.ch, pieces[0], w, W, lane);
     for (int t0 = top, odd = 0; t0 >= begin; t0 -= TILE, odd ^= 1) {
         const int t = t0 + w * K;
         bool cut[K];
@@ -492,20 +493,20 @@ __global__ __launch_bounds__(W_MAX *WAVE) void advantages(procgen_amd_advantage 
 
 bool shape_ok(int dtype, int T, int N, int D) { return known_dtype(dtype) && T >= 0 && T <= 0x7fffff00 && N >= 0 && D >= 0 && (long long)N * D <= 0x7fffff00ll; }
 
-constexpr int FULL = 1024;  // blocks of 8 waves that fill the card: two on each of the 256 compute units
-int tiles_of(int T) { return (T + TILE - 1) / TILE; }
-// how many segments a window of this many blocks' worth of chains is cut into: by its sizes alone, so that the workspace does not depend on strides
+constexpr int FULL = 512;  // blocks that fill the card: two on each of the 256 compute units
+int units_of(int T) { return (T + UNIT - 1) / UNIT; }
+// How many segments a window of so many chains is cut into: by its sizes alone, so that the workspace does not depend on strides.  Not more than 128, since
+// every segment begins with the maps of all before it.
 int segments_of(int T, long long chains) {
     const long long blocks = (chains + WAVE - 1) / WAVE;
-    if (blocks >= FULL / 2) return 1;
-    const long long wanted = (FULL + blocks - 1) / blocks, most = tiles_of(T) / 2;  // two tiles each at the least
-    return (int)std::max(1ll, std::min(wanted, most));
+    if (blocks >= FULL) return 1;
+    return (int)std::max(1ll, std::min({(FULL + blocks - 1) / blocks, units_of(T) / 2ll, 128ll}));
 }
 Segments segments(int T, long long chains, void *workspace) {
     Segments g;
     const int wanted = segments_of(T, chains);
-    g.tiles = (tiles_of(T) + wanted - 1) / wanted;
-    g.count = (tiles_of(T) + g.tiles - 1) / g.tiles;
+    g.tiles = (units_of(T) + wanted - 1) / wanted;
+    g.count = (units_of(T) + g.tiles - 1) / g.tiles;
     g.maps = (float *)workspace;
     g.state = g.maps + 2ll * g.count * chains;
     g.cuts = (uint8_t *)(g.state + chains);
@@ -523,17 +524,22 @@ int vec_for(const procgen_amd_recurrence *a, bool backward) {
     for (int i = 0; i < (backward ? 6 : 3); i++)
         if (all[i]->data && all[i]->d_stride != 1 && a->D > 1) return 1;
     for (int vec = backward || a->dtype == PROCGEN_AMD_F32 ? 2 : 4; vec > 1; vec /= 2)
-        if (a->D >= vec && (long long)a->N * ((a->D + vec - 1) / vec) >= FULL / 2 * (long long)WAVE) return vec;
+        if (a->D >= vec && (long long)a->N * ((a->D + vec - 1) / vec) >= FULL * (long long)WAVE) return vec;
     return 1;
 }
+// fn(VEC, WAVES): a window in segments has too few chains for more than one a lane
 template <class Fn>
-int by_vec(int vec, Fn fn) {
+int by_shape(const Segments &g, int vec, Fn fn) {
+    typedef std::integral_constant<int, 1> One;
+    if (g.count > 1) return fn(One(), std::integral_constant<int, WS>());
+    const std::integral_constant<int, W1> waves;
     switch (vec) {
-        case 4: return fn(std::integral_constant<int, 4>());
-        case 2: return fn(std::integral_constant<int, 2>());
-        default: return fn(std::integral_constant<int, 1>());
+        case 4: return fn(std::integral_constant<int, 4>(), waves);
+        case 2: return fn(std::integral_constant<int, 2>(), waves);
+        default: return fn(One(), waves);
     }
 }
+unsigned chain_blocks(const procgen_amd_recurrence *a, int vec) { return (unsigned)(((long long)a->N * ((a->D + vec - 1) / vec) + WAVE - 1) / WAVE); }
 
 }  // namespace
 }  // namespace learner
@@ -555,15 +561,15 @@ LIBENV_API int procgen_amd_recurrence_forward(const struct procgen_amd_recurrenc
     OnDevice on(device);
     if (on.err != hipSuccess) return (int)on.err;
     return by_dtype(a->dtype, [&](auto e) {
-        return by_vec(vec_for(a, false), [&](auto vec) {
+        return by_shape(g, vec_for(a, false), [&](auto vec, auto waves) {
             typedef decltype(e) E;
-            constexpr int VEC = decltype(vec)::value;
-            const dim3 grid((unsigned)(((long long)a->N * ((a->D + VEC - 1) / VEC) + WAVE - 1) / WAVE), g.count), block(WAVE, std::min(W_MAX, (a->T + KF - 1) / KF));
-            if (g.count > 1) {
-                recurrence_segments<E, VEC, false><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
+            constexpr int VEC = decltype(vec)::value, WAVES = decltype(waves)::value;
+            const dim3 grid(chain_blocks(a, VEC), g.count), block(WAVE, std::min(WAVES, (a->T + KF - 1) / KF));
+            if constexpr (WAVES == WS) {
+                recurrence_segments<E, VEC, WAVES, false><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
                 if (int err = launched()) return err;
             }
-            recurrence_forward<E, VEC><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
+            recurrence_forward<E, VEC, WAVES><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
             return launched();
         });
     });
@@ -578,15 +584,15 @@ LIBENV_API int procgen_amd_recurrence_backward(const struct procgen_amd_recurren
     OnDevice on(device);
     if (on.err != hipSuccess) return (int)on.err;
     return by_dtype(a->dtype, [&](auto e) {
-        return by_vec(vec_for(a, true), [&](auto vec) {
+        return by_shape(g, vec_for(a, true), [&](auto vec, auto waves) {
             typedef decltype(e) E;
-            constexpr int VEC = std::min(2, decltype(vec)::value);
-            const dim3 grid((unsigned)(((long long)a->N * ((a->D + VEC - 1) / VEC) + WAVE - 1) / WAVE), g.count), block(WAVE, std::min(W_MAX, (a->T + KB - 1) / KB));
-            if (g.count > 1) {
-                recurrence_segments<E, VEC, true><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
+            constexpr int VEC = std::min(2, decltype(vec)::value), WAVES = decltype(waves)::value;
+            const dim3 grid(chain_blocks(a, VEC), g.count), block(WAVE, std::min(WAVES, (a->T + KB - 1) / KB));
+            if constexpr (WAVES == WS) {
+                recurrence_segments<E, VEC, WAVES, true><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
                 if (int err = launched()) return err;
             }
-            recurrence_backward<E, VEC><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
+            recurrence_backward<E, VEC, WAVES><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
             return launched();
         });
     });
@@ -601,12 +607,15 @@ LIBENV_API int procgen_amd_advantages(const struct procgen_amd_advantage *a, int
     if (on.err != hipSuccess) return (int)on.err;
     return by_dtype(a->dtype, [&](auto e) {
         typedef decltype(e) E;
-        const dim3 grid((a->N + WAVE - 1) / WAVE, g.count), block(WAVE, std::min(W_MAX, (a->T + KF - 1) / KF));
+        const unsigned blocks = (a->N + WAVE - 1) / WAVE;
         if (g.count > 1) {
-            advantage_segments<E><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
+            const dim3 grid(blocks, g.count), block(WAVE, WS);
+            advantage_segments<E, WS><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
             if (int err = launched()) return err;
+            advantages<E, WS><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
+        } else {
+            advantages<E, W1><<<blocks, dim3(WAVE, std::min(W1, (a->T + KF - 1) / KF)), 0, (hipStream_t)stream>>>(*a, g);
         }
-        advantages<E><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
         return launched();
     });
 }
