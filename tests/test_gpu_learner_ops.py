@@ -117,7 +117,9 @@ RECURRENCES = [
     (63, 2, 32, "f32", False, True, "tnd"), (64, 1, 256, "bf16", True, True, "tnd"), (65, 3, 40, "f16", True, True, "ntd"), (127, 9, 24, "bf16", False, False, "slice"),
     (129, 2, 33, "f32", True, True, "strided"), (256, 8, 64, "bf16", True, True, "ntd"), (1000, 1, 5, "f32", True, True, "tnd"), (2049, 1, 16, "f16", False, True, "tnd"),
     (5000, 2, 3, "bf16", True, True, "ntd"), (31, 1, 2000, "f32", True, False, "slice"), (40, 300, 1, "bf16", True, True, "strided"), (7, 129, 65, "f16", True, True, "tnd"),
-    (12345, 1, 1, "f32", True, True, "tnd"),
+    (12345, 1, 1, "f32", True, True, "tnd"), (3, 700, 100, "bf16", True, True, "tnd"), (4, 300, 257, "f16", True, False, "ntd"), (1, 2100, 133, "f32", True, True, "slice"),
+    (1, 9000, 61, "bf16", True, True, "tnd"), (4, 40, 30, "f32", False, True, "strided"), (5, 900, 150, "bf16", True, True, "tnd"), (100, 700, 101, "bf16", True, True, "ntd"),
+    (20000, 1, 70, "bf16", True, True, "slice"),
 ]
 
 
