@@ -12,7 +12,8 @@
 // product() is the hardware's multiplication in which zero times anything is zero.
 // Partial sums of a row are taken against the largest value their lane or wave has seen and rescaled when they meet (Stats::join), so a row is read once.
 //
-// Bound by memory: a column costs 12 operations for 4 to 8 bytes, 23 for 6 to 12 with a reference.  By the number of columns:
+// Bound by memory: a column costs 12 operations for 4 to 8 bytes, 23 for 6 to 12 with a reference (a 1 GiB copy reaches 5.1 TB/s on the same card).  By
+// the number of columns:
 //   up to 32      a wave takes 64 rows through LDS, a lane per row: no reduction over lanes, coalesced although a row is no multiple of anything
 //   up to 4096    a group of 4 to 64 lanes per row, the whole row in their registers between the sums and the gradient (2048 in float32)
 //   more          a block per row, in batches; the gradient goes through them backwards: the last is still in registers, those before it in LDS, and
@@ -384,6 +385,8 @@ constexpr int short_residents() {
     return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? 3 : sizeof(typename E::T) == 4 ? 4 : 5) : REF ? 2 : 3;
 }
 
+// Loss and gradient of 4 194 304 x 15 bf16: 70 to 76 us, 306 MB, 4.1 to 4.4 TB/s; without fetching ahead 98, with the register limit of six blocks (and
+// spills) 93, of four 78.  What is left is the issue of vector instructions: some 300 for 64 rows.
 template <class E, int MOST, bool REF, class Op>
 __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void short_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
@@ -520,6 +523,8 @@ struct Place {
 };
 
 // Rows that fit the registers of a group inside of a wave: the next rows are on their way while these are worked on.
+// Loss and gradient of 64 M bf16 logits at 64, 512, 1024, 2000 columns: 68, 55, 55, 57 us (4.2 to 4.9 TB/s), with a reference 91, 81, 81, 87; at 65 and 300
+// columns, which leave two fifths of the lanes without any, 115 and 98.
 template <class E, int G, int CH, bool REF, class Op>
 __global__ __launch_bounds__(BLOCK) void group_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
@@ -622,6 +627,8 @@ __global__ __launch_bounds__(BLOCK) void group_rows(procgen_amd_rows p, Op op, c
 }
 
 // A block per row, in batches of G lanes times CH chunks; the next batch is on its way while one is summed up.
+// Loss and gradient of 2048 x 50021 bf16 with a reference: 154 us for 615 MB, 4.0 TB/s; some 230 MB are read twice, so that memory sees 5.5.  With rows at
+// their own alignment 204, without columns kept in LDS 173.  Log-probabilities of 1000 x 32001: 15 us, 4.3 TB/s.
 template <class E, int G, int CH, bool REF, class Op>
 __global__ __launch_bounds__(G, 4) void long_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
@@ -760,7 +767,7 @@ __global__ __launch_bounds__(G, 4) void long_rows(procgen_amd_rows p, Op op, con
     if (partial) put_sums(sums, op, partial);
 }
 
-// the gradient of long rows' log-probabilities: lse and entropy are known, so every column stands for itself
+// The gradient of long rows' log-probabilities: lse and entropy are known, so every column stands for itself.  1000 x 32001 bf16: 24 us, 5.3 TB/s.
 template <class E>
 __global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, const float *lse, const float *entropy, const float *d_logp, const float *d_entropy) {
     typedef typename E::T T;
@@ -798,7 +805,8 @@ __global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, c
 
 // ---- the mean ------------------------------------------------------------------------------------------------------------------------------------
 
-// how many rows count: one partial sum per block, added up by every wave that needs the number (whole numbers: any order gives the same)
+// 4 194 304 flags in 5 us, most of it the launch's own.
+// How many rows count: one partial sum per block, added up by every wave that needs the number (whole numbers: any order gives the same)
 __global__ __launch_bounds__(BLOCK) void count_valid(const uint8_t *valid, long long rows, long long *counts) {
     long long n = 0;
     const long long head = min(rows, (long long)(-(uintptr_t)valid & 15)), wide = (rows - head) / 16;  // bytes before the first aligned 16, and 16s

@@ -10,6 +10,9 @@
 //   segment  where there are too few chains to fill the card, the window is cut into segments for blocks of their own: a first kernel composes each
 //            segment's map, the second begins each segment with the maps of those before it (the data is read twice)
 // Lanes are chains (VEC neighbouring channels each), so that every load of a step is one coalesced row piece.
+//
+// Bound by memory: two to five operations an element.  A 1 GiB copy reaches 5.1 TB/s on the same card, a read alone 3.9; times below are of kernels whose
+// inputs come from HBM.
 #include "learner.h"
 
 #include <algorithm>
@@ -212,7 +215,8 @@ __device__ inline void convert(bool (&cut)[K], const uint8_t (&raw)[K], uint8_t 
     for (int k = 0; k < K; k++) cut[k] = t + k < end && (raw[k] & mask);
 }
 
-// the map of every segment (blockIdx.y): forwards of gate and update, backwards of gate and d_h.  The waves take a part of the segment each.
+// 32768 x 512 float32: 37 us forwards (134 MB read, 3.6 TB/s: the rate of a read), 25 backwards (the gates still in the Infinity Cache).
+// The map of every segment (blockIdx.y): forwards of gate and update, backwards of gate and d_h.  The waves take a part of the segment each.
 template <class E, int VEC, int WAVES, bool REVERSE>
 __global__ __launch_bounds__(WAVES *WAVE) void recurrence_segments(procgen_amd_recurrence p, Segments g) {
     constexpr int K = KF;
@@ -255,6 +259,8 @@ __global__ __launch_bounds__(WAVES *WAVE) void recurrence_segments(procgen_amd_r
     }
 }
 
+// 256 x 512 x 256 bf16: 46 us, 210 MB with the checkpoints, 4.6 TB/s (eight waves a block 49, two channels a lane 49).  32768 x 512 float32 behind its
+// segments: 39 us, 5.2 TB/s.  What is left: the last tiles of a block have nothing on its way, and 2048 blocks of four waves end at different times.
 template <class E, int VEC, int WAVES>
 __global__ __launch_bounds__(WAVES *WAVE) void recurrence_forward(procgen_amd_recurrence p, Segments g) {
     constexpr int K = KF, TILE = K * WAVES;
@@ -307,6 +313,8 @@ __global__ __launch_bounds__(WAVES *WAVE) void recurrence_forward(procgen_amd_re
 
 // Backwards over the tiles.  h is not read: its 32-bit value before every step comes from the checkpoint at the tile's start and the same joins as in
 // the forward pass (update is read in its place, so the bytes are the same and 16-bit rounding of h does not reach d_gate).
+// 256 x 512 x 256 bf16: 74 us, 344 MB, 4.6 TB/s; tiles of 64 steps over eight waves took 96 (158 registers, one block on a compute unit), of 32 steps 78.
+// 32768 x 512 float32: 63 us, 5.4 TB/s.
 template <class E, int VEC, int WAVES>
 __global__ __launch_bounds__(WAVES *WAVE) void recurrence_backward(procgen_amd_recurrence p, Segments g) {
     constexpr int K = KB, TILE = K * WAVES;
@@ -529,6 +537,7 @@ __global__ __launch_bounds__(WAVES *WAVE) void advantage_segments(procgen_amd_ad
     put_segment<1>(g, s, p.N, r.ch, m);
 }
 
+// 256 x 65536, values in float32: 55 us, 286 MB, 5.2 TB/s: the rate of a copy.
 template <class E, int WAVES>
 __global__ __launch_bounds__(WAVES *WAVE) void advantages(procgen_amd_advantage p, Segments g) {
     constexpr int K = KF, TILE = K * WAVES;
