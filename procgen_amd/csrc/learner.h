@@ -1,7 +1,5 @@
 // learner.h -- what the learner kernels (learner_scan.hip, learner_rows.hip) share: element types, wave reductions, launches at a C entry.
 #pragma once
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -22,14 +20,6 @@ struct F16 {
 struct BF16 {
     typedef __bf16 T;
 };
-template <class E>
-__device__ inline float load(const void *p, long long i) {
-    return (float)((const typename E::T *)p)[i];
-}
-template <class E>
-__device__ inline void store(void *p, long long i, float v) {
-    ((typename E::T *)p)[i] = (typename E::T)v;  // nearest even
-}
 
 // ---- reductions over a wave (every lane gets the result); `op` is taken in a fixed order, so results do not change from run to run ----
 template <class T, class Op>
@@ -37,9 +27,6 @@ __device__ inline T wave_reduce(T v, Op op) {
     for (int d = WAVE / 2; d > 0; d >>= 1) v = op(v, __shfl_xor(v, d, WAVE));
     return v;
 }
-struct Max {
-    __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
-};
 struct Sum {
     template <class T>
     __device__ T operator()(T a, T b) const { return a + b; }

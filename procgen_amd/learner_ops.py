@@ -74,6 +74,14 @@ def _number(x, what, low=float("-inf"), high=float("inf")):
         raise ValueError(f"{what} has to lie in [{low}, {high}], not {x}")
 
 
+_MOST = 0x7FFFFF00  # steps, chains, rows: counted in 32 bits
+
+
+def _not_too_many(n, what):
+    if n > _MOST:
+        raise ValueError(f"{n} {what}: more than {_MOST} are not taken")
+
+
 _FLAGS = (torch.uint8, torch.bool)
 _F32 = (torch.float32,)
 _INTS = (torch.int32, torch.int64)
@@ -126,6 +134,8 @@ def gated_recurrence(gate, update, first=None, state=None, state_out=None):
         _need(state_out.is_contiguous(), "state_out has to be contiguous")
         _need(not _wants_grad(gate, update, state, state_out), "state_out overwrites a state: call under torch.no_grad(), or take the returned state")
     _on_gpu(gate, update, first, state, state_out)
+    _not_too_many(shape[0], "steps")
+    _not_too_many(shape[1:].numel(), "chains")
     if state_out is not None:
         for x, what in ((gate, "gate"), (update, "update"), (first, "first"), (state, "state")):
             if x is not None and _overlap(x, state_out) and not (what == "state" and x.data_ptr() == state_out.data_ptr() and x.is_contiguous()):
@@ -166,6 +176,8 @@ def advantages(rew, values, first, *, gamma, lam):
     _constant(rew, "rew")
     _constant(values, "values")
     device = _on_gpu(rew, values, first)
+    _not_too_many(T, "steps")
+    _not_too_many(N, "envs")
     if T and N:
         return _ext.advantages(rew, values, first, gamma, lam)
     return tuple(torch.empty((T, N), dtype=torch.float32, device=device) for _ in range(2))
@@ -201,6 +213,8 @@ def _check_rows(logits, actions):
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError("logits have to be [..., columns] with one column at least")
     _tensor(actions, "actions", _INTS, logits.shape[:-1])
+    _not_too_many(actions.numel(), "rows")
+    _not_too_many(logits.shape[-1] + (1 << 18), "columns")
 
 
 def action_logprobs(logits, actions):

@@ -116,6 +116,8 @@ class Rollout:
         for _ in range(256):
             env.act(actions); env.observe(); window.record()
         adv, ret = window.advantages(values, gamma=0.999, lam=0.95)   # values [steps + 1, N]: the value head on observations 0 .. steps
+        h, memory = window.recurrence(gate, update, memory)       # a recurrent policy over the window
+        out = window.policy_loss(logits, old_logprobs, adv)       # logits [steps, N, columns]
         window.restart()                                          # the last observation is the first of the next window
 
     rew float32 [steps, N] and action int32 [steps, N]: of the acts; first uint8 [steps + 1, N]: of the observations.  record() copies the part arrays
@@ -152,15 +154,31 @@ class Rollout:
 
     def restart(self):
         """begins the next window with the observation that this one ended with"""
-        if self.recorded <= self.steps:
-            raise ValueError(f"{self.recorded} of the window's {self.steps + 1} observations are recorded")
+        self._full()
         self.first[0].copy_(self.first[-1])
         self.recorded = 1
 
-    def advantages(self, values, *, gamma, lam):
-        """(adv, ret) float32 [steps, N] of the full window: learner_ops.advantages of its rewards and episode starts"""
+    def _full(self):
         from . import learner_ops
 
         if self.recorded <= self.steps:
             raise ValueError(f"{self.recorded} of the window's {self.steps + 1} observations are recorded")
-        return learner_ops.advantages(self.rew, values, self.first, gamma=gamma, lam=lam)
+        return learner_ops
+
+    def advantages(self, values, *, gamma, lam):
+        """(adv, ret) float32 [steps, N] of the full window: learner_ops.advantages of its rewards and episode starts"""
+        return self._full().advantages(self.rew, values, self.first, gamma=gamma, lam=lam)
+
+    def recurrence(self, gate, update, state=None):
+        """learner_ops.gated_recurrence over the observations 0 .. steps - 1, cut where an episode begins: gate, update [steps, N, D]; state: the
+        memory that the window began with"""
+        return self._full().gated_recurrence(gate, update, self.first[:-1], state)
+
+    def action_logprobs(self, logits):
+        """learner_ops.action_logprobs of the window's actions; NaN for a forced reset's"""
+        return self._full().action_logprobs(logits, self.action)
+
+    def policy_loss(self, logits, old_logprobs, advantages, valid=None, **kw):
+        """learner_ops.policy_loss of the window's actions; forced resets (action -1) are left out, whatever `valid` says of them"""
+        acted = self.action >= 0
+        return self._full().policy_loss(logits, self.action, old_logprobs, advantages, valid=acted if valid is None else acted & valid.bool(), **kw)

@@ -960,6 +960,15 @@ def test_rollout_of_a_handle_feeds_the_operators(names, devices):
         out = ops().policy_loss(logits, window.action, logp, adv, valid=valid)
         (d,) = torch.autograd.grad(out.loss, logits)
         assert abs(out.loss.item() + adv[valid].double().mean().item()) < 1e-5 and d.isfinite().all() and (d[~valid] == 0).all()  # ratio 1: the loss is minus the mean advantage
+        same = window.policy_loss(logits, logp, adv)
+        assert torch.equal(same.loss, out.loss) and torch.equal(same.stats, out.stats) and torch.equal(window.action_logprobs(logits.detach())[0].nan_to_num(9.0), logp.nan_to_num(9.0))
+        half = window.policy_loss(logits, logp, adv, valid=torch.arange(n, device="cuda").expand(T, n) % 2)
+        assert abs(half.loss.item() + adv[:, 1::2][valid[:, 1::2]].double().mean().item()) < 1e-5
+        gate, update = torch.rand((T, n, 8), generator=gen(part)).cuda(), rand((T, n, 8), gen(20 + part)).cuda()
+        memory = torch.zeros((n, 8), device="cuda") if part == 0 else memory
+        want = recurrence_64(gate.cpu(), update.cpu(), firsts[:-1], memory.cpu())
+        h, memory = window.recurrence(gate, update, memory)
+        check(h, want["h"], want["E_h"] + rounding(want["h"], torch.float32), "memory over the window")
         with pytest.raises(ValueError):
             window.record()
         window.restart()

@@ -93,6 +93,21 @@ def test_refusals(kind, call):
         call()
 
 
+def test_more_than_32_bits_can_count_is_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_on_gpu", lambda x, *others: x.device)  # the shapes are checked behind the devices
+    one = z(1)
+    with pytest.raises(ValueError, match="steps"):
+        ops.gated_recurrence(one.expand(1 << 31, 1), one.expand(1 << 31, 1))
+    with pytest.raises(ValueError, match="chains"):
+        ops.gated_recurrence(one.expand(1, 1 << 16, 1 << 16), one.expand(1, 1 << 16, 1 << 16))
+    with pytest.raises(ValueError, match="envs"):
+        ops.advantages(one.expand(1, 1 << 31), one.expand(2, 1 << 31), z(1, dtype=U).expand(2, 1 << 31), gamma=0.9, lam=0.9)
+    with pytest.raises(ValueError, match="rows"):
+        ops.action_logprobs(one.expand(1 << 31, 1), z(1, dtype=torch.int32).expand(1 << 31))
+    with pytest.raises(ValueError, match="columns"):
+        ops.action_logprobs(one.expand(1, 1 << 31), z(1, dtype=torch.int32))
+
+
 def test_layouts():
     x = torch.zeros(6, 5, 4, 8)
     assert ops._layout(x, "x") == (1, 8, 0)  # (rows per inner group, stride of the groups, stride inside)
