@@ -165,7 +165,7 @@ struct Coef {
 // Each operator's rows: what it fetches for a row besides its logits, whether it wants the row at all, what it makes of the row's sums.  finish() is
 // called once per row by one lane at least, with `first` set in exactly one; it returns whether the row's gradient is anything but zero.
 struct Logprobs {
-    static constexpr bool GRADIENT = false;
+    static constexpr bool GRADIENT = false, HEAVY = false;
     __device__ bool done() const { return false; }
     float *logp, *entropy, *lse;
     struct In {};
@@ -184,7 +184,7 @@ struct Logprobs {
 };
 
 struct LogprobsBackward {  // of rows short enough to sum up again
-    static constexpr bool GRADIENT = true;
+    static constexpr bool GRADIENT = true, HEAVY = false;
     __device__ bool done() const { return false; }
     const float *d_logp, *d_entropy;
     struct In {
@@ -202,7 +202,7 @@ struct LogprobsBackward {  // of rows short enough to sum up again
 };
 
 struct Policy {
-    static constexpr bool GRADIENT = true;
+    static constexpr bool GRADIENT = true, HEAVY = true;  // HEAVY: a row's own numbers, its sums and their addresses keep some 30 registers more
     __device__ bool done() const { return (q.resume & 2) && *q.scale == 1.f; }  // the gradient that is there is the one that is wanted
     procgen_amd_policy q;
     const long long *counts;
@@ -332,7 +332,15 @@ struct Chunk {
 
 // 64 rows on their way from memory to LDS (`rows` of them exist).  Contiguous rows go 16 bytes a lane and, where they are few registers, are fetched
 // while the 64 before them are worked on; others go element by element.
-template <class E, int MOST>
+//
+// Rows of 16 float32 are 64 bytes: lanes that all read one column of theirs would meet in four of the 64 banks.  With TURN a row's four chunks are
+// swapped by the row's place, and 16 lanes that read a chunk each go over every bank once.  Loss and gradient of 4 194 304 x 16 float32: 107 us instead of 150, with a
+// reference 160 instead of 204, of the log-probabilities 103 instead of 143.
+template <class E, int MOST, bool TURN>
+__device__ inline int place(int i) {  // in LDS, of element i of the 64 rows
+    return TURN ? i ^ (i / (4 * MOST) % (MOST / Chunk<E>::N) * Chunk<E>::N) : i;
+}
+template <class E, int MOST, bool TURN = false>
 struct Tile {
     typedef typename E::T T;
     static constexpr int N = Chunk<E>::N, CHUNKS = MOST * (int)sizeof(T) / 16;  // 64 rows of MOST columns: so many 16 bytes a lane
@@ -356,20 +364,20 @@ struct Tile {
 #pragma unroll
                 for (int i = 0; i < (AHEAD ? CHUNKS : 0); i++) {
                     const int at = (i * WAVE + lane) * N;
-                    if (at + N <= n) *(Bits *)(lds + at) = c[i];
+                    if (at + N <= n) *(Bits *)(lds + place<E, MOST, TURN>(at)) = c[i];
                 }
             } else {
                 for (int at = lane * N; at + N <= n; at += WAVE * N) {
                     Bits k;
                     __builtin_memcpy(&k, src + at, 16);
-                    *(Bits *)(lds + at) = k;
+                    *(Bits *)(lds + place<E, MOST, TURN>(at)) = k;
                 }
             }
-            if (n / N * N + lane < n) lds[n / N * N + lane] = src[n / N * N + lane];
+            if (n / N * N + lane < n) lds[place<E, MOST, TURN>(n / N * N + lane)] = src[n / N * N + lane];
         } else {
             for (int i = lane; i < n; i += WAVE) {
                 const int r = i / columns;
-                lds[i] = ((const T *)from)[row_offset(p, r0 + r, outer, inner) + (i - r * columns)];
+                lds[place<E, MOST, TURN>(i)] = ((const T *)from)[row_offset(p, r0 + r, outer, inner) + (i - r * columns)];
             }
         }
     }
@@ -379,27 +387,32 @@ __device__ inline void lds_settled() {  // a wave's own LDS is written and read 
     __builtin_amdgcn_wave_barrier();
 }
 
+// bytes of LDS that 64 rows take, with slack for the columns that the last row does not have
+template <class E, int MOST>
+__host__ __device__ constexpr int short_tile(int columns) {
+    return ((WAVE * columns * (int)sizeof(typename E::T) + 15) & ~15) + MOST * (int)sizeof(typename E::T);
+}
 // blocks of four waves that a compute unit holds: by registers (three, or four with a reference, for each of MOST columns) and by LDS
-template <class E, int MOST, bool REF>
+template <class E, int MOST, bool REF, bool TURN = false>
 constexpr int short_residents() {
-    return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? 3 : sizeof(typename E::T) == 4 ? 4 : 5) : REF ? 2 : 3;
+    return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? (TURN ? 2 : 3) : sizeof(typename E::T) == 4 ? 4 : 5) : REF ? 2 : 3;
 }
 
-// Loss and gradient of 4 194 304 x 15 bf16: 70 to 76 us, 306 MB, 4.1 to 4.4 TB/s; without fetching ahead 98, with the register limit of six blocks (and
-// spills) 93, of four 78.  What is left is the issue of vector instructions: some 300 for 64 rows.
-template <class E, int MOST, bool REF, class Op>
-__global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void short_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
+// Loss and gradient of 4 194 304 x 15 bf16: 67 to 76 us, 306 MB, 4.0 to 4.6 TB/s; without fetching ahead 98, with the register limit of six blocks (and
+// spills) 93, of four 78.  What is left is the issue of instructions: some 380 vector and 230 scalar ones for 64 rows.
+template <class E, int MOST, bool REF, class Op, bool TURN = false>
+__global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) void short_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), columns = (int)p.columns;
-    const int bytes = (WAVE * columns * (int)sizeof(T) + 15) & ~15;
+    const int bytes = short_tile<E, MOST>(columns);
     T *const tile = (T *)(lds + (size_t)wave * bytes * (REF ? 2 : 1)), *const tile2 = (T *)((char *)tile + bytes);
     if (op.done()) return;
     op.begin(p);
     Sums sums;
     const long long step = (long long)gridDim.x * (BLOCK / WAVE) * WAVE;
-    Tile<E, MOST> next;
-    Tile<E, REF ? MOST : 8> next2;
+    Tile<E, MOST, TURN> next;
+    Tile<E, REF ? MOST : 8, REF && TURN> next2;
     typename Op::In next_in;
     int next_a = -1;  // -1: not one of the columns
     auto fetch = [&](long long r0) {
@@ -424,23 +437,28 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
         if (REF) next2.put(tile2, p, ref, ref_outer, ref_inner, r0, rows, lane);
         lds_settled();
         if (r0 + step < p.rows) fetch(r0 + step);
+        const int turn = TURN ? place<E, MOST, TURN>(lane * MOST) % MOST : 0;
         T *const row = tile + lane * columns;
         const T *const row2 = tile2 + lane * columns;
         bool some = false;
         Coef c;
         if (wanted) {
             // more than MOST / 2 columns, the others -inf; l and l2 become t and q
+            // reads what a row has not and drops it, which keeps the reads together; where registers are short it is not read (15 bf16 67 : 76 us)
+            constexpr bool GUARD = Op::HEAVY && MOST == 16 && !REF && sizeof(T) == 2;
+            constexpr int surely = TURN ? MOST : MOST > 8 ? MOST / 2 : 0;
             float l[MOST], e[MOST], l2[REF ? MOST : 1];
             Stats<REF> x;
 #pragma unroll
             for (int j = 0; j < MOST; j++) {
-                const bool real = MOST > 8 && j <= MOST / 2 ? true : j < columns;
-                l[j] = real ? (float)row[j] : -INFINITY;
+                l[j] = !GUARD || j <= surely || j < columns ? (float)row[j ^ turn] : -INFINITY;  // of the row behind, or of the tile's slack, where there is no such column
+                if (REF) l2[j] = (float)row2[j ^ turn];
+            }
+#pragma unroll
+            for (int j = 0; j < MOST; j++) {
+                if (!GUARD && j > surely && j >= columns) l[j] = l2[REF ? j : 0] = -INFINITY;
                 x.m = fmaxf(x.m, l[j]);
-                if (REF) {
-                    l2[j] = real ? (float)row2[j] : -INFINITY;
-                    x.m2 = fmaxf(x.m2, l2[j]);
-                }
+                if (REF) x.m2 = fmaxf(x.m2, l2[j]);
             }
             const Base b(x.m), b2(x.m2);
 #pragma unroll
@@ -456,16 +474,16 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
                 }
             }
             const bool known = a >= 0;
-            const float taken = known ? (float)row[a] : 0.f, taken2 = REF && known ? (float)row2[a] : 0.f;
+            const float taken = known ? (float)row[a ^ turn] : 0.f, taken2 = REF && known ? (float)row2[a ^ turn] : 0.f;
             some = op.template finish<REF>(r, in, x, known, taken, true, c, sums);
             if (Op::GRADIENT && some && p.d_logits) {
 #pragma unroll
                 for (int j = 0; j < MOST; j++) {
                     float f = fmaf(c.cd, l[j], c.c0);
                     if (REF) f = fmaf(c.cq, l2[j], f);
-                    if ((MOST > 8 && j <= MOST / 2) || j < columns) row[j] = (T)product(e[j], f);
+                    if (j <= surely || j < columns) row[j ^ turn] = (T)product(e[j], f);
                 }
-                if (known) row[a] = (T)(c.gradient<REF>(taken, taken2) + c.pick);
+                if (known) row[a ^ turn] = (T)(c.gradient<REF>(taken, taken2) + c.pick);
                 if (c.b.base != c.b.base)
                     for (int j = 0; j < columns; j++) row[j] = (T)NAN;
             }
@@ -480,10 +498,10 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF>())) void shor
             for (int i = lane * N; i < n; i += WAVE * N) {
                 if (i + N <= n) {
                     Chunk<E> k;
-                    k.w = *(const Bits *)(tile + i);
+                    k.w = *(const Bits *)(tile + place<E, MOST, TURN>(i));
                     k.store(out + i);
                 } else {
-                    for (int k = i; k < n; k++) out[k] = tile[k];
+                    for (int k = i; k < n; k++) out[k] = tile[place<E, MOST, TURN>(k)];
                 }
             }
             lds_settled();
@@ -868,15 +886,17 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
     const bool aligned = ((uintptr_t)p.logits | (uintptr_t)(p.outer_stride * SIZE) | (uintptr_t)(p.inner_stride * SIZE)) % 16 == 0;
     const long long padded = p.columns + (aligned ? 0 : N - 1);
     // A lane per row, where its registers leave enough waves.  Over 64 M columns in all, against the
-    // groups: 16-bit 17 columns 102 : 190 us, 24 80 : 122, 32 88 : 96, 33 127 : 152, 48 112 : 87; float32 16 149 : 171, 24 137 : 143, 32
-    // 276 : 127; float32 with a reference 16 227 : 203, 24 252 : 168.
-    const bool lane_per_row = SIZE == 2 ? p.columns <= 32 : p.columns <= (REF ? 15 : 24);
+    // groups: 16-bit 17 columns 95 : 190 us, 24 70 : 122, 32 68 : 96, 33 127 : 152, 48 112 : 87; float32 16 107 : 171, 24 140 : 143, 32
+    // 276 : 127; float32 with a reference 16 160 : 203, 24 252 : 168.
+    const bool lane_per_row = SIZE == 2 ? p.columns <= 32 : p.columns <= (REF ? 16 : 24);
     if (lane_per_row) {
-        const size_t lds = ((WAVE * p.columns * SIZE + 15) & ~15ull) * (BLOCK / WAVE) * (REF ? 2 : 1);
-        if (p.columns <= 8) short_rows<E, 8, REF, Op><<<short_grid(CUS * short_residents<E, 8, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<short_grid(CUS * short_residents<E, 16, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        auto lds = [&](int tile) { return (size_t)tile * (BLOCK / WAVE) * (REF ? 2 : 1); };
+        if (p.columns <= 8) short_rows<E, 8, REF, Op><<<short_grid(CUS * short_residents<E, 8, REF>()), BLOCK, lds(short_tile<E, 8>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if (SIZE == 4 && p.columns == 16)
+            short_rows<E, 16, REF, Op, SIZE == 4><<<short_grid(CUS * short_residents<E, 16, REF, SIZE == 4>()), BLOCK, lds(short_tile<E, 16>(16)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<short_grid(CUS * short_residents<E, 16, REF>()), BLOCK, lds(short_tile<E, 16>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         else if constexpr (SIZE == 2 || !REF)
-            short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+            short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds(short_tile<E, 32>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (padded <= 4 * 1 * N) {
         group_rows<E, 4, 1, REF, Op><<<grid(BLOCK / 4, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (padded <= 4 * 2 * N) {

@@ -401,6 +401,8 @@ LOGITS = [
     (1, 1, "f32", "plain"), (1, 2, "bf16", "plain"), (3, 15, "f32", "plain"), (64, 15, "bf16", "plain"), (130, 15, "f16", "pitch"), (1000, 15, "bf16", "window"), (257, 16, "f32", "plain"),
     (65, 7, "bf16", "plain"), (100, 63, "f16", "window"), (77, 64, "bf16", "plain"), (77, 65, "f32", "plain"), (40, 128, "bf16", "pitch"), (33, 1000, "bf16", "plain"), (8, 1023, "f16", "pitch"),
     (5, 4099, "f32", "plain"), (300, 4096, "bf16", "plain"), (2, 32001, "bf16", "plain"), (1, 131072, "f16", "plain"), (3, 50021, "bf16", "pitch"), (1, 100003, "f32", "plain"), (6, 20000, "f32", "window"),
+    (129, 16, "f32", "pitch"), (514, 16, "f32", "window"), (1000, 16, "f32", "plain"), (70, 17, "bf16", "plain"), (130, 31, "f16", "window"), (66, 24, "f32", "plain"), (200, 9, "bf16", "pitch"),
+    (66, 8, "f16", "plain"), (129, 32, "bf16", "plain"),
 ]
 
 
