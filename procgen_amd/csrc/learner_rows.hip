@@ -333,18 +333,18 @@ struct Chunk {
 // 64 rows on their way from memory to LDS (`rows` of them exist).  Contiguous rows go 16 bytes a lane and, where they are few registers, are fetched
 // while the 64 before them are worked on; others go element by element.
 //
-// Rows of 16 float32 are 64 bytes: lanes that all read one column of theirs would meet in four of the 64 banks.  With TURN a row's four chunks are
-// swapped by the row's place, and 16 lanes that read a chunk each go over every bank once.  Loss and gradient of 4 194 304 x 16 float32: 107 us instead of 150, with a
-// reference 160 instead of 204, of the log-probabilities 103 instead of 143.
+// Rows of 16 or 32 float32 are 64 or 128 bytes: lanes that all read one column of theirs would meet in four or two of the 64 banks.  With TURN a row's
+// chunks are swapped by the row's place, and 16 lanes that read a chunk each go over every bank once.  Loss and gradient of 4 194 304 x 16 float32: 107
+// us instead of 150, with a reference 160 instead of 204, of the log-probabilities 103 instead of 143.
 template <class E, int MOST, bool TURN>
 __device__ inline int place(int i) {  // in LDS, of element i of the 64 rows
-    return TURN ? i ^ (i / (4 * MOST) % (MOST / Chunk<E>::N) * Chunk<E>::N) : i;
+    return TURN ? i ^ (i / MOST * MOST / 64 % (MOST / Chunk<E>::N) * Chunk<E>::N) : i;
 }
 template <class E, int MOST, bool TURN = false>
 struct Tile {
     typedef typename E::T T;
     static constexpr int N = Chunk<E>::N, CHUNKS = MOST * (int)sizeof(T) / 16;  // 64 rows of MOST columns: so many 16 bytes a lane
-    static constexpr bool AHEAD = CHUNKS <= 4;
+    static constexpr bool AHEAD = CHUNKS <= 8;
     Bits c[AHEAD ? CHUNKS : 1];
     __device__ void fetch(const procgen_amd_rows &p, const void *from, long long outer, long long r0, int rows, int lane) {
         if (!AHEAD || p.inner != 1 || outer != p.columns) return;
@@ -395,7 +395,7 @@ __host__ __device__ constexpr int short_tile(int columns) {
 // blocks of four waves that a compute unit holds: by registers (three, or four with a reference, for each of MOST columns) and by LDS
 template <class E, int MOST, bool REF, bool TURN = false>
 constexpr int short_residents() {
-    return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? (TURN ? 2 : 3) : sizeof(typename E::T) == 4 ? 4 : 5) : REF ? 2 : 3;
+    return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? (TURN ? 2 : 3) : sizeof(typename E::T) == 4 ? 4 : 5) : MOST <= 24 ? (REF ? 2 : sizeof(typename E::T) == 4 ? 3 : 4) : REF || sizeof(typename E::T) == 4 ? 2 : 3;
 }
 
 // Loss and gradient of 4 194 304 x 15 bf16: 67 to 76 us, 306 MB, 4.0 to 4.6 TB/s; without fetching ahead 98, with the register limit of six blocks (and
@@ -443,10 +443,10 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) voi
         bool some = false;
         Coef c;
         if (wanted) {
-            // more than MOST / 2 columns, the others -inf; l and l2 become t and q
+            // the columns that a row has not are -inf; l and l2 become t and q
             // reads what a row has not and drops it, which keeps the reads together; where registers are short it is not read (15 bf16 67 : 76 us)
             constexpr bool GUARD = Op::HEAVY && MOST == 16 && !REF && sizeof(T) == 2;
-            constexpr int surely = TURN ? MOST : MOST > 8 ? MOST / 2 : 0;
+            constexpr int surely = TURN ? MOST : MOST > 16 ? MOST - 8 : MOST > 8 ? MOST / 2 : 0;
             float l[MOST], e[MOST], l2[REF ? MOST : 1];
             Stats<REF> x;
 #pragma unroll
@@ -885,18 +885,21 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
     // as many columns as a row can span in aligned chunks
     const bool aligned = ((uintptr_t)p.logits | (uintptr_t)(p.outer_stride * SIZE) | (uintptr_t)(p.inner_stride * SIZE)) % 16 == 0;
     const long long padded = p.columns + (aligned ? 0 : N - 1);
-    // A lane per row, where its registers leave enough waves.  Over 64 M columns in all, against the
-    // groups: 16-bit 17 columns 95 : 190 us, 24 70 : 122, 32 68 : 96, 33 127 : 152, 48 112 : 87; float32 16 107 : 171, 24 140 : 143, 32
-    // 276 : 127; float32 with a reference 16 160 : 203, 24 252 : 168.
-    const bool lane_per_row = SIZE == 2 ? p.columns <= 32 : p.columns <= (REF ? 16 : 24);
+    // A lane per row, where its registers leave enough waves.  Over 64 M columns in all, against the groups: 16-bit 17 columns 81 : 190 us, 24 58 : 122,
+    // 32 60 : 96; float32 16 107 : 171, 24 110 : 143, 31 109 : 189, 32 107 : 127; float32 with a reference 16 160 : 203, 24 156 : 168, but 25 311 : 204.
+    const bool lane_per_row = SIZE == 2 ? p.columns <= 32 : p.columns <= (SIZE == 4 && REF ? 24 : 32);
     if (lane_per_row) {
         auto lds = [&](int tile) { return (size_t)tile * (BLOCK / WAVE) * (REF ? 2 : 1); };
         if (p.columns <= 8) short_rows<E, 8, REF, Op><<<short_grid(CUS * short_residents<E, 8, REF>()), BLOCK, lds(short_tile<E, 8>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         else if (SIZE == 4 && p.columns == 16)
             short_rows<E, 16, REF, Op, SIZE == 4><<<short_grid(CUS * short_residents<E, 16, REF, SIZE == 4>()), BLOCK, lds(short_tile<E, 16>(16)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<short_grid(CUS * short_residents<E, 16, REF>()), BLOCK, lds(short_tile<E, 16>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if constexpr (SIZE == 2 || !REF)
-            short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds(short_tile<E, 32>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if (p.columns <= 24) short_rows<E, 24, REF, Op><<<short_grid(CUS * short_residents<E, 24, REF>()), BLOCK, lds(short_tile<E, 24>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if constexpr (SIZE == 2 || !REF) {
+            if (SIZE == 4 && p.columns == 32)
+                short_rows<E, 32, REF, Op, SIZE == 4><<<short_grid(CUS * short_residents<E, 32, REF, SIZE == 4>()), BLOCK, lds(short_tile<E, 32>(32)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+            else short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds(short_tile<E, 32>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        }
     } else if (padded <= 4 * 1 * N) {
         group_rows<E, 4, 1, REF, Op><<<grid(BLOCK / 4, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (padded <= 4 * 2 * N) {

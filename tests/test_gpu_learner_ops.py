@@ -403,6 +403,7 @@ LOGITS = [
     (5, 4099, "f32", "plain"), (300, 4096, "bf16", "plain"), (2, 32001, "bf16", "plain"), (1, 131072, "f16", "plain"), (3, 50021, "bf16", "pitch"), (1, 100003, "f32", "plain"), (6, 20000, "f32", "window"),
     (129, 16, "f32", "pitch"), (514, 16, "f32", "window"), (1000, 16, "f32", "plain"), (70, 17, "bf16", "plain"), (130, 31, "f16", "window"), (66, 24, "f32", "plain"), (200, 9, "bf16", "pitch"),
     (66, 8, "f16", "plain"), (129, 32, "bf16", "plain"),
+    (321, 32, "f32", "plain"), (66, 32, "f32", "window"), (65, 32, "f32", "pitch"), (193, 25, "f32", "plain"), (70, 31, "f32", "pitch"), (500, 23, "f32", "plain"), (259, 20, "f16", "plain"),
 ]
 
 
