@@ -21,6 +21,7 @@
 #include "learner.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace pgamd {
 namespace learner {
@@ -541,8 +542,9 @@ struct Place {
 };
 
 // Rows that fit the registers of a group inside of a wave: the next rows are on their way while these are worked on.
-// Loss and gradient of 64 M bf16 logits at 64, 512, 1024, 2000 columns: 68, 55, 55, 57 us (4.2 to 4.9 TB/s), with a reference 91, 81, 81, 87; at 65 and 300
-// columns, which leave two fifths of the lanes without any, 115 and 98.
+// Loss and gradient of 64 M bf16 logits at 64, 512, 1024, 2000 columns: 68, 55, 55, 57 us (4.2 to 4.9 TB/s), with a reference 91, 81, 81, 87.  Three, four
+// or five chunks a lane leave at most a quarter of the lanes without columns: at 127, 255, 300, 511, 2047 columns 85, 78, 66, 73, 68 us; with four alone, and
+// so up to half of them without, 127, 123, 97, 121, 106.
 template <class E, int G, int CH, bool REF, class Op>
 __global__ __launch_bounds__(BLOCK) void group_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
@@ -873,6 +875,9 @@ bool rows_ok(const procgen_amd_rows *p) {
     return p && known_dtype(p->dtype) && p->rows >= 0 && p->rows <= 0x7fffff00ll && p->columns >= 1 && p->columns <= 0x7ffffff0ll - (1 << 18) && p->inner >= 1;
 }
 
+template <int I>
+using Const = std::integral_constant<int, I>;
+
 // one kernel over all rows; returns the blocks it was launched with (the partial sums), or -1 - error
 template <class E, bool REF, class Op>
 int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long long ref_outer, long long ref_inner, double *partial, hipStream_t stream) {
@@ -888,6 +893,13 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
     // A lane per row, where its registers leave enough waves.  Over 64 M columns in all, against the groups: 16-bit 17 columns 81 : 190 us, 24 58 : 122,
     // 32 60 : 96; float32 16 107 : 171, 24 110 : 143, 31 109 : 189, 32 107 : 127; float32 with a reference 16 160 : 203, 24 156 : 168, but 25 311 : 204.
     const bool lane_per_row = SIZE == 2 ? p.columns <= 32 : p.columns <= (SIZE == 4 && REF ? 24 : 32);
+    auto group = [&](auto lanes, auto chunks) {  // whether a row fits, and if so the launch
+        constexpr int G = decltype(lanes)::value, CH = decltype(chunks)::value;
+        if (padded > G * CH * N) return false;
+        group_rows<E, G, CH, REF, Op><<<grid(BLOCK / G, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        return true;
+    };
+    auto groups = [&](auto lanes) { return group(lanes, Const<3>()) || group(lanes, Const<4>()) || group(lanes, Const<5>()); };
     if (lane_per_row) {
         auto lds = [&](int tile) { return (size_t)tile * (BLOCK / WAVE) * (REF ? 2 : 1); };
         if (p.columns <= 8) short_rows<E, 8, REF, Op><<<short_grid(CUS * short_residents<E, 8, REF>()), BLOCK, lds(short_tile<E, 8>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
@@ -900,22 +912,8 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
                 short_rows<E, 32, REF, Op, SIZE == 4><<<short_grid(CUS * short_residents<E, 32, REF, SIZE == 4>()), BLOCK, lds(short_tile<E, 32>(32)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
             else short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds(short_tile<E, 32>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         }
-    } else if (padded <= 4 * 1 * N) {
-        group_rows<E, 4, 1, REF, Op><<<grid(BLOCK / 4, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (padded <= 4 * 2 * N) {
-        group_rows<E, 4, 2, REF, Op><<<grid(BLOCK / 4, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (padded <= 4 * 4 * N) {
-        group_rows<E, 4, 4, REF, Op><<<grid(BLOCK / 4, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (padded <= 8 * 4 * N) {
-        group_rows<E, 8, 4, REF, Op><<<grid(BLOCK / 8, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (padded <= 16 * 4 * N) {
-        group_rows<E, 16, 4, REF, Op><<<grid(BLOCK / 16, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (padded <= 32 * 4 * N) {
-        group_rows<E, 32, 4, REF, Op><<<grid(BLOCK / 32, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (padded <= 64 * 4 * N) {
-        group_rows<E, 64, 4, REF, Op><<<grid(BLOCK / 64, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (padded <= 64 * 8 * N) {
-        group_rows<E, 64, 8, REF, Op><<<grid(BLOCK / 64, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (group(Const<4>(), Const<1>()) || group(Const<4>(), Const<2>()) || groups(Const<4>()) || groups(Const<8>()) || groups(Const<16>()) || groups(Const<32>()) ||
+               groups(Const<64>()) || group(Const<64>(), Const<8>())) {
     } else if (p.columns <= 256 * 2 * N || (p.rows >= 2 * CUS && !(REF && p.d_logits))) {
         long_rows<E, 256, 2, REF, Op><<<grid(1, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.rows >= 2 * CUS) {  // 2048 x 50021 bf16 with a reference: 154 us, against 173 with 256 lanes and two chunks, 179 with 1024
