@@ -96,6 +96,11 @@ struct Stats {
             u += product(e, t - q);
         }
     }
+    // lanes that hold no wave's sums take the first one's
+    __device__ void from_first() {
+        m = __shfl(m, 0, WAVE), s = __shfl(s, 0, WAVE), w = __shfl(w, 0, WAVE);
+        if (REF) m2 = __shfl(m2, 0, WAVE), s2 = __shfl(s2, 0, WAVE), u = __shfl(u, 0, WAVE);
+    }
     // over `width` neighbouring lanes, all of which get the same bits
     template <int WIDTH>
     __device__ void join() {
@@ -541,15 +546,18 @@ struct Place {
     __device__ int chunk_of(int column) const { return (column + ahead) / N; }
 };
 
-// Rows that fit the registers of a group inside of a wave: the next rows are on their way while these are worked on.
+// Rows that fit the registers of a group, of lanes inside of a wave or of two or four waves: the next rows are on their way while these are worked on.
 // Loss and gradient of 64 M bf16 logits at 64, 512, 1024, 2000 columns: 68, 55, 55, 57 us (4.2 to 4.9 TB/s), with a reference 91, 81, 81, 87.  Three, four
 // or five chunks a lane leave at most a quarter of the lanes without columns: at 127, 255, 300, 511, 2047 columns 85, 78, 66, 73, 68 us; with four alone, and
-// so up to half of them without, 127, 123, 97, 121, 106.
+// so up to half of them without, 127, 123, 97, 121, 106.  A group of two or four waves holds 4100, 5000, 8200 columns: 69, 56, 66 us, in batches of a block 113,
+// 90, 77; with a reference 107, 87, 104, in batches 232, 188, 148.
 template <class E, int G, int CH, bool REF, class Op>
 __global__ __launch_bounds__(BLOCK) void group_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
-    constexpr int N = Chunk<E>::N, PER = N / 4, PER_BLOCK = BLOCK / G;
+    constexpr int N = Chunk<E>::N, PER = N / 4, PER_BLOCK = BLOCK / G, WAVES = G / WAVE, LANES = WAVES ? WAVE : G;
     const int g = threadIdx.x % G, columns = (int)p.columns;
+    __shared__ float wave_stats[2][WAVES > 1 ? BLOCK / WAVE : 1][6];
+    int odd = 0;
     if (op.done()) return;
     op.begin(p);
     Sums sums;
@@ -603,7 +611,7 @@ __global__ __launch_bounds__(BLOCK) void group_rows(procgen_amd_rows p, Op op, c
                 to = fmaxf(to, l[i][k]);
                 if (REF) to2 = fmaxf(to2, l2[i][k]);
             }
-        for (int d = G / 2; d > 0; d >>= 1) {
+        for (int d = LANES / 2; d > 0; d >>= 1) {
             to = fmaxf(to, __shfl_xor(to, d, WAVE));
             if (REF) to2 = fmaxf(to2, __shfl_xor(to2, d, WAVE));
         }
@@ -616,13 +624,23 @@ __global__ __launch_bounds__(BLOCK) void group_rows(procgen_amd_rows p, Op op, c
 #pragma unroll
             for (int k = 0; k < N; k++) x.add(b, b2, l[i][k], REF ? l2[i][k] : 0.f);
         }
-        for (int d = G / 2; d > 0; d >>= 1) {
+        for (int d = LANES / 2; d > 0; d >>= 1) {
             x.s += __shfl_xor(x.s, d, WAVE);
             x.w += __shfl_xor(x.w, d, WAVE);
             if (REF) {
                 x.s2 += __shfl_xor(x.s2, d, WAVE);
                 x.u += __shfl_xor(x.u, d, WAVE);
             }
+        }
+        if constexpr (WAVES > 1) {
+            const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+            if (lane == 0) x.put(wave_stats[odd][wave]);
+            __syncthreads();
+            x = Stats<REF>();
+            if (lane < WAVES) x.get(wave_stats[odd][wave / WAVES * WAVES + lane]);
+            x.template join<WAVES>();
+            x.from_first();
+            odd ^= 1;
         }
         Coef c;
         const bool some = mine && op.wanted(in) && op.template finish<REF>(here, in, x, a >= 0, taken, g == 0, c, sums);
@@ -741,9 +759,7 @@ __global__ __launch_bounds__(G, 4) void long_rows(procgen_amd_rows p, Op op, con
             x = Stats<REF>();
             if (lane < G / WAVE) x.get(wave_stats[odd][lane]);
             x.template join<G / WAVE>();
-            // lanes beyond the first G / WAVE hold no wave's sums: they take the first one's
-            x.m = __shfl(x.m, 0, WAVE), x.s = __shfl(x.s, 0, WAVE), x.w = __shfl(x.w, 0, WAVE);
-            if (REF) x.m2 = __shfl(x.m2, 0, WAVE), x.s2 = __shfl(x.s2, 0, WAVE), x.u = __shfl(x.u, 0, WAVE);
+            x.from_first();
             odd ^= 1;
             if (Op::GRADIENT && out && batches > 1 + KEPT) load(batches - 2 - KEPT);  // the first batch that has to be read again
             some = op.template finish<REF>(r, in, x, known, taken, g == 0, c, sums);
@@ -893,6 +909,8 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
     // A lane per row, where its registers leave enough waves.  Over 64 M columns in all, against the groups: 16-bit 17 columns 81 : 190 us, 24 58 : 122,
     // 32 60 : 96; float32 16 107 : 171, 24 110 : 143, 31 109 : 189, 32 107 : 127; float32 with a reference 16 160 : 203, 24 156 : 168, but 25 311 : 204.
     const bool lane_per_row = SIZE == 2 ? p.columns <= 32 : p.columns <= (SIZE == 4 && REF ? 24 : 32);
+    // with a gradient, float32 goes in chunks of as many values as 16 bits do: loss of 16000 columns 133 -> 122 us, with a reference 153 -> 119
+    constexpr int MORE = Op::GRADIENT && SIZE == 4 ? 2 : 1;
     auto group = [&](auto lanes, auto chunks) {  // whether a row fits, and if so the launch
         constexpr int G = decltype(lanes)::value, CH = decltype(chunks)::value;
         if (padded > G * CH * N) return false;
@@ -913,11 +931,11 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
             else short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds(short_tile<E, 32>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         }
     } else if (group(Const<4>(), Const<1>()) || group(Const<4>(), Const<2>()) || groups(Const<4>()) || groups(Const<8>()) || groups(Const<16>()) || groups(Const<32>()) ||
-               groups(Const<64>()) || group(Const<64>(), Const<8>())) {
+               groups(Const<64>()) || group(Const<128>(), Const<3>()) || group(Const<64>(), Const<8>()) || (p.rows >= 2 * CUS && (group(Const<128>(), Const<5>()) || groups(Const<256>())))) {
     } else if (p.columns <= 256 * 2 * N || (p.rows >= 2 * CUS && !(REF && p.d_logits))) {
-        long_rows<E, 256, 2, REF, Op><<<grid(1, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        long_rows<E, 256, 2 * MORE, REF, Op><<<grid(1, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else if (p.rows >= 2 * CUS) {  // 2048 x 50021 bf16 with a reference: 154 us, against 173 with 256 lanes and two chunks, 179 with 1024
-        long_rows<E, 512, 1, REF, Op><<<grid(1, CUS * 2), 512, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        long_rows<E, 512, MORE, REF, Op><<<grid(1, CUS * 2), 512, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else {  // too few rows to fill the card: more lanes for each
         long_rows<E, 1024, 2, REF, Op><<<grid(1, CUS), 1024, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     }

@@ -654,7 +654,9 @@ def test_policy_loss(B, A, dtype, layout, ref):
     assert torch.equal(again.loss, out.loss.detach()) and torch.equal(again.stats, out.stats)
 
 
-@pytest.mark.parametrize("B,A,dtype,ref", [(513, 20011, "f32", True), (515, 40003, "bf16", True), (600, 5000, "f16", True), (520, 33333, "bf16", False), (1030, 2500, "f32", False)])
+@pytest.mark.parametrize("B,A,dtype,ref", [(513, 20011, "f32", True), (515, 40003, "bf16", True), (600, 5000, "f16", True), (520, 33333, "bf16", False), (1030, 2500, "f32", False),
+                                           (520, 6000, "bf16", False), (515, 8101, "bf16", True), (513, 9999, "f16", False), (513, 2900, "f32", True), (600, 4090, "f32", False),
+                                           (530, 5100, "f32", True), (515, 9001, "f32", False)])
 def test_policy_loss_of_many_long_rows(B, A, dtype, ref):
     """rows of several batches, enough of them to fill the card; the 64-bit loss on the GPU for its time"""
     g = torch.Generator(device="cuda").manual_seed(A)
