@@ -334,7 +334,7 @@ struct Chunk {
     __device__ void forget() { asm volatile("" : "+v"(w)); }
 };
 
-// ---- up to 32 columns: a lane per row -------------------------------------------------------------------------------------------------------------
+// ---- up to 32 columns, or 63: a lane per row -------------------------------------------------------------------------------------------------------------
 
 // 64 rows on their way from memory to LDS (`rows` of them exist).  Contiguous rows go 16 bytes a lane and, where they are few registers, are fetched
 // while the 64 before them are worked on; others go element by element.
@@ -401,7 +401,7 @@ __host__ __device__ constexpr int short_tile(int columns) {
 // blocks of four waves that a compute unit holds: by registers (three, or four with a reference, for each of MOST columns) and by LDS
 template <class E, int MOST, bool REF, bool TURN = false>
 constexpr int short_residents() {
-    return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? (TURN ? 2 : 3) : sizeof(typename E::T) == 4 ? 4 : 5) : MOST <= 24 ? (REF ? 2 : sizeof(typename E::T) == 4 ? 3 : 4) : REF || sizeof(typename E::T) == 4 ? 2 : 3;
+    return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? (TURN ? 2 : 3) : sizeof(typename E::T) == 4 ? 4 : 5) : MOST <= 24 ? (REF ? 2 : sizeof(typename E::T) == 4 ? 3 : 4) : MOST > 32 || REF || sizeof(typename E::T) == 4 ? 2 : 3;
 }
 
 // Loss and gradient of 4 194 304 x 15 bf16: 67 to 76 us, 306 MB, 4.0 to 4.6 TB/s; without fetching ahead 98, with the register limit of six blocks (and
@@ -451,8 +451,9 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) voi
         if (wanted) {
             // the columns that a row has not are -inf; l and l2 become t and q
             // reads what a row has not and drops it, which keeps the reads together; where registers are short it is not read (15 bf16 67 : 76 us)
+            constexpr bool AGAIN = MOST > 48 || (REF && MOST > 24 && sizeof(T) == 4);  // exponentials are taken again for the gradient: registers for all of them would be spilled
             constexpr bool GUARD = Op::HEAVY && MOST == 16 && !REF && sizeof(T) == 2;
-            constexpr int surely = TURN ? MOST : MOST > 16 ? MOST - 8 : MOST > 8 ? MOST / 2 : 0;
+            constexpr int surely = TURN ? MOST : MOST > 32 ? MOST - 16 : MOST > 16 ? MOST - 8 : MOST > 8 ? MOST / 2 : 0;
             float l[MOST], e[MOST], l2[REF ? MOST : 1];
             Stats<REF> x;
 #pragma unroll
@@ -485,6 +486,10 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) voi
             if (Op::GRADIENT && some && p.d_logits) {
 #pragma unroll
                 for (int j = 0; j < MOST; j++) {
+                    if (AGAIN) {
+                        asm volatile("" : "+v"(l[j]));
+                        e[j] = exp2_of(l[j]);
+                    }
                     float f = fmaf(c.cd, l[j], c.c0);
                     if (REF) f = fmaf(c.cq, l2[j], f);
                     if (j <= surely || j < columns) row[j ^ turn] = (T)product(e[j], f);
@@ -906,9 +911,10 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
     // as many columns as a row can span in aligned chunks
     const bool aligned = ((uintptr_t)p.logits | (uintptr_t)(p.outer_stride * SIZE) | (uintptr_t)(p.inner_stride * SIZE)) % 16 == 0;
     const long long padded = p.columns + (aligned ? 0 : N - 1);
-    // A lane per row, where its registers leave enough waves.  Over 64 M columns in all, against the groups: 16-bit 17 columns 81 : 190 us, 24 58 : 122,
-    // 32 60 : 96; float32 16 107 : 171, 24 110 : 143, 31 109 : 189, 32 107 : 127; float32 with a reference 16 160 : 203, 24 156 : 168, but 25 311 : 204.
-    const bool lane_per_row = SIZE == 2 ? p.columns <= 32 : p.columns <= (SIZE == 4 && REF ? 24 : 32);
+    // A lane per row, where its registers leave enough waves.  Over 64 M columns in all, against the groups: 16-bit 17 columns 81 : 190 us, 32 60 : 96,
+    // 33 83 : 160, 48 62 : 86, 63 68 : 113, but 64 152 : 68, with a reference 32 98 : 150, but 33 291 : 225; float32 16 107 : 171, 24 110 : 143, 31 109 : 189,
+    // 32 107 : 127, with a reference 16 160 : 203, 24 156 : 168, 25 169 : 203, 31 149 : 201, but 32 314 : 141.
+    const bool lane_per_row = p.columns <= (SIZE == 2 ? (REF ? 32 : 63) : REF ? 31 : 32);
     // with a gradient, float32 goes in chunks of as many values as 16 bits do: loss of 16000 columns 133 -> 122 us, with a reference 153 -> 119
     constexpr int MORE = Op::GRADIENT && SIZE == 4 ? 2 : 1;
     auto group = [&](auto lanes, auto chunks) {  // whether a row fits, and if so the launch
@@ -925,10 +931,13 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
             short_rows<E, 16, REF, Op, SIZE == 4><<<short_grid(CUS * short_residents<E, 16, REF, SIZE == 4>()), BLOCK, lds(short_tile<E, 16>(16)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<short_grid(CUS * short_residents<E, 16, REF>()), BLOCK, lds(short_tile<E, 16>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         else if (p.columns <= 24) short_rows<E, 24, REF, Op><<<short_grid(CUS * short_residents<E, 24, REF>()), BLOCK, lds(short_tile<E, 24>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if constexpr (SIZE == 2 || !REF) {
-            if (SIZE == 4 && p.columns == 32)
-                short_rows<E, 32, REF, Op, SIZE == 4><<<short_grid(CUS * short_residents<E, 32, REF, SIZE == 4>()), BLOCK, lds(short_tile<E, 32>(32)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-            else short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds(short_tile<E, 32>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if (SIZE == 4 && !REF && p.columns == 32) {
+            if constexpr (SIZE == 4 && !REF)
+                short_rows<E, 32, REF, Op, true><<<short_grid(CUS * short_residents<E, 32, REF, true>()), BLOCK, lds(short_tile<E, 32>(32)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        } else if (p.columns <= 32) short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds(short_tile<E, 32>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else if constexpr (SIZE == 2 && !REF) {
+            if (p.columns <= 48) short_rows<E, 48, REF, Op><<<short_grid(CUS * short_residents<E, 48, REF>()), BLOCK, lds(short_tile<E, 48>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+            else short_rows<E, 64, REF, Op><<<short_grid(CUS * short_residents<E, 64, REF>()), BLOCK, lds(short_tile<E, 64>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         }
     } else if (group(Const<4>(), Const<1>()) || group(Const<4>(), Const<2>()) || groups(Const<4>()) || groups(Const<8>()) || groups(Const<16>()) || groups(Const<32>()) ||
                groups(Const<64>()) || group(Const<128>(), Const<3>()) || group(Const<64>(), Const<8>()) || (p.rows >= 2 * CUS && (group(Const<128>(), Const<5>()) || groups(Const<256>())))) {

@@ -404,6 +404,7 @@ LOGITS = [
     (129, 16, "f32", "pitch"), (514, 16, "f32", "window"), (1000, 16, "f32", "plain"), (70, 17, "bf16", "plain"), (130, 31, "f16", "window"), (66, 24, "f32", "plain"), (200, 9, "bf16", "pitch"),
     (66, 8, "f16", "plain"), (129, 32, "bf16", "plain"),
     (321, 32, "f32", "plain"), (66, 32, "f32", "window"), (65, 32, "f32", "pitch"), (193, 25, "f32", "plain"), (70, 31, "f32", "pitch"), (500, 23, "f32", "plain"), (259, 20, "f16", "plain"),
+    (321, 33, "bf16", "plain"), (130, 48, "f16", "window"), (193, 49, "bf16", "pitch"), (259, 63, "f16", "plain"), (129, 64, "bf16", "pitch"), (129, 55, "bf16", "plain"),
     (33, 90, "bf16", "plain"), (20, 150, "f16", "pitch"), (18, 190, "bf16", "window"), (21, 300, "bf16", "plain"), (17, 380, "f16", "plain"), (9, 600, "bf16", "pitch"), (9, 700, "f16", "plain"),
     (5, 1200, "bf16", "plain"), (6, 1500, "bf16", "window"), (5, 2047, "bf16", "plain"), (50, 45, "f32", "plain"), (40, 70, "f32", "window"), (30, 95, "f32", "pitch"), (19, 155, "f32", "plain"),
     (17, 190, "f32", "plain"), (12, 310, "f32", "window"), (9, 380, "f32", "plain"), (7, 601, "f32", "pitch"), (5, 767, "f32", "plain"), (5, 1277, "f32", "plain"), (3, 2040, "f32", "plain"),
