@@ -21,7 +21,7 @@ namespace pgamd {
 namespace learner {
 namespace {
 
-constexpr int W1 = 4, WS = 8;     // waves of a block: where there are chains enough, and where a window is cut into segments
+constexpr int W1 = 4, WS = 8;     // waves of a block: where there are chains enough, and where there are few or a window is cut into segments
 constexpr int KF = 8, KB = 4;     // steps of a wave in a tile: forwards (and advantages), backwards
 constexpr int UNIT = KF * WS;     // a segment is a whole number of these: of the tiles of either direction
 constexpr int CHECK = KB * W1;    // steps from one checkpoint to the next: a tile of the backward pass, or half of one
@@ -578,17 +578,21 @@ __global__ __launch_bounds__(WAVES *WAVE) void advantages(procgen_amd_advantage 
 bool shape_ok(int dtype, int T, int N, int D) { return known_dtype(dtype) && T >= 0 && T <= 0x7fffff00 && N >= 0 && D >= 0 && (long long)N * D <= 0x7fffff00ll; }
 
 constexpr int FULL = 512;  // blocks that fill the card: two on each of the 256 compute units
+// Blocks from which on a window stays whole.  256 blocks of eight waves read the inputs once in less time than 512 blocks of segments read them twice: 2048
+// x 32 x 512 float32 forward 78 : 122 us, backward 153 : 186; at 192 blocks 4000 x 24 x 512 bf16 does not, 276 : 232 backwards.  Advantages, one kernel
+// with little to keep, go on to 128 blocks of sixteen waves: 1000 x 10000 float32 36 : 55.
+constexpr int ENOUGH = FULL / 2, ENOUGH_ADVANTAGES = FULL / 4, WA = 16;
 int units_of(int T) { return (T + UNIT - 1) / UNIT; }
 // How many segments a window of so many chains is cut into: by its sizes alone, so that the workspace does not depend on strides.  Not more than 256, since
 // every segment begins with the maps of all before it (100 000 x 16 float32: forward and backward 125 us with 128, 87 with 256, 85 with 512).
-int segments_of(int T, long long chains) {
+int segments_of(int T, long long chains, int enough = ENOUGH) {
     const long long blocks = (chains + WAVE - 1) / WAVE;
-    if (blocks >= FULL) return 1;
+    if (blocks >= enough) return 1;
     return (int)std::max(1ll, std::min({(FULL + blocks - 1) / blocks, units_of(T) / 2ll, 256ll}));
 }
-Segments segments(int T, long long chains, void *workspace) {
+Segments segments(int T, long long chains, void *workspace, int enough = ENOUGH) {
     Segments g;
-    const int wanted = segments_of(T, chains);
+    const int wanted = segments_of(T, chains, enough);
     g.tiles = (units_of(T) + wanted - 1) / wanted;
     g.count = (units_of(T) + g.tiles - 1) / g.tiles;
     g.maps = (float *)workspace;
@@ -615,16 +619,16 @@ int vec_for(const procgen_amd_recurrence *a, bool backward) {
         if (a->D >= vec && (long long)a->N * ((a->D + vec - 1) / vec) >= FULL * (long long)WAVE) return vec;
     return 1;
 }
-// fn(VEC, WAVES): a window in segments has too few chains for more than one a lane
+// fn(VEC, WAVES): a window in segments has too few chains for more than one a lane.  With one a lane eight waves: 1024 x 64 x 512 bf16 forward 53 us,
+// backward 109, with four 66 and 126
 template <class Fn>
 int by_shape(const Segments &g, int vec, Fn fn) {
     typedef std::integral_constant<int, 1> One;
-    if (g.count > 1) return fn(One(), std::integral_constant<int, WS>());
     const std::integral_constant<int, W1> waves;
-    switch (vec) {
+    switch (g.count > 1 ? 1 : vec) {
         case 4: return fn(std::integral_constant<int, 4>(), waves);
         case 2: return fn(std::integral_constant<int, 2>(), waves);
-        default: return fn(One(), waves);
+        default: return fn(One(), std::integral_constant<int, WS>());
     }
 }
 // fn(VEC) for a few steps: up to 16 bytes a lane, where that leaves a block for every compute unit.  65 536 x 256 bf16, one step: forward 31 us
@@ -673,7 +677,7 @@ LIBENV_API int procgen_amd_recurrence_forward(const struct procgen_amd_recurrenc
         return by_shape(g, vec_for(a, false), [&](auto vec, auto waves) {
             constexpr int VEC = decltype(vec)::value, WAVES = decltype(waves)::value;
             const dim3 grid(chain_blocks(a, VEC), g.count), block(WAVE, std::min(WAVES, (a->T + KF - 1) / KF));
-            if constexpr (WAVES == WS) {
+            if (WAVES == WS && g.count > 1) {
                 recurrence_segments<E, VEC, WAVES, false><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
                 if (int err = launched()) return err;
             }
@@ -701,7 +705,7 @@ LIBENV_API int procgen_amd_recurrence_backward(const struct procgen_amd_recurren
         return by_shape(g, vec_for(a, true), [&](auto vec, auto waves) {
             constexpr int VEC = std::min(2, decltype(vec)::value), WAVES = decltype(waves)::value;
             const dim3 grid(chain_blocks(a, VEC), g.count), block(WAVE, std::min(WAVES, (a->T + KB - 1) / KB));
-            if constexpr (WAVES == WS) {
+            if (WAVES == WS && g.count > 1) {
                 recurrence_segments<E, VEC, WAVES, true><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
                 if (int err = launched()) return err;
             }
@@ -714,7 +718,7 @@ LIBENV_API int procgen_amd_recurrence_backward(const struct procgen_amd_recurren
 LIBENV_API int procgen_amd_advantages(const struct procgen_amd_advantage *a, int device, void *stream) {
     if (!a || !shape_ok(a->dtype, a->T, a->N, 1)) return -1;
     if (a->T == 0 || a->N == 0) return 0;
-    const Segments g = segments(a->T, a->N, a->workspace);
+    const Segments g = segments(a->T, a->N, a->workspace, ENOUGH_ADVANTAGES);
     if (!a->rew || !a->values || !a->first || (g.count > 1 && !a->workspace)) return -1;
     OnDevice on(device);
     if (on.err != hipSuccess) return (int)on.err;
@@ -726,6 +730,8 @@ LIBENV_API int procgen_amd_advantages(const struct procgen_amd_advantage *a, int
             advantage_segments<E, WS><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
             if (int err = launched()) return err;
             advantages<E, WS><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
+        } else if (blocks < FULL) {  // 256 x 16384 float32: 15 us, with four waves 21
+            advantages<E, WA><<<blocks, dim3(WAVE, std::min(WA, (a->T + KF - 1) / KF)), 0, (hipStream_t)stream>>>(*a, g);
         } else {
             advantages<E, W1><<<blocks, dim3(WAVE, std::min(W1, (a->T + KF - 1) / KF)), 0, (hipStream_t)stream>>>(*a, g);
         }

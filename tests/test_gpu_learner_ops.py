@@ -119,7 +119,7 @@ RECURRENCES = [
     (5000, 2, 3, "bf16", True, True, "ntd"), (31, 1, 2000, "f32", True, False, "slice"), (40, 300, 1, "bf16", True, True, "strided"), (7, 129, 65, "f16", True, True, "tnd"),
     (12345, 1, 1, "f32", True, True, "tnd"), (3, 700, 100, "bf16", True, True, "tnd"), (4, 300, 257, "f16", True, False, "ntd"), (1, 2100, 133, "f32", True, True, "slice"),
     (1, 9000, 61, "bf16", True, True, "tnd"), (4, 40, 30, "f32", False, True, "strided"), (5, 900, 150, "bf16", True, True, "tnd"), (100, 700, 101, "bf16", True, True, "ntd"),
-    (20000, 1, 70, "bf16", True, True, "slice"),
+    (20000, 1, 70, "bf16", True, True, "slice"), (200, 33, 500, "f32", True, True, "tnd"), (150, 64, 257, "bf16", True, True, "ntd"), (97, 5, 3301, "f16", False, True, "slice"),
 ]
 
 
@@ -321,6 +321,7 @@ def advantages_64(rew, values, first, gamma, lam):
     (1, 1, "f32", 0.999, 0.95, "tn"), (2, 65, "bf16", 0.99, 0.9, "tn"), (16, 64, "f32", 0.999, 0.95, "tn"), (31, 1000, "f16", 0.999, 0.95, "nt"), (64, 3, "f32", 1.0, 1.0, "tn"),
     (65, 130, "bf16", 0.9, 0.0, "nt"), (257, 512, "f32", 0.999, 0.95, "slice"), (1000, 7, "f16", 0.0, 0.95, "tn"), (4097, 2, "f32", 0.999, 0.95, "nt"), (10007, 1, "bf16", 1.0, 1.0, "tn"),
     (5, 70000, "f32", 0.999, 0.95, "tn"),
+    (300, 8195, "f32", 0.999, 0.95, "tn"), (70, 20001, "bf16", 0.999, 0.95, "nt"), (7, 9000, "f32", 0.999, 0.95, "tn"),
 ])
 def test_advantages(T, N, dtype, gamma, lam, layout):
     g = gen(T + N)
