@@ -15,7 +15,9 @@
 // Bound by memory: a column costs 12 operations for 4 to 8 bytes, 23 for 6 to 12 with a reference (a 1 GiB copy reaches 5.1 TB/s on the same card).  By
 // the number of columns:
 //   up to 32      a wave takes 64 rows through LDS, a lane per row: no reduction over lanes, coalesced although a row is no multiple of anything
-//   up to 4096    a group of 4 to 64 lanes per row, the whole row in their registers between the sums and the gradient (2048 in float32)
+//                 (16 bits without a reference up to 63)
+//   up to 10240   a group of 4 to 256 lanes per row, the whole row in their registers between the sums and the gradient (5120 in float32; 4096 and 2048
+//                 where the rows are too few to fill the card one a block)
 //   more          a block per row, in batches; the gradient goes through them backwards: the last is still in registers, those before it in LDS, and
 //                 only what is left is read from memory again
 #include "learner.h"

@@ -4,7 +4,7 @@
 // A step is the affine map x -> a x + b, or x -> b where an episode begins (`cut`: a select, so that nothing of the other episode, NaN or infinite,
 // passes).  Maps compose to maps of the same kind, so a chain is cut into pieces that are summed up at the same time and joined afterwards:
 //   wave     8 consecutive steps in registers (4 backwards), their composition (A, B, cut) by an FMA each
-//   block    four waves (eight where a window is in segments) take consecutive pieces of a tile; the pieces' maps meet in LDS, every wave runs its value
+//   block    four waves (eight or sixteen where chains are few) take consecutive pieces of a tile; the pieces' maps meet in LDS, every wave runs its value
 //            at the tile's start through the pieces before its own, and does its steps again from there: one read and one write of the data, one barrier
 //            a tile
 //   segment  where there are too few chains to fill the card, the window is cut into segments for blocks of their own: a first kernel composes each
