@@ -338,8 +338,10 @@ struct Chunk {
 
 // ---- up to 32 columns, or 63: a lane per row -------------------------------------------------------------------------------------------------------------
 
-// 64 rows on their way from memory to LDS (`rows` of them exist).  Contiguous rows go 16 bytes a lane and, where they are few registers, are fetched
-// while the 64 before them are worked on; others go element by element.
+// 64 rows on their way from memory to LDS (`rows` of them exist), fetched while the 64 before them are worked on.  Contiguous rows are one array of 16
+// bytes a lane.  Rows apart from each other (APART, kernels of their own: one for both would spill registers) are cut into such pieces each, the last moved
+// back to end with its row; rows under 16 bytes go element by element.  Loss and gradient of 2 097 152 x 15
+// out of rows of 16: bf16 51 us (element by element 73), with a reference 68 (171), float32 52 (105); of 31 out of 32 bf16 90 (214), float32 108 (367).
 //
 // Rows of 16 or 32 float32 are 64 or 128 bytes: lanes that all read one column of theirs would meet in four or two of the 64 banks.  With TURN a row's
 // chunks are swapped by the row's place, and 16 lanes that read a chunk each go over every bank once.  Loss and gradient of 4 194 304 x 16 float32: 107
@@ -348,46 +350,55 @@ template <class E, int MOST, bool TURN>
 __device__ inline int place(int i) {  // in LDS, of element i of the 64 rows
     return TURN ? i ^ (i / MOST * MOST / 64 % (MOST / Chunk<E>::N) * Chunk<E>::N) : i;
 }
-template <class E, int MOST, bool TURN = false>
+template <class E, int MOST, bool TURN, bool APART>
 struct Tile {
     typedef typename E::T T;
     static constexpr int N = Chunk<E>::N, CHUNKS = MOST * (int)sizeof(T) / 16;  // 64 rows of MOST columns: so many 16 bytes a lane
-    static constexpr bool AHEAD = CHUNKS <= 8;
-    Bits c[AHEAD ? CHUNKS : 1];
-    __device__ void fetch(const procgen_amd_rows &p, const void *from, long long outer, long long r0, int rows, int lane) {
-        if (!AHEAD || p.inner != 1 || outer != p.columns) return;
-        const int n = rows * (int)p.columns;
-        const T *const src = (const T *)from + r0 * p.columns;
+    Chunk<E> c[CHUNKS];
+    struct Piece {  // of a row that is not followed by the next
+        int row, column;
+        __device__ Piece(int i, int lane, int columns) {
+            const uint32_t pieces = (columns + N - 1) / N, at = i * WAVE + lane;
+            row = at * (65536 / pieces + 1) >> 16;  // at / pieces: at < 512, pieces <= 8
+            column = min((int)(at - row * pieces) * N, columns - N);
+        }
+    };
+    __device__ void fetch(const procgen_amd_rows &p, const void *from, long long outer, long long inner, long long r0, int rows, int lane) {
+        const int columns = (int)p.columns, n = rows * columns;
+        const T *const src = (const T *)from + r0 * columns;
+        if (APART && columns < N) return;
 #pragma unroll
-        for (int i = 0; i < (AHEAD ? CHUNKS : 0); i++) {
-            const int at = (i * WAVE + lane) * N;
-            if (at + N <= n) __builtin_memcpy(&c[i], src + at, 16);
+        for (int i = 0; i < CHUNKS; i++) {
+            if constexpr (APART) {
+                const Piece q(i, lane, columns);
+                if (q.row < rows) c[i].load((const T *)from + row_offset(p, r0 + q.row, outer, inner) + q.column);
+            } else {
+                const int at = (i * WAVE + lane) * N;
+                if (at + N <= n) c[i].load(src + at);
+            }
         }
     }
     __device__ void put(T *lds, const procgen_amd_rows &p, const void *from, long long outer, long long inner, long long r0, int rows, int lane) const {
         const int columns = (int)p.columns, n = rows * columns;
-        if (p.inner == 1 && outer == columns) {
-            const T *const src = (const T *)from + r0 * columns;
-            if (AHEAD) {
-#pragma unroll
-                for (int i = 0; i < (AHEAD ? CHUNKS : 0); i++) {
-                    const int at = (i * WAVE + lane) * N;
-                    if (at + N <= n) *(Bits *)(lds + place<E, MOST, TURN>(at)) = c[i];
-                }
-            } else {
-                for (int at = lane * N; at + N <= n; at += WAVE * N) {
-                    Bits k;
-                    __builtin_memcpy(&k, src + at, 16);
-                    *(Bits *)(lds + place<E, MOST, TURN>(at)) = k;
-                }
-            }
-            if (n / N * N + lane < n) lds[place<E, MOST, TURN>(n / N * N + lane)] = src[n / N * N + lane];
-        } else {
+        if (APART && columns < N) {
             for (int i = lane; i < n; i += WAVE) {
                 const int r = i / columns;
                 lds[place<E, MOST, TURN>(i)] = ((const T *)from)[row_offset(p, r0 + r, outer, inner) + (i - r * columns)];
             }
+            return;
         }
+#pragma unroll
+        for (int i = 0; i < CHUNKS; i++) {
+            if constexpr (APART) {
+                const Piece q(i, lane, columns);
+                if (q.row < rows)
+                    for (int k = 0; k < N; k++) lds[place<E, MOST, TURN>(q.row * columns + q.column + k)] = c[i].piece(k);
+            } else {
+                const int at = (i * WAVE + lane) * N;
+                if (at + N <= n) *(Bits *)(lds + place<E, MOST, TURN>(at)) = c[i].w;
+            }
+        }
+        if (!APART && n / N * N + lane < n) lds[place<E, MOST, TURN>(n / N * N + lane)] = ((const T *)from)[r0 * columns + n / N * N + lane];
     }
 };
 __device__ inline void lds_settled() {  // a wave's own LDS is written and read in order; this holds the compiler to it
@@ -408,7 +419,7 @@ constexpr int short_residents() {
 
 // Loss and gradient of 4 194 304 x 15 bf16: 67 to 76 us, 306 MB, 4.0 to 4.6 TB/s; without fetching ahead 98, with the register limit of six blocks (and
 // spills) 93, of four 78.  What is left is the issue of instructions: some 380 vector and 230 scalar ones for 64 rows.
-template <class E, int MOST, bool REF, class Op, bool TURN = false>
+template <class E, int MOST, bool REF, class Op, bool TURN, bool APART>
 __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) void short_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -419,8 +430,8 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) voi
     op.begin(p);
     Sums sums;
     const long long step = (long long)gridDim.x * (BLOCK / WAVE) * WAVE;
-    Tile<E, MOST, TURN> next;
-    Tile<E, REF ? MOST : 8, REF && TURN> next2;
+    Tile<E, MOST, TURN, APART> next;
+    Tile<E, REF ? MOST : 8, REF && TURN, APART> next2;
     typename Op::In next_in;
     int next_a = -1;  // -1: not one of the columns
     auto fetch = [&](long long r0) {
@@ -429,8 +440,8 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) voi
         next_in = op.fetch(r);
         const long long a = action_of(p, r);
         next_a = a >= 0 && a < columns ? (int)a : -1;
-        next.fetch(p, p.logits, p.outer_stride, r0, rows, lane);
-        if (REF) next2.fetch(p, ref, ref_outer, r0, rows, lane);
+        next.fetch(p, p.logits, p.outer_stride, p.inner_stride, r0, rows, lane);
+        if (REF) next2.fetch(p, ref, ref_outer, ref_inner, r0, rows, lane);
     };
     long long r0 = ((long long)blockIdx.x * (BLOCK / WAVE) + wave) * WAVE;
     if (r0 < p.rows) fetch(r0);
@@ -926,20 +937,28 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
         return true;
     };
     auto groups = [&](auto lanes) { return group(lanes, Const<3>()) || group(lanes, Const<4>()) || group(lanes, Const<5>()); };
+    const bool apart = p.inner != 1 || p.outer_stride != p.columns || (REF && ref_outer != p.columns);
+    auto lanes = [&](auto most, auto turn) {
+        constexpr int MOST = decltype(most)::value;
+        constexpr bool TURN = decltype(turn)::value;
+        const int n = short_grid(CUS * short_residents<E, MOST, REF, TURN>());
+        const size_t lds = (size_t)short_tile<E, MOST>((int)p.columns) * (BLOCK / WAVE) * (REF ? 2 : 1);
+        if (apart) short_rows<E, MOST, REF, Op, TURN, true><<<n, BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        else short_rows<E, MOST, REF, Op, TURN, false><<<n, BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    };
     if (lane_per_row) {
-        auto lds = [&](int tile) { return (size_t)tile * (BLOCK / WAVE) * (REF ? 2 : 1); };
-        if (p.columns <= 8) short_rows<E, 8, REF, Op><<<short_grid(CUS * short_residents<E, 8, REF>()), BLOCK, lds(short_tile<E, 8>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if (SIZE == 4 && p.columns == 16)
-            short_rows<E, 16, REF, Op, SIZE == 4><<<short_grid(CUS * short_residents<E, 16, REF, SIZE == 4>()), BLOCK, lds(short_tile<E, 16>(16)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if (p.columns <= 16) short_rows<E, 16, REF, Op><<<short_grid(CUS * short_residents<E, 16, REF>()), BLOCK, lds(short_tile<E, 16>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if (p.columns <= 24) short_rows<E, 24, REF, Op><<<short_grid(CUS * short_residents<E, 24, REF>()), BLOCK, lds(short_tile<E, 24>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if (SIZE == 4 && !REF && p.columns == 32) {
-            if constexpr (SIZE == 4 && !REF)
-                short_rows<E, 32, REF, Op, true><<<short_grid(CUS * short_residents<E, 32, REF, true>()), BLOCK, lds(short_tile<E, 32>(32)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        } else if (p.columns <= 32) short_rows<E, 32, REF, Op><<<short_grid(CUS * short_residents<E, 32, REF>()), BLOCK, lds(short_tile<E, 32>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        else if constexpr (SIZE == 2 && !REF) {
-            if (p.columns <= 48) short_rows<E, 48, REF, Op><<<short_grid(CUS * short_residents<E, 48, REF>()), BLOCK, lds(short_tile<E, 48>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-            else short_rows<E, 64, REF, Op><<<short_grid(CUS * short_residents<E, 64, REF>()), BLOCK, lds(short_tile<E, 64>((int)p.columns)), stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+        const std::integral_constant<bool, false> straight;
+        const std::integral_constant<bool, SIZE == 4> turned;
+        if (p.columns <= 8) lanes(Const<8>(), straight);
+        else if (SIZE == 4 && p.columns == 16) lanes(Const<16>(), turned);
+        else if (p.columns <= 16) lanes(Const<16>(), straight);
+        else if (p.columns <= 24) lanes(Const<24>(), straight);
+        else if (p.columns < 32) lanes(Const<32>(), straight);
+        else if (p.columns == 32) {
+            if constexpr (SIZE == 2 || !REF) lanes(Const<32>(), turned);
+        } else if constexpr (SIZE == 2 && !REF) {
+            if (p.columns <= 48) lanes(Const<48>(), straight);
+            else lanes(Const<64>(), straight);
         }
     } else if (group(Const<4>(), Const<1>()) || group(Const<4>(), Const<2>()) || groups(Const<4>()) || groups(Const<8>()) || groups(Const<16>()) || groups(Const<32>()) ||
                groups(Const<64>()) || group(Const<128>(), Const<3>()) || group(Const<64>(), Const<8>()) || (p.rows >= 2 * CUS && (group(Const<128>(), Const<5>()) || groups(Const<256>())))) {

@@ -406,6 +406,7 @@ LOGITS = [
     (66, 8, "f16", "plain"), (129, 32, "bf16", "plain"),
     (321, 32, "f32", "plain"), (66, 32, "f32", "window"), (65, 32, "f32", "pitch"), (193, 25, "f32", "plain"), (70, 31, "f32", "pitch"), (500, 23, "f32", "plain"), (259, 20, "f16", "plain"),
     (321, 33, "bf16", "plain"), (130, 48, "f16", "window"), (193, 49, "bf16", "pitch"), (259, 63, "f16", "plain"), (129, 64, "bf16", "pitch"), (129, 55, "bf16", "plain"),
+    (130, 3, "bf16", "pitch"), (66, 2, "f32", "window"), (130, 24, "f32", "window"), (195, 8, "bf16", "pitch"), (70, 5, "f32", "pitch"), (259, 40, "f16", "pitch"),
     (33, 90, "bf16", "plain"), (20, 150, "f16", "pitch"), (18, 190, "bf16", "window"), (21, 300, "bf16", "plain"), (17, 380, "f16", "plain"), (9, 600, "bf16", "pitch"), (9, 700, "f16", "plain"),
     (5, 1200, "bf16", "plain"), (6, 1500, "bf16", "window"), (5, 2047, "bf16", "plain"), (50, 45, "f32", "plain"), (40, 70, "f32", "window"), (30, 95, "f32", "pitch"), (19, 155, "f32", "plain"),
     (17, 190, "f32", "plain"), (12, 310, "f32", "window"), (9, 380, "f32", "plain"), (7, 601, "f32", "pitch"), (5, 767, "f32", "plain"), (5, 1277, "f32", "plain"), (3, 2040, "f32", "plain"),
@@ -654,6 +655,20 @@ def test_policy_loss(B, A, dtype, layout, ref):
     with torch.no_grad():
         again = ops().policy_loss(t, flat(actions), flat(old), flat(adv), **kw)
     assert torch.equal(again.loss, out.loss.detach()) and torch.equal(again.stats, out.stats)
+
+
+@pytest.mark.parametrize("B,A,dtype", [(130, 15, "bf16"), (70, 16, "f32"), (257, 31, "f32"), (66, 5, "f16"), (129, 200, "bf16")])
+def test_policy_loss_beside_a_reference_laid_out_otherwise(B, A, dtype):
+    g, x, actions, old, adv = policy_inputs(B, A, dtype, B + 3 * A)
+    ref = (x.float() + rand((B, A), g, scale=0.5)).to(x.dtype)
+    loss, T_loss, stats, T_stats, d, T_d = policy_64(x, actions, old, adv, 0.2, 0.2, 0.3, 0.02, None, ref, None)
+    for ours, theirs in (("plain", "pitch"), ("pitch", "plain"), ("pitch", "pitch")):
+        t = put_rows(x, ours).requires_grad_()
+        out = ops().policy_loss(t, actions.cuda(), old.cuda(), adv.cuda(), kl_coef=0.3, entropy_coef=0.02, ref_logits=put_rows(ref, theirs))
+        check(out.loss, loss, T_loss, "loss")
+        check(out.stats, stats, T_stats, "stats")
+        (got,) = torch.autograd.grad(out.loss, t)
+        check(got, d, T_d + rounding(d, x.dtype), "gradient")
 
 
 @pytest.mark.parametrize("B,A,dtype,ref", [(513, 20011, "f32", True), (515, 40003, "bf16", True), (600, 5000, "f16", True), (520, 33333, "bf16", False), (1030, 2500, "f32", False),
