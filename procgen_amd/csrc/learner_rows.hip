@@ -418,7 +418,7 @@ constexpr int short_residents() {
 }
 
 // Loss and gradient of 4 194 304 x 15 bf16: 67 to 76 us, 306 MB, 4.0 to 4.6 TB/s; without fetching ahead 98, with the register limit of six blocks (and
-// spills) 93, of four 78.  What is left is the issue of instructions: some 380 vector and 230 scalar ones for 64 rows.
+// spills) 93, of four 78.  What is left is the issue of instructions: some 360 vector and 190 scalar ones for 64 rows.
 template <class E, int MOST, bool REF, class Op, bool TURN, bool APART>
 __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) void short_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
