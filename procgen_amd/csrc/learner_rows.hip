@@ -1,15 +1,15 @@
 // learner_rows.hip -- rows of logits, one column per action: log-probabilities and entropy of the actions taken (forward, backward) and the clipped
 // policy loss with its gradient.
 //
-// With m = max l and everything in powers of two, t[j] = (l[j] - m) log2 e as ONE FMA of l[j] (the rounding of m log2 e is the same in every column; `delta`,
-// what the maximum itself comes to, takes it out again), e[j] = 2^t[j], s = sum e:
-//     p[j] = e[j] / s,   log p[j] = ln 2 (t[j] - delta) - log s,   H = log s - ln 2 (sum e t / s - delta),
-// and against a reference row r (q, delta', s' alike)  KL = ln 2 (sum e (t - q) / s - delta + delta') + log s' - log s: every term is of the size of the
-// differences, so nothing of the size of the logits cancels.  The gradients of all three operators have one form,
+// With m = max l, x[j] = l[j] - m, e[j] = exp(x[j]), s = sum e:
+//     p[j] = e[j] / s,   log p[j] = x[j] - log s,   H = log s - sum e x / s,
+// and against a reference row r (y[j] = r[j] - max r, s' alike)  KL = sum e (x - y) / s + log s' - log s: every term is of the size of the differences, so
+// nothing of the size of the logits cancels.  The gradients of all three operators have one form,
 //     dl[j] = pick * (1[j = a] - p[j]) + p[j] * (kl * (log p[j] - log q[j] - KL) + ent * (log p[j] + H))
-//           = e[j] * (cd t[j] + cq q[j] + c0)  (+ pick at a)
-// with three coefficients of the row.  A column that is -inf (or too far below the maximum) has e = 0 and counts as 0 whatever it is multiplied with:
-// product() is the hardware's multiplication in which zero times anything is zero.
+//           = e[j] * (cd x[j] + cq y[j] + c0)  (+ pick at a)
+// with three coefficients of the row.  The difference comes first and is rounded by itself, at any size of l.  (Taken as one FMA, l log2 e - m log2 e, it
+// would be off by half a step of m log2 e, which from |m| of 2^30 on is more than float32's exponents reach.)  A column that is -inf (or too far below
+// the maximum) has e = 0 and counts as 0 whatever it is multiplied with: product() is the hardware's multiplication in which zero times anything is zero.
 // Partial sums of a row are taken against the largest value their lane or wave has seen and rescaled when they meet (Stats::join), so a row is read once.
 //
 // Bound by memory: a column costs 12 operations for 4 to 8 bytes, 23 for 6 to 12 with a reference (a 1 GiB copy reaches 5.1 TB/s on the same card).  By
@@ -43,29 +43,20 @@ __device__ inline long long row_offset(const procgen_amd_rows &p, long long r, l
     return group * outer + ((uint32_t)r - group * per) * inner;
 }
 
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
+constexpr float LOG2E = 1.44269504088896340736f;
 __device__ inline float exp2_of(float t) { return __builtin_amdgcn_exp2f(t); }
 __device__ float multiply_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");  // v_mul_legacy_f32, which has no builtin function
 __device__ inline float product(float e, float x) { return multiply_legacy(e, x); }
 
-// the difference to a maximum in powers of two, t = scale * l - base.  Near the ends of float32 m log2 e would overflow; there two different numbers are
-// so far apart that any scale tells them apart, and a power of two is exact.
-struct Base {
-    float scale, base;
-    __device__ explicit Base(float m) {
-#pragma clang fp contract(off)  // base is this rounded number wherever it is used, or delta does not cancel
-        const bool far = fabsf(m) > 1e38f && fabsf(m) < INFINITY;
-        scale = far ? 0x1p-64f : LOG2E;
-        base = m == -INFINITY ? 0.f : m * scale;
-    }
-    __device__ float t(float l) const { return fmaf(l, scale, -base); }
-};
+__device__ inline float exp_of(float x) { return exp2_of(x * LOG2E); }
+// what a row's columns are taken against: its maximum, or 0 where no column is finite
+__device__ inline float level_of(float m) { return m == -INFINITY ? 0.f : m; }
 
 // sums over the columns seen so far.  m = -inf: none that is finite; s is then 0, or NaN where a NaN was among them
 template <bool REF>
 struct Stats {
-    float m = -INFINITY, s = 0.f, w = 0.f;   // max, sum e, sum e t
-    float m2 = -INFINITY, s2 = 0.f, u = 0.f; // of the reference row, and sum e (t - q)
+    float m = -INFINITY, s = 0.f, w = 0.f;   // max, sum e, sum e x
+    float m2 = -INFINITY, s2 = 0.f, u = 0.f; // of the reference row, and sum e (x - y)
     __device__ void put(float *to) const {
         to[0] = m, to[1] = s, to[2] = w;
         if (REF) to[3] = m2, to[4] = s2, to[5] = u;
@@ -77,25 +68,25 @@ struct Stats {
     __device__ bool empty() const { return m == -INFINITY && s == 0.f; }
     // the same sums against larger maxima
     __device__ void rescale(float to, float to2) {
-        const float d = m == -INFINITY ? 0.f : Base(m).base - Base(to).base, c = exp2_of(d), d2 = !REF || m2 == -INFINITY ? 0.f : Base(m2).base - Base(to2).base;
+        const float d = m == -INFINITY ? 0.f : m - to, c = exp_of(d), d2 = !REF || m2 == -INFINITY ? 0.f : m2 - to2;
         if (REF) {
-            u = product(c, fmaf(s, d - d2, u));
-            s2 *= exp2_of(d2);
+            u = product(c, product(s, d - d2) + u);
+            s2 = product(exp_of(d2), s2);
             m2 = to2;
         }
-        w = product(c, fmaf(s, d, w));
+        w = product(c, product(s, d) + w);
         s *= c;
         m = to;
     }
-    // columns against maxima that cover them
-    __device__ void add(const Base &b, const Base &b2, float l, float r) {
-        const float t = b.t(l), e = exp2_of(t);
+    // columns against levels that cover them
+    __device__ void add(float level, float level2, float l, float r) {
+        const float x = l - level, e = exp_of(x);
         s += e;
-        w += product(e, t);
+        w += product(e, x);
         if (REF) {
-            const float q = b2.t(r);
-            s2 += exp2_of(q);
-            u += product(e, t - q);
+            const float y = r - level2;
+            s2 += exp_of(y);
+            u += product(e, x - y);
         }
     }
     // lanes that hold no wave's sums take the first one's
@@ -122,21 +113,19 @@ struct Stats {
         }
     }
 };
-// a row's own numbers: natural logarithms, the largest value taken out
+// a row's own numbers
 template <bool REF>
 struct Row {
-    float m, log_s, inv_s, H, delta, delta2, log_s2, KL;
+    float m, log_s, inv_s, H, log_s2, KL;
     __device__ explicit Row(const Stats<REF> &x) {
-        m = x.m == -INFINITY ? 0.f : x.m;
-        delta = Base(x.m).t(m);
+        m = level_of(x.m);
         inv_s = 1.f / x.s;
-        log_s = logf(x.s) - LN2 * delta;
-        H = log_s - LN2 * (x.w * inv_s - delta);
-        delta2 = log_s2 = KL = 0.f;
+        log_s = logf(x.s);
+        H = log_s - x.w * inv_s;
+        log_s2 = KL = 0.f;
         if (REF) {
-            delta2 = x.m2 == -INFINITY ? 0.f : Base(x.m2).t(x.m2);
-            log_s2 = logf(x.s2) - LN2 * delta2;
-            KL = x.s2 == 0.f ? INFINITY : fmaf(LN2, x.u * inv_s, logf(x.s2 * inv_s));  // the deltas are in both terms and cancel
+            log_s2 = logf(x.s2);
+            KL = x.s2 == 0.f ? INFINITY : fmaf(x.u, inv_s, logf(x.s2 * inv_s));
         }
     }
     __device__ float logp(float l) const { return (l - m) - log_s; }
@@ -147,26 +136,24 @@ struct Sums {
     double policy = 0, kl = 0, entropy = 0, clipped = 0;
 };
 struct Coef {
-    Base b, b2;
-    float cd, cq, c0, pick;
-    __device__ Coef() : b(0.f), b2(0.f) {}
+    float level, level2, cd, cq, c0, pick;
     // from the formula's numbers, all of them times `scale`.  Without a known action, or with a NaN among the logits, everything is NaN.
     template <bool REF>
     __device__ void set(bool known, const Stats<REF> &x, const Row<REF> &row, float choice, float kl, float ent, float scale) {
-        b = Base(x.m), b2 = Base(x.m2);
-        if (!known || x.s != x.s) b.base = NAN;
+        level = known && x.s == x.s ? row.m : NAN, level2 = level_of(x.m2);
         const float by = row.inv_s * scale;
-        cd = (ent + kl) * by * LN2;
-        cq = -kl * by * LN2;
-        c0 = (ent * (row.H - row.log_s) + (REF && kl != 0.f ? kl * ((row.log_s2 - row.log_s) - row.KL) : 0.f) - choice) * by - cd * row.delta - cq * row.delta2;
+        cd = (ent + kl) * by;
+        cq = -kl * by;
+        c0 = (ent * (row.H - row.log_s) + (REF && kl != 0.f ? kl * ((row.log_s2 - row.log_s) - row.KL) : 0.f) - choice) * by;
         pick = choice * scale;
     }
+    __device__ bool nan() const { return level != level; }
     template <bool REF>
     __device__ float gradient(float l, float r) const {
-        const float t = b.t(l);
-        float f = fmaf(cd, t, c0);
-        if (REF) f = fmaf(cq, b2.t(r), f);
-        return product(exp2_of(t), f);
+        const float x = l - level;
+        float f = fmaf(cd, x, c0);
+        if (REF) f = fmaf(cq, r - level2, f);
+        return product(exp_of(x), f);
     }
 };
 
@@ -462,7 +449,7 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) voi
         bool some = false;
         Coef c;
         if (wanted) {
-            // the columns that a row has not are -inf; l and l2 become t and q
+            // the columns that a row has not are -inf; l and l2 become x and y
             // reads what a row has not and drops it, which keeps the reads together; where registers are short it is not read (15 bf16 67 : 76 us)
             constexpr bool AGAIN = MOST > 48 || (REF && MOST > 24 && sizeof(T) == 4);  // exponentials are taken again for the gradient: registers for all of them would be spilled
             constexpr bool GUARD = Op::HEAVY && MOST == 16 && !REF && sizeof(T) == 2;
@@ -480,16 +467,16 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) voi
                 x.m = fmaxf(x.m, l[j]);
                 if (REF) x.m2 = fmaxf(x.m2, l2[j]);
             }
-            const Base b(x.m), b2(x.m2);
+            const float level = level_of(x.m), level2 = level_of(x.m2);
 #pragma unroll
             for (int j = 0; j < MOST; j++) {
-                l[j] = b.t(l[j]);
-                e[j] = exp2_of(l[j]);
+                l[j] -= level;
+                e[j] = exp_of(l[j]);
                 x.s += e[j];
                 x.w += product(e[j], l[j]);
                 if (REF) {
-                    l2[j] = b2.t(l2[j]);
-                    x.s2 += exp2_of(l2[j]);
+                    l2[j] -= level2;
+                    x.s2 += exp_of(l2[j]);
                     x.u += product(e[j], l[j] - l2[j]);
                 }
             }
@@ -501,14 +488,14 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) voi
                 for (int j = 0; j < MOST; j++) {
                     if (AGAIN) {
                         asm volatile("" : "+v"(l[j]));
-                        e[j] = exp2_of(l[j]);
+                        e[j] = exp_of(l[j]);
                     }
                     float f = fmaf(c.cd, l[j], c.c0);
                     if (REF) f = fmaf(c.cq, l2[j], f);
                     if (j <= surely || j < columns) row[j ^ turn] = (T)product(e[j], f);
                 }
                 if (known) row[a ^ turn] = (T)(c.gradient<REF>(taken, taken2) + c.pick);
-                if (c.b.base != c.b.base)
+                if (c.nan())
                     for (int j = 0; j < columns; j++) row[j] = (T)NAN;
             }
         }
@@ -634,13 +621,13 @@ __global__ __launch_bounds__(BLOCK) void group_rows(procgen_amd_rows p, Op op, c
             if (REF) to2 = fmaxf(to2, __shfl_xor(to2, d, WAVE));
         }
         x.m = to, x.m2 = to2;
-        const Base b(to), b2(to2);
+        const float level = level_of(to), level2 = level_of(to2);
 #pragma unroll
         for (int i = 0; i < CH; i++) {
             l[i].forget();
             if (REF) l2[i].forget();
 #pragma unroll
-            for (int k = 0; k < N; k++) x.add(b, b2, l[i][k], REF ? l2[i][k] : 0.f);
+            for (int k = 0; k < N; k++) x.add(level, level2, l[i][k], REF ? l2[i][k] : 0.f);
         }
         for (int d = LANES / 2; d > 0; d >>= 1) {
             x.s += __shfl_xor(x.s, d, WAVE);
@@ -739,7 +726,7 @@ __global__ __launch_bounds__(G, 4) void long_rows(procgen_amd_rows p, Op op, con
             const bool known = a >= 0 && a < columns;
             const float taken = (float)row[known ? a : 0];
             Stats<REF> x;
-            Base base(x.m), base2(x.m2);
+            float level = 0.f, level2 = 0.f;
             load(0);
             for (int b = 0; b < batches; b++) {
                 take(b);
@@ -763,13 +750,13 @@ __global__ __launch_bounds__(G, 4) void long_rows(procgen_amd_rows p, Op op, con
                 // m need not be the largest value, only near it: it is moved where it is left behind by more than 8, which after the first batches is rare
                 if (!(to <= x.m + 8.f) || (REF && !(to2 <= x.m2 + 8.f))) {
                     x.rescale(to, to2);
-                    base = Base(to);
-                    base2 = Base(to2);
+                    level = level_of(to);
+                    level2 = level_of(to2);
                 }
                 forget();
 #pragma unroll
                 for (int i = 0; i < CH; i++)
-                    for (int k = 0; k < N; k++) x.add(base, base2, l[i][k], REF ? l2[i][k] : 0.f);
+                    for (int k = 0; k < N; k++) x.add(level, level2, l[i][k], REF ? l2[i][k] : 0.f);
             }
             x.template join<WAVE>();
             if (lane == 0) x.put(wave_stats[odd][threadIdx.x / WAVE]);

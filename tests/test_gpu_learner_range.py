@@ -1,0 +1,118 @@
+"""
+GPU: rows of logits over the whole range of their type -- finite masks of any size, rows of one value, diverged logits -- against 64 bits.
+
+Tolerances are those of test_gpu_learner_ops (running error bounds in 64 bits).  They hold at any size of the logits, because a logit enters only as
+its difference to the row's largest one: that subtraction is rounded once, relative to the difference.
+"""
+import pytest
+import torch
+
+from test_gpu_learner_ops import DTYPES, U, Rows64, check, gen, ops, pick, policy_64, put_rows, rounding
+
+pytestmark = pytest.mark.gpu
+
+LOW = torch.finfo(torch.float32).min
+FILLS = [s * v for v in (1e3, 1e6, 1e8, 1e9, 1.5e9, 3e9, 1e10, 1e12, 1e20, 1e30, 1e37, 9e37, 2e38, 3.3e38) for s in (1.0, -1.0)] + [LOW]
+HALVES = [(1.5e38, 9e37), (2e38, 1e19), (-2e38, -0.9e38), (-1e10, -1e20), (-1e30, LOW), (1e20, 2e38), (1e10, 0.0), (-1e10, 0.0), (5e8, 4.9e8), (1.7e7, 1.7e7 - 2), (3e9, LOW), (0.0, LOW)]
+# columns and how often the rows are repeated: a lane per row; groups inside a wave; of two waves (2700 of 16 bits, 1400 of 32); of four (where there
+# are 512 rows); a block per row in one batch, several, and more than its LDS keeps
+WIDTHS = [(2, 1), (15, 1), (16, 1), (31, 1), (40, 1), (200, 1), (1000, 1), (1400, 1), (2700, 1), (9000, 1), (9000, 20), (50021, 1)]
+
+
+def gradient_64(w, actions, d_logp, d_entropy):
+    """of sum(d_logp * logp + d_entropy * entropy), and how far 32 bits may be off"""
+    onehot = torch.zeros_like(w.p).scatter_(1, actions.long()[:, None], 1.0)
+    gl, ge = d_logp.double()[:, None], d_entropy.double()[:, None]
+    both = torch.where(w.p > 0, w.finite_logp + w.H[:, None], torch.zeros_like(w.p))
+    want = gl * (onehot - w.p) - ge * w.p * both
+    tol = gl.abs() * w.p * w.rel_p + ge.abs() * w.p * (both.abs() * w.rel_p + w.T_logp + w.T_H[:, None]) + 8 * U * (gl.abs() * (onehot + w.p) + ge.abs() * w.p * both.abs())
+    return want, tol
+
+
+def compare(x, actions, seed, ref=None, wide_gradient=True):
+    """the three calls on rows x [B, A] (on the GPU, at any size) against their definitions in 64 bits"""
+    B, A = x.shape
+    g = gen(seed)
+    w = Rows64(x)
+    t = x.detach().clone().requires_grad_()
+    logp, entropy = ops().action_logprobs(t, actions)
+    check(logp, pick(w.logp, actions).cpu(), pick(w.T_logp, actions).cpu(), "log-probabilities")
+    check(entropy, w.H.cpu(), w.T_H.cpu(), "entropy")
+    d_logp, d_entropy = (torch.randn((B,), generator=g).cuda() for _ in range(2))
+    (d,) = torch.autograd.grad([logp, entropy], [t], [d_logp, d_entropy])
+    if wide_gradient or A <= 1024:
+        want, tol = gradient_64(w, actions, d_logp, d_entropy)
+        check(d, want.cpu(), (tol + rounding(want, x.dtype)).cpu(), "gradient of the log-probabilities")
+    step, adv = (0.05 * torch.rand((B,), generator=g).cuda() + 0.01), torch.randn((B,), generator=g).cuda()
+    old = (pick(w.logp, actions) - step).float()
+    kl_coef = 0.0 if ref is None else 0.3
+    want = [v.cpu() for v in policy_64(x, actions, old, adv, 0.2, 0.2, kl_coef, 0.02, None, ref)]
+    out = ops().policy_loss(t, actions, old, adv, kl_coef=kl_coef, ref_logits=ref, entropy_coef=0.02)
+    check(out.loss, want[0], want[1], "loss")
+    check(out.stats, want[2], want[3], "stats")
+    (d,) = torch.autograd.grad(out.loss, t)
+    check(d, want[4], want[5] + rounding(want[4], x.dtype), "gradient of the loss")
+
+
+def rows_of(values, A, dtype, repeat):
+    values = [v for v in values if abs(v) <= torch.finfo(DTYPES[dtype]).max] if dtype == "f16" else values
+    return torch.tensor(values, dtype=torch.float64).clamp(torch.finfo(DTYPES[dtype]).min, torch.finfo(DTYPES[dtype]).max).to(DTYPES[dtype])[:, None].repeat(repeat, A).cuda()
+
+
+@pytest.mark.parametrize("A,repeat", WIDTHS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_rows_of_one_value(A, repeat, dtype):
+    """wholly masked, or diverged all alike: a uniform distribution, whatever the value; beside an ordinary reference, and as one"""
+    x = rows_of(FILLS, A, dtype, repeat)
+    g = gen(A)
+    actions = torch.randint(0, A, (x.shape[0],), generator=g).cuda()
+    compare(x, actions, 1, None, wide_gradient=False)
+    other = (2 * torch.randn(x.shape, generator=g)).to(x.dtype).cuda()
+    compare(x, actions, 2, other, wide_gradient=False)
+    compare(other, actions, 3, x, wide_gradient=False)
+
+
+@pytest.mark.parametrize("A,repeat", WIDTHS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_of_two_values(A, repeat, dtype):
+    """two values in a row, one in its first half and one in the second, or in one column alone: whole lanes, waves and batches see only one of them"""
+    rows = []
+    for a, b in HALVES:
+        for row in (torch.full((A,), a, dtype=torch.float64), torch.full((A,), b, dtype=torch.float64)):
+            row[A // 2:] = b
+            rows.append(row.clone())
+            rows.append(row.flip(0))
+        alone = torch.full((A,), b, dtype=torch.float64)
+        alone[A - 1] = a
+        rows.append(alone)
+    x = torch.stack(rows).clamp(torch.finfo(DTYPES[dtype]).min, torch.finfo(DTYPES[dtype]).max).to(DTYPES[dtype]).repeat(1 if repeat == 1 else 9, 1).cuda()
+    actions = x.argmax(1)
+    compare(x, actions, 4, None, wide_gradient=False)
+    compare(x, actions, 5, x.flip(0) * 0 + x, wide_gradient=False)
+
+
+@pytest.mark.parametrize("A,repeat", WIDTHS[1:])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_rows_with_finite_masks(A, repeat, dtype):
+    """columns masked with one finite value, or with several: those of whole lanes, waves and batches among them, in the logits, the reference or both"""
+    g = gen(A + 1)
+    dt = DTYPES[dtype]
+    masks = [-1e4, -65504.0] if dtype == "f16" else [-1e9, -1e10, -1e12, -1e20, -1e30, -3e38, torch.finfo(dt).min]
+    B = (len(masks) + 2) * (1 if repeat == 1 else 58)
+    x, ref = ((2 * torch.randn((B, A), generator=g)).to(dt) for _ in range(2))
+    masked = torch.rand((B, A), generator=g) < 0.3
+    masked[:, A // 8:A // 2] = True
+    masked[1::3, A // 2:A - 3] = True
+    masked[:, A - 1] = False
+    several = torch.tensor(masks)[torch.randint(0, len(masks), (B, A), generator=g)]
+    value = torch.tensor((masks + [0.0, 0.0]) * (B // (len(masks) + 2)))[:, None].expand(B, A)
+    value = torch.where(value == 0, several, value).to(dt)
+    both, mine = torch.where(masked, value, x), torch.where(masked, torch.tensor(masks[0], dtype=dt), x)
+    masked_ref = torch.where(masked, value, ref)
+    actions = torch.full((B,), A - 1).cuda()
+    compare(both.cuda(), actions, 6, None)
+    compare(both.cuda(), actions, 7, masked_ref.cuda())
+    compare(mine.cuda(), actions, 8, ref.cuda())
+    # a reference that excludes with a finite number what the policy may do: KL is about as large as that number, and a number
+    far = torch.where(masked, torch.where(value.float() < -1e30, torch.tensor(-1e30), value.float()).to(dt), ref)
+    compare(x.cuda(), actions, 9, far.cuda())
