@@ -152,7 +152,7 @@ struct Coef {
     __device__ float gradient(float l, float r) const {
         const float x = l - level;
         float f = fmaf(cd, x, c0);
-        if (REF) f = fmaf(cq, r - level2, f);
+        if (REF) f += product(cq, r - level2);  // a reference without weight may hold anything
         return product(exp_of(x), f);
     }
 };
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) voi
                         e[j] = exp_of(l[j]);
                     }
                     float f = fmaf(c.cd, l[j], c.c0);
-                    if (REF) f = fmaf(c.cq, l2[j], f);
+                    if (REF) f += product(c.cq, l2[j]);
                     if (j <= surely || j < columns) row[j ^ turn] = (T)product(e[j], f);
                 }
                 if (known) row[a ^ turn] = (T)(c.gradient<REF>(taken, taken2) + c.pick);

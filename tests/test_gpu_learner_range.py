@@ -116,3 +116,35 @@ def test_rows_with_finite_masks(A, repeat, dtype):
     # a reference that excludes with a finite number what the policy may do: KL is about as large as that number, and a number
     far = torch.where(masked, torch.where(value.float() < -1e30, torch.tensor(-1e30), value.float()).to(dt), ref)
     compare(x.cuda(), actions, 9, far.cuda())
+
+
+def watched_inputs(B, A, dtype, seed):
+    g = gen(seed)
+    x = (2 * torch.randn((B, A), generator=g)).to(DTYPES[dtype])
+    actions = torch.randint(0, A, (B,), generator=g)
+    old = (pick(Rows64(x).logp, actions) - 0.05 * torch.rand((B,), generator=g) - 0.01).float()
+    return g, x, actions, old, torch.randn((B,), generator=g)
+
+
+@pytest.mark.parametrize("A,repeat", WIDTHS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_reference_without_weight_does_not_reach_the_gradient(A, repeat, dtype):
+    """kl_coef = 0, the KL only watched: reference columns of -inf, of the lowest value and NaN, and rows of nothing else, change the statistics alone"""
+    B = 6 * (1 if repeat == 1 else 87)
+    g, x, actions, old, adv = watched_inputs(B, A, dtype, A + 2)
+    ref = (x.float() + 0.3 * torch.randn((B, A), generator=g)).to(x.dtype)
+    ref[1::6, A // 2:] = float("-inf")
+    ref[2::6, ::2] = torch.finfo(x.dtype).min
+    ref[3::6] = float("-inf")
+    ref[4::6, A - 1] = float("nan")
+    ref[5::6, 0] = float("inf")
+    want = [v.cpu() for v in policy_64(x.cuda(), actions.cuda(), old.cuda(), adv.cuda(), 0.2, 0.2, 0.0, 0.02)]
+    t = x.cuda().requires_grad_()
+    out = ops().policy_loss(t, actions.cuda(), old.cuda(), adv.cuda(), kl_coef=0.0, ref_logits=ref.cuda(), entropy_coef=0.02)
+    assert out.stats[1].isnan()
+    check(out.loss, want[0], want[1], "loss")
+    check(out.stats[[0, 2, 3]], want[2][[0, 2, 3]], want[3][[0, 2, 3]], "stats")
+    (d,) = torch.autograd.grad(out.loss, t, retain_graph=True)
+    check(d, want[4], want[5] + rounding(want[4], x.dtype), "gradient")
+    (d,) = torch.autograd.grad(out.loss * 4, t)
+    check(d, want[4] * 4, want[5] * 4 + rounding(want[4] * 4, x.dtype), "gradient of 4 times the loss")
