@@ -230,7 +230,7 @@ struct Policy {
         if (!REF && q.ref_logprobs) {
             const float d = in.ref - logp, f = expm1f(d);
             KL = f - d;
-            pick -= q.kl_coef * f;
+            pick -= product(q.kl_coef, f);  // without weight it may be infinite
         }
         if (first) {
             sums.policy -= out ? held : plain;

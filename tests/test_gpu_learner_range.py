@@ -148,3 +148,29 @@ def test_a_reference_without_weight_does_not_reach_the_gradient(A, repeat, dtype
     check(d, want[4], want[5] + rounding(want[4], x.dtype), "gradient")
     (d,) = torch.autograd.grad(out.loss * 4, t)
     check(d, want[4] * 4, want[5] * 4 + rounding(want[4] * 4, x.dtype), "gradient of 4 times the loss")
+
+
+@pytest.mark.parametrize("A,repeat", WIDTHS)
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_an_estimator_without_weight_does_not_reach_the_gradient(A, repeat, dtype):
+    """as above with the reference's log-probabilities: of actions that the policy has all but excluded (the estimator's exponential is infinite), or has"""
+    B = 5 * (1 if repeat == 1 else 104)
+    g, x, actions, old, adv = watched_inputs(B, A, dtype, A + 3)
+    x[0::5] = 0
+    x[0::5, A - 1] = -120.0
+    x[1::5, A - 1] = float("-inf")
+    actions[0::5] = actions[1::5] = A - 1
+    old[0::5] = old[1::5] = -1.0
+    ref = old + 0.2
+    ref[0::5] = ref[1::5] = 0.0
+    ref[2::5] = float("-inf")
+    ref[3::5] = float("nan")
+
+    def loss(t, **kw):
+        return ops().policy_loss(t, actions.cuda(), old.cuda(), adv.cuda(), entropy_coef=0.02, **kw)
+
+    t = x.cuda().requires_grad_()
+    want, out = loss(t), loss(t, kl_coef=0.0, ref_logprobs=ref.cuda())
+    (d,), (e,) = torch.autograd.grad(want.loss, t), torch.autograd.grad(out.loss, t)
+    assert torch.equal(out.loss, want.loss) and torch.equal(out.stats[[0, 2, 3]], want.stats[[0, 2, 3]]) and out.stats[1].isnan()
+    assert d.isfinite().all() and torch.equal(d, e)
