@@ -88,11 +88,16 @@ struct procgen_amd_rows {
 };
 LIBENV_API long long procgen_amd_rows_workspace(long long rows, long long columns);
 
-/* logp[r] = log p(actions[r]), entropy[r], lse[r] = log sum exp of the row (read by the backward call); float [rows] each */
-LIBENV_API int procgen_amd_action_logprobs(const struct procgen_amd_rows *rows, float *logp, float *entropy, float *lse, int device, void *stream);
+/* log sum exp of a row = largest + log_sum, with log_sum = log sum exp(logit - largest).  In two parts: one float of the size of the logits would round
+ * log_sum away.  largest = -inf: a row without any finite column. */
+struct procgen_amd_lse {
+    float largest, log_sum;
+};
+/* logp[r] = log p(actions[r]), entropy[r]: float [rows]; lse: [rows], read by the backward call, or NULL */
+LIBENV_API int procgen_amd_action_logprobs(const struct procgen_amd_rows *rows, float *logp, float *entropy, struct procgen_amd_lse *lse, int device, void *stream);
 /* d_logits of sum(d_logp * logp + d_entropy * entropy); d_logp, d_entropy: float [rows] or NULL (zeros).  A row whose two are zero gets zeros,
  * whatever its logits hold. */
-LIBENV_API int procgen_amd_action_logprobs_backward(const struct procgen_amd_rows *rows, const float *lse, const float *entropy, const float *d_logp, const float *d_entropy, int device, void *stream);
+LIBENV_API int procgen_amd_action_logprobs_backward(const struct procgen_amd_rows *rows, const struct procgen_amd_lse *lse, const float *entropy, const float *d_logp, const float *d_entropy, int device, void *stream);
 
 /* Clipped policy loss with a KL term:
  *     ratio = exp(logp - old_logprobs);  objective = min(ratio * adv, clip(ratio, 1 - clip_low, 1 + clip_high) * adv)

@@ -162,7 +162,8 @@ struct Coef {
 struct Logprobs {
     static constexpr bool GRADIENT = false, HEAVY = false;
     __device__ bool done() const { return false; }
-    float *logp, *entropy, *lse;
+    float *logp, *entropy;
+    procgen_amd_lse *lse;
     struct In {};
     __device__ void begin(const procgen_amd_rows &) {}
     __device__ In fetch(long long) const { return In(); }
@@ -173,7 +174,7 @@ struct Logprobs {
         const Row<REF> row(x);
         logp[r] = !known ? NAN : x.empty() ? -INFINITY : row.logp(l);
         entropy[r] = x.empty() ? 0.f : row.H;
-        if (lse) lse[r] = x.empty() ? -INFINITY : row.m + row.log_s;
+        if (lse) lse[r] = x.empty() ? procgen_amd_lse{-INFINITY, 0.f} : procgen_amd_lse{row.m, row.log_s};
         return false;
     }
 };
@@ -808,9 +809,9 @@ __global__ __launch_bounds__(G, 4) void long_rows(procgen_amd_rows p, Op op, con
     if (partial) put_sums(sums, op, partial);
 }
 
-// The gradient of long rows' log-probabilities: lse and entropy are known, so every column stands for itself.  1000 x 32001 bf16: 24 us, 5.3 TB/s.
+// The gradient of long rows' log-probabilities: the largest value, the log of the sum and the entropy are known, so every column stands for itself.  1000 x 32001 bf16: 24 us, 5.3 TB/s.
 template <class E>
-__global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, const float *lse, const float *entropy, const float *d_logp, const float *d_entropy) {
+__global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, const procgen_amd_lse *lse, const float *entropy, const float *d_logp, const float *d_entropy) {
     typedef typename E::T T;
     constexpr int N = Chunk<E>::N;
     const int columns = (int)p.columns;
@@ -820,15 +821,16 @@ __global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, c
         const int ahead = (int)((uintptr_t)row / sizeof(T) % N), j = (int)(((long long)blockIdx.x * BLOCK + threadIdx.x) * N) - ahead;
         if (j >= columns) continue;
         const long long a = action_of(p, r);
-        const float pick = d_logp ? d_logp[r] : 0.f, ent = d_entropy ? -d_entropy[r] : 0.f, z = lse[r];
-        const bool known = a >= 0 && a < columns, some = !(pick == 0.f && ent == 0.f) && z != -INFINITY;
+        const float pick = d_logp ? d_logp[r] : 0.f, ent = d_entropy ? -d_entropy[r] : 0.f;
+        const procgen_amd_lse z = lse[r];
+        const bool known = a >= 0 && a < columns, some = !(pick == 0.f && ent == 0.f) && z.largest != -INFINITY;
         Chunk<E> x;
         const int at = max(0, min(j, columns - N));  // aligned 16 bytes but for the first and the last, which write only their own
         x.load(row + at);
         const float H = entropy[r];
         constexpr int PER = N / 4;
         auto gradient = [&](int k) {
-            const float log_p = x[k] - z, p = __expf(log_p);
+            const float log_p = (x[k] - z.largest) - z.log_sum, p = __expf(log_p);
             return product(p, ent * (log_p + H) - pick) + (at + k == a ? pick : 0.f) + (known ? 0.f : NAN);
         };
         for (int k = 0; k < N; k += PER) {
@@ -970,7 +972,7 @@ extern "C" {
 
 LIBENV_API long long procgen_amd_rows_workspace(long long rows, long long columns) { return MAX_COUNT_BLOCKS * (long long)sizeof(long long) + MAX_BLOCKS * 4ll * (long long)sizeof(double); }
 
-LIBENV_API int procgen_amd_action_logprobs(const struct procgen_amd_rows *p, float *logp, float *entropy, float *lse, int device, void *stream) {
+LIBENV_API int procgen_amd_action_logprobs(const struct procgen_amd_rows *p, float *logp, float *entropy, struct procgen_amd_lse *lse, int device, void *stream) {
     if (!rows_ok(p)) return -1;
     if (p->rows == 0) return 0;
     if (!p->logits || !p->actions || !logp || !entropy) return -1;
@@ -980,7 +982,7 @@ LIBENV_API int procgen_amd_action_logprobs(const struct procgen_amd_rows *p, flo
     return got < 0 ? -1 - got : 0;
 }
 
-LIBENV_API int procgen_amd_action_logprobs_backward(const struct procgen_amd_rows *p, const float *lse, const float *entropy, const float *d_logp, const float *d_entropy, int device, void *stream) {
+LIBENV_API int procgen_amd_action_logprobs_backward(const struct procgen_amd_rows *p, const struct procgen_amd_lse *lse, const float *entropy, const float *d_logp, const float *d_entropy, int device, void *stream) {
     if (!rows_ok(p)) return -1;
     if (p->rows == 0) return 0;
     if (!p->logits || !p->actions || !p->d_logits || !lse || !entropy) return -1;

@@ -147,12 +147,12 @@ Tensor as_saved(const Tensor &x, const std::vector<int64_t> &strides, Layout *at
 
 void logprobs_forward(const Tensor &logits, const Layout &at, const Tensor &actions, const Tensor &logp, const Tensor &entropy, const Tensor &lse) {
     const procgen_amd_rows a = rows_of(logits, at, actions, Tensor(), Tensor());
-    check(procgen_amd_action_logprobs(&a, data_as<float>(logp), data_as<float>(entropy), data_as<float>(lse), logits.get_device(), stream_of(logits)), "action_logprobs");
+    check(procgen_amd_action_logprobs(&a, data_as<float>(logp), data_as<float>(entropy), data_as<procgen_amd_lse>(lse), logits.get_device(), stream_of(logits)), "action_logprobs");
 }
 
 struct ActionLogprobs : torch::autograd::Function<ActionLogprobs> {
     static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &actions, Layout at) {
-        Tensor logp = floats(actions.sizes(), logits), entropy = floats(actions.sizes(), logits), lse = floats(actions.sizes(), logits);
+        Tensor logp = floats(actions.sizes(), logits), entropy = floats(actions.sizes(), logits), lse = floats({actions.numel(), 2}, logits);
         logprobs_forward(logits, at, actions, logp, entropy, lse);
         ctx->save_for_backward({logits, actions, lse, entropy});
         ctx->saved_data["strides"] = logits.strides().vec();
@@ -168,7 +168,7 @@ struct ActionLogprobs : torch::autograd::Function<ActionLogprobs> {
         Tensor d_logits = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
         Tensor d_logp = d[0].defined() ? d[0].contiguous() : Tensor(), d_entropy = d[1].defined() ? d[1].contiguous() : Tensor();
         const procgen_amd_rows a = rows_of(logits, at, saved[1], d_logits, Tensor());
-        check(procgen_amd_action_logprobs_backward(&a, data_as<float>(saved[2]), data_as<float>(saved[3]), data_as<float>(d_logp), data_as<float>(d_entropy), logits.get_device(),
+        check(procgen_amd_action_logprobs_backward(&a, data_as<procgen_amd_lse>(saved[2]), data_as<float>(saved[3]), data_as<float>(d_logp), data_as<float>(d_entropy), logits.get_device(),
                                                    stream_of(logits)),
               "action_logprobs");
         return once({d_logits, Tensor(), Tensor()});

@@ -29,7 +29,7 @@ def gradient_64(w, actions, d_logp, d_entropy):
     return want, tol
 
 
-def compare(x, actions, seed, ref=None, wide_gradient=True):
+def compare(x, actions, seed, ref=None):
     """the three calls on rows x [B, A] (on the GPU, at any size) against their definitions in 64 bits"""
     B, A = x.shape
     g = gen(seed)
@@ -40,9 +40,8 @@ def compare(x, actions, seed, ref=None, wide_gradient=True):
     check(entropy, w.H.cpu(), w.T_H.cpu(), "entropy")
     d_logp, d_entropy = (torch.randn((B,), generator=g).cuda() for _ in range(2))
     (d,) = torch.autograd.grad([logp, entropy], [t], [d_logp, d_entropy])
-    if wide_gradient or A <= 1024:
-        want, tol = gradient_64(w, actions, d_logp, d_entropy)
-        check(d, want.cpu(), (tol + rounding(want, x.dtype)).cpu(), "gradient of the log-probabilities")
+    want, tol = gradient_64(w, actions, d_logp, d_entropy)
+    check(d, want.cpu(), (tol + rounding(want, x.dtype)).cpu(), "gradient of the log-probabilities")
     step, adv = (0.05 * torch.rand((B,), generator=g).cuda() + 0.01), torch.randn((B,), generator=g).cuda()
     old = (pick(w.logp, actions) - step).float()
     kl_coef = 0.0 if ref is None else 0.3
@@ -66,10 +65,10 @@ def test_rows_of_one_value(A, repeat, dtype):
     x = rows_of(FILLS, A, dtype, repeat)
     g = gen(A)
     actions = torch.randint(0, A, (x.shape[0],), generator=g).cuda()
-    compare(x, actions, 1, None, wide_gradient=False)
+    compare(x, actions, 1, None)
     other = (2 * torch.randn(x.shape, generator=g)).to(x.dtype).cuda()
-    compare(x, actions, 2, other, wide_gradient=False)
-    compare(other, actions, 3, x, wide_gradient=False)
+    compare(x, actions, 2, other)
+    compare(other, actions, 3, x)
 
 
 @pytest.mark.parametrize("A,repeat", WIDTHS)
@@ -87,8 +86,8 @@ def test_rows_of_two_values(A, repeat, dtype):
         rows.append(alone)
     x = torch.stack(rows).clamp(torch.finfo(DTYPES[dtype]).min, torch.finfo(DTYPES[dtype]).max).to(DTYPES[dtype]).repeat(1 if repeat == 1 else 9, 1).cuda()
     actions = x.argmax(1)
-    compare(x, actions, 4, None, wide_gradient=False)
-    compare(x, actions, 5, x.flip(0) * 0 + x, wide_gradient=False)
+    compare(x, actions, 4, None)
+    compare(x, actions, 5, x.flip(0) * 0 + x)
 
 
 @pytest.mark.parametrize("A,repeat", WIDTHS[1:])
@@ -116,6 +115,16 @@ def test_rows_with_finite_masks(A, repeat, dtype):
     # a reference that excludes with a finite number what the policy may do: KL is about as large as that number, and a number
     far = torch.where(masked, torch.where(value.float() < -1e30, torch.tensor(-1e30), value.float()).to(dt), ref)
     compare(x.cuda(), actions, 9, far.cuda())
+
+
+@pytest.mark.parametrize("A,repeat", WIDTHS + [(32001, 1)])
+@pytest.mark.parametrize("dtype,shift", [("f32", 500.0), ("f32", -5000.0), ("f32", 1e5), ("bf16", 500.0), ("bf16", -30.0), ("f16", -500.0)])
+def test_shifted_rows_keep_their_precision(A, repeat, dtype, shift):
+    """the gradients of every width carry the rounding of differences, not of the logits themselves"""
+    g = gen(A + 4)
+    x = (2 * torch.randn((10 * repeat, A), generator=g) + shift).to(DTYPES[dtype])
+    actions = torch.randint(0, A, (x.shape[0],), generator=g)
+    compare(x.cuda(), actions.cuda(), 10, (x.float() + 0.3 * torch.randn(x.shape, generator=g)).to(x.dtype).cuda())
 
 
 def watched_inputs(B, A, dtype, seed):
