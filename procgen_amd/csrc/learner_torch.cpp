@@ -45,6 +45,19 @@ variable_list once(variable_list out) {
     return out;
 }
 
+// What a backward pass got back of the tensors that were saved.  Hooks (torch.autograd.graph.saved_tensors_hooks) may have kept them elsewhere meanwhile:
+// other strides are taken, anything else would be read as what it is not.
+void came_back(const Tensor &x, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+    if (!x.defined() || x.sizes() != sizes || x.scalar_type() != type || x.device() != device || x.layout() != at::kStrided)
+        throw std::runtime_error("a saved tensor came back from its hooks with another shape, type or device than it was saved with");
+}
+// one that was contiguous, or undefined
+Tensor dense(const Tensor &x, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+    if (!x.defined()) return x;
+    came_back(x, sizes, type, device);
+    return x.contiguous();
+}
+
 // ---- the recurrence -------------------------------------------------------------------------------------------------------------------------
 
 procgen_amd_array3 array3(const Tensor &x) {
@@ -80,16 +93,24 @@ struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
         Tensor checkpoints = floats({procgen_amd_recurrence_checkpoints((int)gate.size(0)), gate.size(1), gate.size(2)}, gate);
         auto [h, last] = recurrence_forward(gate, update, first, state, Tensor(), checkpoints);
         ctx->save_for_backward({gate, update, first, state, checkpoints});
+        ctx->saved_data["shape"] = std::vector<int64_t>{gate.size(0), gate.size(1), gate.size(2), (int64_t)gate.scalar_type(), first.defined() ? (int64_t)first.scalar_type() : 0, gate.get_device()};
         ctx->set_materialize_grads(false);
         return {h, last};
     }
     static variable_list backward(AutogradContext *ctx, variable_list d) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &gate = saved[0], &update = saved[1], &state = saved[3];
+        const std::vector<int64_t> s = ctx->saved_data["shape"].toIntVector();
+        const std::array<int64_t, 3> shape{s[0], s[1], s[2]}, checks{procgen_amd_recurrence_checkpoints((int)s[0]), s[1], s[2]};
+        const at::Device device(at::kCUDA, (at::DeviceIndex)s[5]);
+        const Tensor &gate = saved[0], &update = saved[1], &first = saved[2];
+        came_back(gate, shape, (at::ScalarType)s[3], device);
+        came_back(update, shape, (at::ScalarType)s[3], device);
+        if (first.defined()) came_back(first, {s[0], s[1]}, (at::ScalarType)s[4], device);
+        const Tensor state = dense(saved[3], {s[1], s[2]}, at::kFloat, device), checkpoints = dense(saved[4], checks, at::kFloat, device);
         Tensor work = recurrence_workspace(gate), d_last = d[1].defined() ? d[1].contiguous() : Tensor();
         Tensor d_gate = ctx->needs_input_grad(0) ? at::empty_like(gate) : Tensor(), d_update = ctx->needs_input_grad(1) ? at::empty_like(update) : Tensor();
-        Tensor d_state = state.defined() && ctx->needs_input_grad(saved[2].defined() ? 3 : 2) ? at::empty_like(state) : Tensor();
-        procgen_amd_recurrence a = recurrence(gate, update, saved[2], state, saved[4], work);
+        Tensor d_state = state.defined() && ctx->needs_input_grad(first.defined() ? 3 : 2) ? at::empty_like(state) : Tensor();
+        procgen_amd_recurrence a = recurrence(gate, update, first, state, checkpoints, work);
         a.d_h = array3(d[0]), a.d_gate = array3(d_gate), a.d_update = array3(d_update);
         a.d_state_out = data_as<float>(d_last);
         a.d_state = data_as<float>(d_state);
@@ -138,12 +159,29 @@ procgen_amd_rows rows_of(const Tensor &logits, const Layout &at, const Tensor &a
     a.workspace = data(work);
     return a;
 }
-// a saved tensor may come back with other strides (hooks that keep it elsewhere meanwhile)
-Tensor as_saved(const Tensor &x, const std::vector<int64_t> &strides, Layout *at) {
-    if (x.strides() == at::IntArrayRef(strides)) return x;
-    *at = Layout::contiguous(x);
-    return x.contiguous();
-}
+// what a backward pass needs to know of the logits and actions that were saved
+struct Kind {
+    std::vector<int64_t> sizes;
+    at::ScalarType logits, actions;
+    at::Device device;
+    static void keep(AutogradContext *ctx, const Tensor &logits, const Tensor &actions) {
+        ctx->saved_data["sizes"] = logits.sizes().vec();
+        ctx->saved_data["kind"] = std::vector<int64_t>{(int64_t)logits.scalar_type(), (int64_t)actions.scalar_type(), logits.get_device()};
+    }
+    static Kind kept(AutogradContext *ctx) {
+        const std::vector<int64_t> k = ctx->saved_data["kind"].toIntVector();
+        return {ctx->saved_data["sizes"].toIntVector(), (at::ScalarType)k[0], (at::ScalarType)k[1], at::Device(at::kCUDA, (at::DeviceIndex)k[2])};
+    }
+    at::IntArrayRef rows() const { return at::IntArrayRef(sizes).slice(0, sizes.size() - 1); }
+    Tensor per_row(const Tensor &x, at::ScalarType type) const { return dense(x, rows(), type, device); }
+    // logits, laid out as `at` says or else contiguous
+    Tensor matrix(const Tensor &x, const std::vector<int64_t> &strides, Layout *at) const {
+        came_back(x, sizes, logits, device);
+        if (x.strides() == at::IntArrayRef(strides)) return x;
+        *at = Layout::contiguous(x);
+        return x.contiguous();
+    }
+};
 
 void logprobs_forward(const Tensor &logits, const Layout &at, const Tensor &actions, const Tensor &logp, const Tensor &entropy, const Tensor &lse) {
     const procgen_amd_rows a = rows_of(logits, at, actions, Tensor(), Tensor());
@@ -155,6 +193,7 @@ struct ActionLogprobs : torch::autograd::Function<ActionLogprobs> {
         Tensor logp = floats(actions.sizes(), logits), entropy = floats(actions.sizes(), logits), lse = floats({actions.numel(), 2}, logits);
         logprobs_forward(logits, at, actions, logp, entropy, lse);
         ctx->save_for_backward({logits, actions, lse, entropy});
+        Kind::keep(ctx, logits, actions);
         ctx->saved_data["strides"] = logits.strides().vec();
         ctx->saved_data["layout"] = std::vector<int64_t>{at.inner, at.outer_stride, at.inner_stride};
         ctx->set_materialize_grads(false);
@@ -164,11 +203,13 @@ struct ActionLogprobs : torch::autograd::Function<ActionLogprobs> {
         const variable_list saved = ctx->get_saved_variables();
         const std::vector<int64_t> l = ctx->saved_data["layout"].toIntVector();
         Layout at{l[0], l[1], l[2]};
-        const Tensor logits = as_saved(saved[0], ctx->saved_data["strides"].toIntVector(), &at);
+        const Kind kind = Kind::kept(ctx);
+        const Tensor logits = kind.matrix(saved[0], ctx->saved_data["strides"].toIntVector(), &at), actions = kind.per_row(saved[1], kind.actions);
+        const Tensor lse = dense(saved[2], {actions.numel(), 2}, at::kFloat, kind.device), entropy = kind.per_row(saved[3], at::kFloat);
         Tensor d_logits = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
         Tensor d_logp = d[0].defined() ? d[0].contiguous() : Tensor(), d_entropy = d[1].defined() ? d[1].contiguous() : Tensor();
-        const procgen_amd_rows a = rows_of(logits, at, saved[1], d_logits, Tensor());
-        check(procgen_amd_action_logprobs_backward(&a, data_as<procgen_amd_lse>(saved[2]), data_as<float>(saved[3]), data_as<float>(d_logp), data_as<float>(d_entropy), logits.get_device(),
+        const procgen_amd_rows a = rows_of(logits, at, actions, d_logits, Tensor());
+        check(procgen_amd_action_logprobs_backward(&a, data_as<procgen_amd_lse>(lse), data_as<float>(entropy), data_as<float>(d_logp), data_as<float>(d_entropy), logits.get_device(),
                                                    stream_of(logits)),
               "action_logprobs");
         return once({d_logits, Tensor(), Tensor()});
@@ -223,6 +264,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         const PolicyOut out = policy_forward(p, d_logits, logits, actions, old, adv, valid, ref_logits, ref_logp);
         ctx->save_for_backward({logits, actions, old, adv, valid, ref_logits, ref_logp});
         ctx->saved_data["strides"] = logits.strides().vec();
+        Kind::keep(ctx, logits, actions);
         ctx->saved_data["ref_strides"] = ref_logits.defined() ? ref_logits.strides().vec() : std::vector<int64_t>();
         ctx->saved_data["layout"] = std::vector<int64_t>{p.at.inner, p.at.outer_stride, p.at.inner_stride, p.ref_at.outer_stride, p.ref_at.inner_stride};
         ctx->saved_data["coefs"] = std::vector<double>{p.clip_low, p.clip_high, p.kl_coef, p.entropy_coef};
@@ -237,22 +279,27 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         const std::vector<int64_t> l = ctx->saved_data["layout"].toIntVector();
         const auto coefs = ctx->saved_data["coefs"].toDoubleVector();
         PolicyArgs p{{l[0], l[1], l[2]}, {l[0], l[3], l[4]}, coefs[0], coefs[1], coefs[2], coefs[3]};
+        const Kind kind = Kind::kept(ctx);
         Tensor logits = saved[0], ref_logits = saved[5];
+        came_back(logits, kind.sizes, kind.logits, kind.device);
+        if (ref_logits.defined()) came_back(ref_logits, kind.sizes, kind.logits, kind.device);
         const bool moved = logits.strides() != at::IntArrayRef(ctx->saved_data["strides"].toIntVector()) ||
                            (ref_logits.defined() && ref_logits.strides() != at::IntArrayRef(ctx->saved_data["ref_strides"].toIntVector()));
-        if (moved) {  // hooks that kept a tensor elsewhere may give it back with other strides
+        if (moved) {  // the two share one split of their rows
             logits = logits.contiguous();
             p.at = Layout::contiguous(logits);
             if (ref_logits.defined()) ref_logits = ref_logits.contiguous(), p.ref_at = Layout::contiguous(ref_logits);
         }
+        const Tensor actions = kind.per_row(saved[1], kind.actions), old = kind.per_row(saved[2], at::kFloat), adv = kind.per_row(saved[3], at::kFloat);
+        const Tensor valid = kind.per_row(saved[4], saved[4].defined() && saved[4].scalar_type() == at::kBool ? at::kBool : at::kByte), ref_logp = kind.per_row(saved[6], at::kFloat);
         const Tensor work = ctx->saved_data["work"].toTensor(), scale = d[0].contiguous();
         Tensor d_logits = ctx->saved_data["d_logits"].toTensor();
         ctx->saved_data["d_logits"] = Tensor();
         const int64_t capture = ctx->saved_data["capture"].toInt();
         const bool held = d_logits.defined() && capture >= 0 && capture == procgen_amd_capture_id(stream_of(logits));
         if (!held) d_logits = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
-        const procgen_amd_rows a = rows_of(logits, p.at, saved[1], d_logits, work);
-        procgen_amd_policy q = policy_of(p, saved[2], saved[3], saved[4], ref_logits, saved[6]);
+        const procgen_amd_rows a = rows_of(logits, p.at, actions, d_logits, work);
+        procgen_amd_policy q = policy_of(p, old, adv, valid, ref_logits, ref_logp);
         q.scale = data_as<float>(scale);
         q.resume = held ? 3 : 1;
         check(procgen_amd_policy_loss(&a, &q, logits.get_device(), stream_of(logits)), "policy_loss");
