@@ -32,7 +32,7 @@ struct procgen_amd_array3 {
  * Where first is set the old state and the gate are not looked at, whatever they hold.  Products of neighbouring gates are formed on the way: where one
  * passes float's range, h behind it is not finite.
  * state, state_out: float [N][D], contiguous; state_out may be state (updated in place), or NULL.  checkpoints: NULL, or float
- * [procgen_amd_recurrence_checkpoints(T)][N][D], which the backward pass reads.  summaries: workspace of
+ * [procgen_amd_recurrence_checkpoints(T)][N][D], which the backward pass reads (it does not read state).  workspace: memory of
  * procgen_amd_recurrence_workspace(T, N, D) bytes (NULL when that is 0). */
 struct procgen_amd_recurrence {
     int dtype;                                    /* of gate, update, h and their gradients */

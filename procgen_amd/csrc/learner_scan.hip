@@ -397,7 +397,7 @@ struct FewSteps {
     const Chain<VEC> ch;
     float a[FEW][VEC], b[FEW][VEC], x[VEC];
     bool cut[FEW];
-    __device__ explicit FewSteps(const procgen_amd_recurrence &p) : ch(blockIdx.x * blockDim.x + threadIdx.x, p.N, p.D) {
+    __device__ FewSteps(const procgen_amd_recurrence &p, const float *state) : ch(blockIdx.x * blockDim.x + threadIdx.x, p.N, p.D) {
         const Column<E, VEC, FEW> gate(p.gate, ch), update(p.update, ch);
         const Flags first(p.first, p.first_t_stride, p.first_n_stride, ch.n, gate.base);
         Raw<E, VEC> ra[FEW], rb[FEW];
@@ -405,7 +405,7 @@ struct FewSteps {
         gate.load(ra, 0, p.T - 1);
         update.load(rb, 0, p.T - 1);
         first.load(rf, 0, p.T - 1);
-        load_state<VEC>(x, p.state, ch);
+        load_state<VEC>(x, state, ch);
         convert<E, VEC, FEW>(a, ra, 0, p.T, 1.f);
         convert<E, VEC, FEW>(b, rb, 0, p.T, 0.f);
         convert(cut, rf, first.mask, 0, p.T);
@@ -413,7 +413,7 @@ struct FewSteps {
 };
 template <class E, int VEC>
 __global__ __launch_bounds__(256) void recurrence_few_forward(procgen_amd_recurrence p) {
-    FewSteps<E, VEC> s(p);
+    FewSteps<E, VEC> s(p, p.state);
     const Column<E, VEC, FEW> out(p.h, s.ch);
     if (p.checkpoints) store_state<VEC>(p.checkpoints, s.x, s.ch);
 #pragma unroll
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(256) void recurrence_few_forward(procgen_amd_recurr
 }
 template <class E, int VEC>
 __global__ __launch_bounds__(256) void recurrence_few_backward(procgen_amd_recurrence p) {
-    FewSteps<E, VEC> s(p);
+    FewSteps<E, VEC> s(p, p.checkpoints);  // the only one: the state that the window began in
     const bool any = p.d_h.data;
     const Column<E, VEC, FEW> d_h(any ? p.d_h : p.gate, s.ch), d_gate(p.d_gate, s.ch), d_update(p.d_update, s.ch);
     Raw<E, VEC> rd[FEW];
