@@ -895,7 +895,7 @@ __global__ __launch_bounds__(MEANS) void policy_means(procgen_amd_policy q, long
 // ---- launches ------------------------------------------------------------------------------------------------------------------------------------
 
 bool rows_ok(const procgen_amd_rows *p) {
-    return p && known_dtype(p->dtype) && p->rows >= 0 && p->rows <= 0x7fffff00ll && p->columns >= 1 && p->columns <= 0x7ffffff0ll - (1 << 18) && p->inner >= 1;
+    return p && known_dtype(p->dtype) && p->rows >= 0 && p->rows <= 0x7fffff00ll && p->columns >= 1 && p->columns <= 0x7ffffff0ll - (1 << 18) && p->inner >= 1 && p->inner <= 0x7fffff00ll;  // rows are divided by inner in 32 bits
 }
 
 template <int I>
