@@ -6,6 +6,7 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/procgen_amd_learner.h"
@@ -31,6 +32,18 @@ void *stream_of(const Tensor &x) { return c10::hip::getCurrentHIPStream(x.get_de
 int dtype_of(const Tensor &x) { return x.scalar_type() == at::kFloat ? PROCGEN_AMD_F32 : x.scalar_type() == at::kHalf ? PROCGEN_AMD_F16 : PROCGEN_AMD_BF16; }
 void check(int rc, const char *name) {
     if (rc) throw std::runtime_error(std::string(name) + (rc < 0 ? ": the library refused the arguments" : ": HIP error " + std::to_string(rc)));
+}
+
+// What torch would have to carry on beside the values is refused: no formula of a tangent is here, and a trace would hold the allocations alone
+void values_only(std::initializer_list<const Tensor *> all) {
+    if (torch::jit::tracer::isTracing()) throw std::invalid_argument("the learner operators cannot be traced");
+    for (const Tensor *x : all)
+        if (x->defined() && x->_fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+            throw std::invalid_argument("the learner operators have no forward-mode derivatives: an input has a tangent");
+}
+const Tensor *in(const Maybe &x) {
+    static const Tensor none;
+    return x.has_value() ? &*x : &none;
 }
 
 // gradients of a backward pass that is itself recorded (create_graph): they are right, and differentiating them is an error
@@ -120,6 +133,7 @@ struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
 };
 
 std::pair<Tensor, Tensor> gated_recurrence(const Tensor &gate, const Tensor &update, const Maybe &first_, const Maybe &state_, const Maybe &state_out_) {
+    values_only({&gate, &update, in(state_), in(state_out_)});
     const Maybe state = contiguous(state_);
     if (!wants_grad(gate) && !wants_grad(update) && !(state && wants_grad(*state)))
         return recurrence_forward(gate, update, or_none(first_), or_none(state), or_none(state_out_), Tensor());
@@ -128,6 +142,7 @@ std::pair<Tensor, Tensor> gated_recurrence(const Tensor &gate, const Tensor &upd
 }
 
 std::pair<Tensor, Tensor> advantages(const Tensor &rew, const Tensor &values, const Tensor &first, double gamma, double lam) {
+    values_only({&rew, &values});
     const int T = (int)rew.size(0), N = (int)rew.size(1);
     Tensor adv = floats({T, N}, rew), ret = floats({T, N}, rew), work = bytes(procgen_amd_recurrence_workspace(T, N, 1), rew);
     procgen_amd_advantage a = {};
@@ -217,6 +232,7 @@ struct ActionLogprobs : torch::autograd::Function<ActionLogprobs> {
 };
 
 std::pair<Tensor, Tensor> action_logprobs(const Tensor &logits, const Tensor &actions_, int64_t inner, int64_t outer_stride, int64_t inner_stride) {
+    values_only({&logits});
     const Layout at{inner, outer_stride, inner_stride};
     const Tensor actions = actions_.contiguous();
     if (wants_grad(logits)) {
@@ -310,6 +326,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
 std::pair<Tensor, Tensor> policy_loss(const Tensor &logits, const Tensor &actions_, const Tensor &old_, const Tensor &adv_, const Maybe &valid_, const Maybe &ref_logits_,
                                       const Maybe &ref_logp_, double clip_low, double clip_high, double kl_coef, double entropy_coef, int64_t inner, int64_t outer_stride,
                                       int64_t inner_stride, int64_t ref_outer_stride, int64_t ref_inner_stride) {
+    values_only({&logits, &old_, &adv_, in(ref_logits_), in(ref_logp_)});
     const PolicyArgs p{{inner, outer_stride, inner_stride}, {inner, ref_outer_stride, ref_inner_stride}, clip_low, clip_high, kl_coef, entropy_coef};
     const Tensor actions = actions_.contiguous(), old = old_.contiguous(), adv = adv_.contiguous();
     const Maybe valid = contiguous(valid_), ref_logp = contiguous(ref_logp_);

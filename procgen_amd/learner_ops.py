@@ -12,6 +12,7 @@ already are.  Entry points of libenv.so (include/procgen_amd_learner.h), reached
 Every operator runs on the current stream of its tensors' device, does not synchronise, keeps nothing between calls and can be captured into a graph.
 Tensors may be strided (batch-major windows, slices, expanded dimensions); arguments that an operator does not take raise TypeError or ValueError
 before anything runs.  Element types: float32, float16, bfloat16; sums, states and statistics are held in 32 bits or more.
+Gradients are reverse-mode ones of the first order: a tensor with a forward-mode tangent and a call that is being traced are refused, too.
 """
 import importlib.util
 import os

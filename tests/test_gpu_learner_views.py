@@ -1,0 +1,59 @@
+"""GPU: ways of calling the learner operators that torch records beside the values -- tangents, traces, lazy negation."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+from test_gpu_learner_ops import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def inputs():
+    g = torch.Generator().manual_seed(0)
+    x = {k: torch.randn(s, generator=g).cuda() for k, s in {"gate": (6, 3, 4), "update": (6, 3, 4), "state": (3, 4), "rew": (6, 3), "values": (7, 3), "logits": (6, 3, 5), "ref_logits": (6, 3, 5),
+                                                            "old": (6, 3), "adv": (6, 3), "ref_logprobs": (6, 3)}.items()}
+    x["first"] = torch.zeros((7, 3), dtype=torch.uint8, device="cuda")
+    x["actions"] = torch.zeros((6, 3), dtype=torch.int32, device="cuda")
+    return x
+
+
+CALLS = {
+    "recurrence": (lambda x: ops().gated_recurrence(x["gate"], x["update"], x["first"][:-1], x["state"])[0], ["gate", "update", "state"]),
+    "advantages": (lambda x: ops().advantages(x["rew"], x["values"], x["first"], gamma=0.9, lam=0.9)[0], ["rew", "values"]),
+    "logprobs": (lambda x: ops().action_logprobs(x["logits"], x["actions"])[0], ["logits"]),
+    "loss": (lambda x: ops().policy_loss(x["logits"], x["actions"], x["old"], x["adv"], ref_logits=x["ref_logits"], kl_coef=0.1).loss, ["logits", "old", "adv", "ref_logits"]),
+    "loss, estimator": (lambda x: ops().policy_loss(x["logits"], x["actions"], x["old"], x["adv"], ref_logprobs=x["ref_logprobs"], kl_coef=0.1).loss, ["ref_logprobs"]),
+}
+EACH = [(call, name) for call, (_, names) in CALLS.items() for name in names]
+
+
+@pytest.mark.parametrize("call,name", EACH)
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_refused_and_not_dropped(call, name, requires_grad):
+    x = inputs()
+    if requires_grad and name in ("gate", "update", "state", "logits"):
+        x[name].requires_grad_()
+    with fw.dual_level():
+        x[name] = fw.make_dual(x[name], torch.ones_like(x[name]))
+        with pytest.raises(ValueError, match="forward-mode"):
+            CALLS[call][0](x)
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            CALLS[call][0](x)
+    CALLS[call][0](inputs())
+
+
+def test_a_state_out_with_a_tangent_is_refused():
+    x = inputs()
+    with torch.no_grad(), fw.dual_level():
+        out = fw.make_dual(torch.zeros((3, 4), device="cuda"), torch.ones((3, 4), device="cuda"))
+        with pytest.raises(ValueError, match="forward-mode"):
+            ops().gated_recurrence(x["gate"], x["update"], state_out=out)
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_tracing_is_refused_and_does_not_record_empty_outputs(call):
+    x = inputs()
+    name = CALLS[call][1][0]
+    with pytest.raises(ValueError, match="traced"):
+        torch.jit.trace(lambda v: CALLS[call][0]({**x, name: v}), x[name], check_trace=False)
+    CALLS[call][0](x)
