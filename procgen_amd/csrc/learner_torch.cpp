@@ -23,6 +23,7 @@ template <class T>
 T *data_as(const Tensor &x) {
     return (T *)data(x);
 }
+Tensor grad_of(const Tensor &x) { return x.defined() ? x.resolve_neg() : x; }  // a gradient coming in may be a view that is negated when it is read
 Tensor or_none(const Maybe &x) { return x.has_value() ? *x : Tensor(); }
 Maybe contiguous(const Maybe &x) { return x.has_value() ? Maybe(x->contiguous()) : x; }
 bool wants_grad(const Tensor &x) { return at::GradMode::is_enabled() && x.requires_grad(); }
@@ -61,7 +62,7 @@ variable_list once(variable_list out) {
 // What a backward pass got back of the tensors that were saved.  Hooks (torch.autograd.graph.saved_tensors_hooks) may have kept them elsewhere meanwhile:
 // other strides are taken, anything else would be read as what it is not.
 void came_back(const Tensor &x, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
-    if (!x.defined() || x.sizes() != sizes || x.scalar_type() != type || x.device() != device || x.layout() != at::kStrided)
+    if (!x.defined() || x.sizes() != sizes || x.scalar_type() != type || x.device() != device || x.layout() != at::kStrided || x.is_neg())
         throw std::runtime_error("a saved tensor came back from its hooks with another shape, type or device than it was saved with");
 }
 // one that was contiguous, or undefined
@@ -120,11 +121,11 @@ struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
         came_back(update, shape, (at::ScalarType)s[3], device);
         if (first.defined()) came_back(first, {s[0], s[1]}, (at::ScalarType)s[4], device);
         const Tensor state = dense(saved[3], {s[1], s[2]}, at::kFloat, device), checkpoints = dense(saved[4], checks, at::kFloat, device);
-        Tensor work = recurrence_workspace(gate), d_last = d[1].defined() ? d[1].contiguous() : Tensor();
+        Tensor work = recurrence_workspace(gate), d_h = grad_of(d[0]), d_last = d[1].defined() ? grad_of(d[1]).contiguous() : Tensor();
         Tensor d_gate = ctx->needs_input_grad(0) ? at::empty_like(gate) : Tensor(), d_update = ctx->needs_input_grad(1) ? at::empty_like(update) : Tensor();
         Tensor d_state = state.defined() && ctx->needs_input_grad(first.defined() ? 3 : 2) ? at::empty_like(state) : Tensor();
         procgen_amd_recurrence a = recurrence(gate, update, first, state, checkpoints, work);
-        a.d_h = array3(d[0]), a.d_gate = array3(d_gate), a.d_update = array3(d_update);
+        a.d_h = array3(d_h), a.d_gate = array3(d_gate), a.d_update = array3(d_update);
         a.d_state_out = data_as<float>(d_last);
         a.d_state = data_as<float>(d_state);
         check(procgen_amd_recurrence_backward(&a, gate.get_device(), stream_of(gate)), "gated_recurrence");
@@ -222,7 +223,7 @@ struct ActionLogprobs : torch::autograd::Function<ActionLogprobs> {
         const Tensor logits = kind.matrix(saved[0], ctx->saved_data["strides"].toIntVector(), &at), actions = kind.per_row(saved[1], kind.actions);
         const Tensor lse = dense(saved[2], {actions.numel(), 2}, at::kFloat, kind.device), entropy = kind.per_row(saved[3], at::kFloat);
         Tensor d_logits = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
-        Tensor d_logp = d[0].defined() ? d[0].contiguous() : Tensor(), d_entropy = d[1].defined() ? d[1].contiguous() : Tensor();
+        Tensor d_logp = d[0].defined() ? grad_of(d[0]).contiguous() : Tensor(), d_entropy = d[1].defined() ? grad_of(d[1]).contiguous() : Tensor();
         const procgen_amd_rows a = rows_of(logits, at, actions, d_logits, Tensor());
         check(procgen_amd_action_logprobs_backward(&a, data_as<procgen_amd_lse>(lse), data_as<float>(entropy), data_as<float>(d_logp), data_as<float>(d_entropy), logits.get_device(),
                                                    stream_of(logits)),
@@ -308,7 +309,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         }
         const Tensor actions = kind.per_row(saved[1], kind.actions), old = kind.per_row(saved[2], at::kFloat), adv = kind.per_row(saved[3], at::kFloat);
         const Tensor valid = kind.per_row(saved[4], saved[4].defined() && saved[4].scalar_type() == at::kBool ? at::kBool : at::kByte), ref_logp = kind.per_row(saved[6], at::kFloat);
-        const Tensor work = ctx->saved_data["work"].toTensor(), scale = d[0].contiguous();
+        const Tensor work = ctx->saved_data["work"].toTensor(), scale = grad_of(d[0]).contiguous();
         Tensor d_logits = ctx->saved_data["d_logits"].toTensor();
         ctx->saved_data["d_logits"] = Tensor();
         const int64_t capture = ctx->saved_data["capture"].toInt();

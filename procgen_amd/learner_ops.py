@@ -50,6 +50,8 @@ def _tensor(x, what, dtypes, shape=None):
         raise TypeError(f"{what} has to be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, not {x.dtype}")
     if shape is not None and x.shape != shape:
         raise ValueError(f"{what} has to have the shape {tuple(shape)}, not {tuple(x.shape)}")
+    if x.is_neg():
+        raise ValueError(f"{what} is a view that torch negates when it reads it, and the kernels do not: resolve_neg() it")
 
 
 def _on_gpu(x, *others):

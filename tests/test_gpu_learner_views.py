@@ -57,3 +57,42 @@ def test_tracing_is_refused_and_does_not_record_empty_outputs(call):
     with pytest.raises(ValueError, match="traced"):
         torch.jit.trace(lambda v: CALLS[call][0]({**x, name: v}), x[name], check_trace=False)
     CALLS[call][0](x)
+
+
+def lazily_negated(x):
+    """the same values behind a view that torch negates when it reads it"""
+    y = torch.complex(torch.zeros_like(x), -x).conj().imag
+    assert y.is_neg() and torch.equal(y.resolve_neg(), x)
+    return y
+
+
+@pytest.mark.parametrize("call,name", EACH)
+def test_lazily_negated_inputs_are_refused(call, name):
+    x = inputs()
+    x[name] = lazily_negated(x[name])
+    with pytest.raises(ValueError, match="resolve_neg"):
+        CALLS[call][0](x)
+    x[name] = x[name].resolve_neg()
+    assert torch.equal(CALLS[call][0](x), CALLS[call][0](inputs()))
+
+
+def test_a_lazily_negated_state_out_is_refused():
+    x = inputs()
+    with torch.no_grad(), pytest.raises(ValueError, match="resolve_neg"):
+        ops().gated_recurrence(x["gate"], x["update"], state_out=lazily_negated(x["state"]))
+
+
+def test_lazily_negated_gradients_are_taken_as_their_values():
+    x = inputs()
+    g = torch.Generator().manual_seed(1)
+    for k in ("gate", "update", "state", "logits"):
+        x[k].requires_grad_()
+    runs = [(lambda: ops().gated_recurrence(x["gate"], x["update"], None, x["state"]), ["gate", "update", "state"]), (lambda: ops().action_logprobs(x["logits"], x["actions"]), ["logits"]),
+            (lambda: ops().policy_loss(x["logits"], x["actions"], x["old"], x["adv"])[:1], ["logits"])]
+    for run, names in runs:
+        leaves = [x[k] for k in names]
+        out = run()
+        d = [torch.randn(v.shape, generator=g).cuda() for v in out]
+        want = torch.autograd.grad(out, leaves, d)
+        got = torch.autograd.grad(run(), leaves, [lazily_negated(v) for v in d])
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
