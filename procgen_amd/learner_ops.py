@@ -27,7 +27,10 @@ class _Extension:
     """csrc/learner_torch.cpp, loaded when an operator first runs"""
 
     def __getattr__(self, name):
-        spec = importlib.util.spec_from_file_location("learner_torch", os.path.join(DEFAULT_LIB_DIR, "learner_torch.so"))
+        path = os.path.join(DEFAULT_LIB_DIR, "learner_torch.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is not there: make in procgen_amd/csrc builds it, where a torch with ROCm's headers is installed")
+        spec = importlib.util.spec_from_file_location("learner_torch", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         for fn in ("gated_recurrence", "advantages", "action_logprobs", "policy_loss"):
