@@ -160,7 +160,7 @@ struct Coef {
 // Each operator's rows: what it fetches for a row besides its logits, whether it wants the row at all, what it makes of the row's sums.  finish() is
 // called once per row by one lane at least, with `first` set in exactly one; it returns whether the row's gradient is anything but zero.
 struct Logprobs {
-    static constexpr bool GRADIENT = false, HEAVY = false;
+    static constexpr bool GRADIENT = false, HEAVY = false, LONG = true;
     __device__ bool done() const { return false; }
     float *logp, *entropy;
     procgen_amd_lse *lse;
@@ -179,8 +179,8 @@ struct Logprobs {
     }
 };
 
-struct LogprobsBackward {  // of rows short enough to sum up again
-    static constexpr bool GRADIENT = true, HEAVY = false;
+struct LogprobsBackward {  // of rows short enough to sum up again: 256 chunks, which the 64 lanes of a wave hold
+    static constexpr bool GRADIENT = true, HEAVY = false, LONG = false;
     __device__ bool done() const { return false; }
     const float *d_logp, *d_entropy;
     struct In {
@@ -198,7 +198,7 @@ struct LogprobsBackward {  // of rows short enough to sum up again
 };
 
 struct Policy {
-    static constexpr bool GRADIENT = true, HEAVY = true;  // HEAVY: a row's own numbers, its sums and their addresses keep some 30 registers more
+    static constexpr bool GRADIENT = true, HEAVY = true, LONG = true;  // HEAVY: a row's own numbers, its sums and their addresses keep some 30 registers more
     __device__ bool done() const { return (q.resume & 2) && *q.scale == 1.f; }  // the gradient that is there is the one that is wanted
     procgen_amd_policy q;
     const long long *counts;
@@ -916,14 +916,18 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
     // A lane per row, where its registers leave enough waves.  Over 64 M columns in all, against the groups: 16-bit 17 columns 81 : 190 us, 32 60 : 96,
     // 33 83 : 160, 48 62 : 86, 63 68 : 113, but 64 152 : 68, with a reference 32 98 : 150, but 33 291 : 225; float32 16 107 : 171, 24 110 : 143, 31 109 : 189,
     // 32 107 : 127, with a reference 16 160 : 203, 24 156 : 168, 25 169 : 203, 31 149 : 201, but 32 314 : 141.
-    const bool lane_per_row = p.columns <= (SIZE == 2 ? (REF ? 32 : 63) : REF ? 31 : 32);
+    constexpr int LANE_A_ROW = SIZE == 2 ? (REF ? 32 : 63) : REF ? 31 : 32;
     // with a gradient, float32 goes in chunks of as many values as 16 bits do: loss of 16000 columns 133 -> 122 us, with a reference 153 -> 119
     constexpr int MORE = Op::GRADIENT && SIZE == 4 ? 2 : 1;
     auto group = [&](auto lanes, auto chunks) {  // whether a row fits, and if so the launch
         constexpr int G = decltype(lanes)::value, CH = decltype(chunks)::value;
-        if (padded > G * CH * N) return false;
-        group_rows<E, G, CH, REF, Op><<<grid(BLOCK / G, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-        return true;
+        if constexpr (G * CH * N > LANE_A_ROW) {
+            if (padded <= G * CH * N) {
+                group_rows<E, G, CH, REF, Op><<<grid(BLOCK / G, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+                return true;
+            }
+        }
+        return false;
     };
     auto groups = [&](auto lanes) { return group(lanes, Const<3>()) || group(lanes, Const<4>()) || group(lanes, Const<5>()); };
     const bool apart = p.inner != 1 || p.outer_stride != p.columns || (REF && ref_outer != p.columns);
@@ -935,7 +939,7 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
         if (apart) short_rows<E, MOST, REF, Op, TURN, true><<<n, BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
         else short_rows<E, MOST, REF, Op, TURN, false><<<n, BLOCK, lds, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     };
-    if (lane_per_row) {
+    if (p.columns <= LANE_A_ROW) {
         const std::integral_constant<bool, false> straight;
         const std::integral_constant<bool, SIZE == 4> turned;
         if (p.columns <= 8) lanes(Const<8>(), straight);
@@ -949,12 +953,14 @@ int launch_rows(const procgen_amd_rows &p, const Op &op, const void *ref, long l
             if (p.columns <= 48) lanes(Const<48>(), straight);
             else lanes(Const<64>(), straight);
         }
-    } else if (group(Const<4>(), Const<1>()) || group(Const<4>(), Const<2>()) || groups(Const<4>()) || groups(Const<8>()) || groups(Const<16>()) || groups(Const<32>()) ||
-               groups(Const<64>()) || group(Const<128>(), Const<3>()) || group(Const<64>(), Const<8>()) || (p.rows >= 2 * CUS && (group(Const<128>(), Const<5>()) || groups(Const<256>())))) {
+    } else if (group(Const<4>(), Const<2>()) || groups(Const<4>()) || groups(Const<8>()) || groups(Const<16>()) || groups(Const<32>()) || groups(Const<64>())) {
+    } else if constexpr (!Op::LONG) {
+        return -1 - (int)hipErrorInvalidValue;
+    } else if (group(Const<128>(), Const<3>()) || group(Const<64>(), Const<8>()) || (p.rows >= 2 * CUS && (group(Const<128>(), Const<5>()) || groups(Const<256>())))) {
     } else if (p.columns <= 256 * 2 * N || (p.rows >= 2 * CUS && !(REF && p.d_logits))) {
         long_rows<E, 256, 2 * MORE, REF, Op><<<grid(1, CUS * 4), BLOCK, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
-    } else if (p.rows >= 2 * CUS) {  // 2048 x 50021 bf16 with a reference: 154 us, against 173 with 256 lanes and two chunks, 179 with 1024
-        long_rows<E, 512, MORE, REF, Op><<<grid(1, CUS * 2), 512, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
+    } else if (REF && p.rows >= 2 * CUS) {  // 2048 x 50021 bf16 with a reference: 154 us, against 173 with 256 lanes and two chunks, 179 with 1024
+        if constexpr (REF) long_rows<E, 512, MORE, REF, Op><<<grid(1, CUS * 2), 512, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     } else {  // too few rows to fill the card: more lanes for each
         long_rows<E, 1024, 2, REF, Op><<<grid(1, CUS), 1024, 0, stream>>>(p, op, ref, ref_outer, ref_inner, partial);
     }

@@ -621,12 +621,13 @@ int vec_for(const procgen_amd_recurrence *a, bool backward) {
 }
 // fn(VEC, WAVES): a window in segments has too few chains for more than one a lane.  With one a lane eight waves: 1024 x 64 x 512 bf16 forward 53 us,
 // backward 109, with four 66 and 126
-template <class Fn>
+template <int MOST, class Fn>
 int by_shape(const Segments &g, int vec, Fn fn) {
     typedef std::integral_constant<int, 1> One;
     const std::integral_constant<int, W1> waves;
     switch (g.count > 1 ? 1 : vec) {
-        case 4: return fn(std::integral_constant<int, 4>(), waves);
+        case 4:
+            if constexpr (MOST == 4) return fn(std::integral_constant<int, 4>(), waves);
         case 2: return fn(std::integral_constant<int, 2>(), waves);
         default: return fn(One(), std::integral_constant<int, WS>());
     }
@@ -674,12 +675,14 @@ LIBENV_API int procgen_amd_recurrence_forward(const struct procgen_amd_recurrenc
                 recurrence_few_forward<E, decltype(vec)::value><<<blocks, 256, 0, (hipStream_t)stream>>>(*a);
                 return launched();
             });
-        return by_shape(g, vec_for(a, false), [&](auto vec, auto waves) {
+        return by_shape<sizeof(typename E::T) == 2 ? 4 : 2>(g, vec_for(a, false), [&](auto vec, auto waves) {
             constexpr int VEC = decltype(vec)::value, WAVES = decltype(waves)::value;
             const dim3 grid(chain_blocks(a, VEC), g.count), block(WAVE, std::min(WAVES, (a->T + KF - 1) / KF));
-            if (WAVES == WS && g.count > 1) {
-                recurrence_segments<E, VEC, WAVES, false><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
-                if (int err = launched()) return err;
+            if constexpr (VEC == 1) {
+                if (g.count > 1) {
+                    recurrence_segments<E, VEC, WAVES, false><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
+                    if (int err = launched()) return err;
+                }
             }
             recurrence_forward<E, VEC, WAVES><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
             return launched();
@@ -702,12 +705,14 @@ LIBENV_API int procgen_amd_recurrence_backward(const struct procgen_amd_recurren
                 recurrence_few_backward<E, decltype(vec)::value><<<blocks, 256, 0, (hipStream_t)stream>>>(*a);
                 return launched();
             });
-        return by_shape(g, vec_for(a, true), [&](auto vec, auto waves) {
-            constexpr int VEC = std::min(2, decltype(vec)::value), WAVES = decltype(waves)::value;
+        return by_shape<2>(g, vec_for(a, true), [&](auto vec, auto waves) {
+            constexpr int VEC = decltype(vec)::value, WAVES = decltype(waves)::value;
             const dim3 grid(chain_blocks(a, VEC), g.count), block(WAVE, std::min(WAVES, (a->T + KB - 1) / KB));
-            if (WAVES == WS && g.count > 1) {
-                recurrence_segments<E, VEC, WAVES, true><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
-                if (int err = launched()) return err;
+            if constexpr (VEC == 1) {
+                if (g.count > 1) {
+                    recurrence_segments<E, VEC, WAVES, true><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
+                    if (int err = launched()) return err;
+                }
             }
             recurrence_backward<E, VEC, WAVES><<<grid, block, 0, (hipStream_t)stream>>>(*a, g);
             return launched();

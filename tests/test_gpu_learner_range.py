@@ -29,12 +29,12 @@ def gradient_64(w, actions, d_logp, d_entropy):
     return want, tol
 
 
-def compare(x, actions, seed, ref=None):
+def compare(x, actions, seed, ref=None, layout="plain"):
     """the three calls on rows x [B, A] (on the GPU, at any size) against their definitions in 64 bits"""
     B, A = x.shape
     g = gen(seed)
     w = Rows64(x)
-    t = x.detach().clone().requires_grad_()
+    t = put_rows(x.detach(), layout).requires_grad_()
     logp, entropy = ops().action_logprobs(t, actions)
     check(logp, pick(w.logp, actions).cpu(), pick(w.T_logp, actions).cpu(), "log-probabilities")
     check(entropy, w.H.cpu(), w.T_H.cpu(), "entropy")
@@ -125,6 +125,23 @@ def test_shifted_rows_keep_their_precision(A, repeat, dtype, shift):
     x = (2 * torch.randn((10 * repeat, A), generator=g) + shift).to(DTYPES[dtype])
     actions = torch.randint(0, A, (x.shape[0],), generator=g)
     compare(x.cuda(), actions.cuda(), 10, (x.float() + 0.3 * torch.randn(x.shape, generator=g)).to(x.dtype).cuda())
+
+
+def edges(size):
+    """columns around which another number of lanes and chunks, or another kernel, takes a row: of 16-byte chunks of `size` values"""
+    few = [4 * size * 2, 4 * size * 3, 4 * size * 5, 8 * size * 3, 16 * size * 5, 64 * size * 3, 256 * size, 64 * size * 5, 64 * size * 8]
+    many = [128 * size * 5, 256 * size * 5]
+    return [(4, a + d) for a in few for d in (-1, 0, 1)] + [(513, a + d) for a in many for d in (0, 1)]
+
+
+@pytest.mark.parametrize("B,A,dtype", [(B, A, "bf16") for B, A in edges(8)] + [(B, A, "f32") for B, A in edges(4)])
+def test_widths_at_which_another_kernel_begins(B, A, dtype):
+    g = gen(A + 5)
+    x = (2 * torch.randn((B, A), generator=g)).to(DTYPES[dtype]).cuda()
+    actions = torch.randint(0, A, (B,), generator=g).cuda()
+    ref = (x.float() + 0.3 * torch.randn((B, A), generator=g).cuda()).to(x.dtype)
+    compare(x, actions, 11, None, "pitch")
+    compare(x, actions, 12, ref)
 
 
 def watched_inputs(B, A, dtype, seed):
