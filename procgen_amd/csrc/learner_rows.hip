@@ -160,7 +160,7 @@ struct Coef {
 // Each operator's rows: what it fetches for a row besides its logits, whether it wants the row at all, what it makes of the row's sums.  finish() is
 // called once per row by one lane at least, with `first` set in exactly one; it returns whether the row's gradient is anything but zero.
 struct Logprobs {
-    static constexpr bool GRADIENT = false, HEAVY = false, LONG = true;
+    static constexpr bool GRADIENT = false, LONG = true;
     __device__ bool done() const { return false; }
     float *logp, *entropy;
     procgen_amd_lse *lse;
@@ -180,7 +180,7 @@ struct Logprobs {
 };
 
 struct LogprobsBackward {  // of rows short enough to sum up again: 256 chunks, which the 64 lanes of a wave hold
-    static constexpr bool GRADIENT = true, HEAVY = false, LONG = false;
+    static constexpr bool GRADIENT = true, LONG = false;
     __device__ bool done() const { return false; }
     const float *d_logp, *d_entropy;
     struct In {
@@ -198,7 +198,7 @@ struct LogprobsBackward {  // of rows short enough to sum up again: 256 chunks, 
 };
 
 struct Policy {
-    static constexpr bool GRADIENT = true, HEAVY = true, LONG = true;  // HEAVY: a row's own numbers, its sums and their addresses keep some 30 registers more
+    static constexpr bool GRADIENT = true, LONG = true;
     __device__ bool done() const { return (q.resume & 2) && *q.scale == 1.f; }  // the gradient that is there is the one that is wanted
     procgen_amd_policy q;
     const long long *counts;
@@ -399,7 +399,14 @@ template <class E, int MOST>
 __host__ __device__ constexpr int short_tile(int columns) {
     return ((WAVE * columns * (int)sizeof(typename E::T) + 15) & ~15) + MOST * (int)sizeof(typename E::T);
 }
-// blocks of four waves that a compute unit holds: by registers (three, or four with a reference, for each of MOST columns) and by LDS
+// blocks of four waves that a compute unit holds: by registers (three, or four with a reference, for each of MOST columns) and by LDS.  Loss of 64 M bf16 (32 M float32)
+// logits in us with one block less : these : one more, which spills:
+//   columns          4                8               15               24               31              48              63
+//   bf16       155:143:140       87:83:83       89:77:124        76:63:124        92:74:114      113:73:111      115:76:142
+//     reference 256:225:205   140:124:114     149:120:166      181:110:124      176:114:203
+//   float32      93:87:84         69:67:69        66:57:85         71:61:77         88:62:65
+//     reference 145:122:119      101:92:94       93:85:152       125:94:156      113:88:278
+// (16 float32 with a reference, two blocks: 134:89:86.)  The gradient of log-probabilities alone would take one more up to 16 columns (15 bf16 67:62, 31 float32 54:50).
 template <class E, int MOST, bool REF, bool TURN = false>
 constexpr int short_residents() {
     return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? (TURN ? 2 : 3) : sizeof(typename E::T) == 4 ? 4 : 5) : MOST <= 24 ? (REF ? 2 : sizeof(typename E::T) == 4 ? 3 : 4) : MOST > 32 || REF || sizeof(typename E::T) == 4 ? 2 : 3;
@@ -451,20 +458,20 @@ __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) voi
         Coef c;
         if (wanted) {
             // the columns that a row has not are -inf; l and l2 become x and y
-            // reads what a row has not and drops it, which keeps the reads together; where registers are short it is not read (15 bf16 67 : 76 us)
+            // reads what a row has not and drops it, which keeps the reads together: loss of 64 M bf16 logits at 9, 15, 16, 24, 32, 63 columns 105, 76, 70, 63, 68, 76 us, with
+            // a branch around each of those reads 104, 77, 74, 66, 77, 85
             constexpr bool AGAIN = MOST > 48 || (REF && MOST > 24 && sizeof(T) == 4);  // exponentials are taken again for the gradient: registers for all of them would be spilled
-            constexpr bool GUARD = Op::HEAVY && MOST == 16 && !REF && sizeof(T) == 2;
             constexpr int surely = TURN ? MOST : MOST > 32 ? MOST - 16 : MOST > 16 ? MOST - 8 : MOST > 8 ? MOST / 2 : 0;
             float l[MOST], e[MOST], l2[REF ? MOST : 1];
             Stats<REF> x;
 #pragma unroll
             for (int j = 0; j < MOST; j++) {
-                l[j] = !GUARD || j <= surely || j < columns ? (float)row[j ^ turn] : -INFINITY;  // of the row behind, or of the tile's slack, where there is no such column
+                l[j] = (float)row[j ^ turn];  // of the row behind, or of the tile's slack, where there is no such column
                 if (REF) l2[j] = (float)row2[j ^ turn];
             }
 #pragma unroll
             for (int j = 0; j < MOST; j++) {
-                if (!GUARD && j > surely && j >= columns) l[j] = l2[REF ? j : 0] = -INFINITY;
+                if (j > surely && j >= columns) l[j] = l2[REF ? j : 0] = -INFINITY;
                 x.m = fmaxf(x.m, l[j]);
                 if (REF) x.m2 = fmaxf(x.m2, l2[j]);
             }
