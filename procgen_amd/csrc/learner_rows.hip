@@ -71,7 +71,7 @@ struct Stats {
         const float d = m == -INFINITY ? 0.f : m - to, c = exp_of(d), d2 = !REF || m2 == -INFINITY ? 0.f : m2 - to2;
         if (REF) {
             u = product(c, product(s, d - d2) + u);
-            s2 = product(exp_of(d2), s2);
+            s2 *= exp_of(d2);  // a NaN stays one
             m2 = to2;
         }
         w = product(c, product(s, d) + w);

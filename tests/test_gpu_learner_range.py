@@ -58,6 +58,14 @@ def rows_of(values, A, dtype, repeat):
     return torch.tensor(values, dtype=torch.float64).clamp(torch.finfo(DTYPES[dtype]).min, torch.finfo(DTYPES[dtype]).max).to(DTYPES[dtype])[:, None].repeat(repeat, A).cuda()
 
 
+def watched_inputs(B, A, dtype, seed):
+    g = gen(seed)
+    x = (2 * torch.randn((B, A), generator=g)).to(DTYPES[dtype])
+    actions = torch.randint(0, A, (B,), generator=g)
+    old = (pick(Rows64(x).logp, actions) - 0.05 * torch.rand((B,), generator=g) - 0.01).float()
+    return g, x, actions, old, torch.randn((B,), generator=g)
+
+
 @pytest.mark.parametrize("A,repeat", WIDTHS)
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_rows_of_one_value(A, repeat, dtype):
@@ -127,6 +135,28 @@ def test_shifted_rows_keep_their_precision(A, repeat, dtype, shift):
     compare(x.cuda(), actions.cuda(), 10, (x.float() + 0.3 * torch.randn(x.shape, generator=g)).to(x.dtype).cuda())
 
 
+@pytest.mark.parametrize("A,repeat", WIDTHS[1:])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_nan_in_the_reference_is_not_lost(A, repeat, dtype):
+    """among columns so far below the reference's largest that their exponentials are zero, and with the policy's share there zero too"""
+    B = 4 * (1 if repeat == 1 else 130)
+    g, x, actions, old, adv = watched_inputs(B, A, dtype, A + 6)
+    ref = x.clone()
+    ref[1::4, :A // 2] = -300.0
+    ref[1::4, 0] = float("nan")
+    x[2::4, :A // 2] = ref[2::4, :A // 2] = -300.0
+    ref[2::4, 0] = float("nan")
+    actions[2::4] = A - 1
+    old[2::4] = (pick(Rows64(x).logp, actions) - 0.05).float()[2::4]
+    t = x.cuda().requires_grad_()
+    out = ops().policy_loss(t, actions.cuda(), old.cuda(), adv.cuda(), kl_coef=0.3, ref_logits=ref.cuda())
+    (d,) = torch.autograd.grad(out.loss, t)
+    assert out.loss.isnan() and out.stats[1].isnan() and not out.stats[[0, 2, 3]].isnan().any()
+    for r in range(B):
+        held = d[r, A // 2:]  # where the policy has no share its gradient is zero, whatever it is multiplied with
+        assert held.isnan().all() if r % 4 in (1, 2) else d[r].isfinite().all(), r
+
+
 def edges(size):
     """columns around which another number of lanes and chunks, or another kernel, takes a row: of 16-byte chunks of `size` values"""
     few = [4 * size * 2, 4 * size * 3, 4 * size * 5, 8 * size * 3, 16 * size * 5, 64 * size * 3, 256 * size, 64 * size * 5, 64 * size * 8]
@@ -142,14 +172,6 @@ def test_widths_at_which_another_kernel_begins(B, A, dtype):
     ref = (x.float() + 0.3 * torch.randn((B, A), generator=g).cuda()).to(x.dtype)
     compare(x, actions, 11, None, "pitch")
     compare(x, actions, 12, ref)
-
-
-def watched_inputs(B, A, dtype, seed):
-    g = gen(seed)
-    x = (2 * torch.randn((B, A), generator=g)).to(DTYPES[dtype])
-    actions = torch.randint(0, A, (B,), generator=g)
-    old = (pick(Rows64(x).logp, actions) - 0.05 * torch.rand((B,), generator=g) - 0.01).float()
-    return g, x, actions, old, torch.randn((B,), generator=g)
 
 
 @pytest.mark.parametrize("A,repeat", WIDTHS)
