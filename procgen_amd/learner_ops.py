@@ -16,6 +16,7 @@ Gradients are reverse-mode ones of the first order: a tensor with a forward-mode
 """
 import importlib.util
 import os
+import threading
 from typing import NamedTuple
 
 import torch
@@ -26,7 +27,18 @@ from .env import DEFAULT_LIB_DIR
 class _Extension:
     """csrc/learner_torch.cpp, loaded when an operator first runs"""
 
+    def __init__(self):
+        self._loading = threading.Lock()  # several threads may be the first
+
     def __getattr__(self, name):
+        with self._loading:
+            if name not in self.__dict__:
+                self._load()
+        if name not in self.__dict__:
+            raise AttributeError(name)
+        return self.__dict__[name]
+
+    def _load(self):
         path = os.path.join(DEFAULT_LIB_DIR, "learner_torch.so")
         if not os.path.exists(path):
             raise ImportError(f"{path} is not there: make in procgen_amd/csrc builds it, where a torch with ROCm's headers is installed")
@@ -35,7 +47,6 @@ class _Extension:
         spec.loader.exec_module(module)
         for fn in ("gated_recurrence", "advantages", "action_logprobs", "policy_loss"):
             setattr(self, fn, getattr(module, fn))
-        return self.__dict__[name]
 
 
 _ext = _Extension()

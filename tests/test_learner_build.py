@@ -46,3 +46,24 @@ else:
     raise SystemExit("loaded from nowhere")"""
     r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PROCGEN_AMD_LIB_DIR": str(tmp_path)}, stderr=subprocess.PIPE, text=True)
     assert r.returncode == 0, r.stderr
+
+
+@pytest.mark.skipif(not os.path.exists(os.path.join(CSRC, "build", "learner_torch.so")), reason="learner_torch.so not built (run __graft_entry__.build())")
+def test_host_threads_may_be_the_first_to_call():
+    """all of them at once: each finds every operator"""
+    code = f"""import sys, threading; sys.path.insert(0, {REPO!r}); sys.setswitchinterval(1e-6)
+from procgen_amd import learner_ops
+start, errors = threading.Barrier(16), []
+def call():
+    start.wait()
+    try:
+        learner_ops._ext.policy_loss
+    except Exception as e:
+        errors.append(e)
+threads = [threading.Thread(target=call) for _ in range(16)]
+for t in threads: t.start()
+for t in threads: t.join()
+raise SystemExit(repr(errors) if errors else 0)"""
+    for _ in range(5):
+        r = subprocess.run([sys.executable, "-c", code], stderr=subprocess.PIPE, text=True)
+        assert r.returncode == 0, r.stderr[-300:]
