@@ -4,6 +4,7 @@
 // In C++ and not in Python because an operator's kernels take less time than a Python backward function: of the 110 us that a small loss and its gradient
 // took, 50 are torch's engine and some 50 were Python's.
 #include <ATen/core/grad_mode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -37,7 +38,12 @@ void check(int rc, const char *name) {
 
 // What torch would have to carry on beside the values is refused: no formula of a tangent is here, and a trace would hold the allocations alone
 void values_only(std::initializer_list<const Tensor *> all) {
-    if (torch::jit::tracer::isTracing()) throw std::invalid_argument("the learner operators cannot be traced");
+    typedef c10::impl::TorchDispatchModeTLS Modes;
+    bool traced = torch::jit::tracer::isTracing();
+    if (Modes::any_modes_set())
+        for (auto key : {c10::impl::TorchDispatchModeKey::FAKE, c10::impl::TorchDispatchModeKey::PROXY, c10::impl::TorchDispatchModeKey::FUNCTIONAL})
+            traced = traced || Modes::get_mode(key).has_value();
+    if (traced) throw std::invalid_argument("the learner operators cannot be traced");
     for (const Tensor *x : all)
         if (x->defined() && x->_fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
             throw std::invalid_argument("the learner operators have no forward-mode derivatives: an input has a tangent");

@@ -13,12 +13,13 @@ def inputs():
     x = {k: torch.randn(s, generator=g).cuda() for k, s in {"gate": (6, 3, 4), "update": (6, 3, 4), "state": (3, 4), "rew": (6, 3), "values": (7, 3), "logits": (6, 3, 5), "ref_logits": (6, 3, 5),
                                                             "old": (6, 3), "adv": (6, 3), "ref_logprobs": (6, 3)}.items()}
     x["first"] = torch.zeros((7, 3), dtype=torch.uint8, device="cuda")
+    x["begins"] = x["first"][:-1]
     x["actions"] = torch.zeros((6, 3), dtype=torch.int32, device="cuda")
     return x
 
 
 CALLS = {
-    "recurrence": (lambda x: ops().gated_recurrence(x["gate"], x["update"], x["first"][:-1], x["state"])[0], ["gate", "update", "state"]),
+    "recurrence": (lambda x: ops().gated_recurrence(x["gate"], x["update"], x["begins"], x["state"])[0], ["gate", "update", "state"]),
     "advantages": (lambda x: ops().advantages(x["rew"], x["values"], x["first"], gamma=0.9, lam=0.9)[0], ["rew", "values"]),
     "logprobs": (lambda x: ops().action_logprobs(x["logits"], x["actions"])[0], ["logits"]),
     "loss": (lambda x: ops().policy_loss(x["logits"], x["actions"], x["old"], x["adv"], ref_logits=x["ref_logits"], kl_coef=0.1).loss, ["logits", "old", "adv", "ref_logits"]),
@@ -56,6 +57,19 @@ def test_tracing_is_refused_and_does_not_record_empty_outputs(call):
     name = CALLS[call][1][0]
     with pytest.raises(ValueError, match="traced"):
         torch.jit.trace(lambda v: CALLS[call][0]({**x, name: v}), x[name], check_trace=False)
+    CALLS[call][0](x)
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_symbolic_tracing_is_refused(call):
+    """make_fx records what torch dispatches: the outputs' allocations, and nothing that writes them"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = inputs()
+    name = CALLS[call][1][0]
+    for mode in ("real", "fake"):
+        with pytest.raises(ValueError, match="traced"):
+            make_fx(lambda v: CALLS[call][0]({**x, name: v}), tracing_mode=mode)(x[name])
     CALLS[call][0](x)
 
 
