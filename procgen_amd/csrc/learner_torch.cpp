@@ -98,12 +98,12 @@ procgen_amd_recurrence recurrence(const Tensor &gate, const Tensor &update, cons
 Tensor recurrence_workspace(const Tensor &gate) { return bytes(procgen_amd_recurrence_workspace((int)gate.size(0), (int)gate.size(1), (int)gate.size(2)), gate); }
 
 std::pair<Tensor, Tensor> recurrence_forward(const Tensor &gate, const Tensor &update, const Tensor &first, const Tensor &state, const Tensor &state_out, const Tensor &checkpoints) {
+    if (state_out.defined()) torch::autograd::impl::bump_version(state_out);  // a graph that had saved it must not go on with the new values
     Tensor h = at::empty_like(update), last = state_out.defined() ? state_out : floats({gate.size(1), gate.size(2)}, gate), work = recurrence_workspace(gate);
     procgen_amd_recurrence a = recurrence(gate, update, first, state, checkpoints, work);
     a.h = array3(h);
     a.state_out = data_as<float>(last);
     check(procgen_amd_recurrence_forward(&a, gate.get_device(), stream_of(gate)), "gated_recurrence");
-    if (state_out.defined()) torch::autograd::impl::bump_version(state_out);  // a graph that had saved it must not go on with the new values
     return {h, last};
 }
 

@@ -110,3 +110,14 @@ def test_lazily_negated_gradients_are_taken_as_their_values():
         want = torch.autograd.grad(out, leaves, d)
         got = torch.autograd.grad(run(), leaves, [lazily_negated(v) for v in d])
         assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_a_state_out_that_may_not_be_written_is_left_as_it_was():
+    x = inputs()
+    with torch.inference_mode():
+        out = torch.full((3, 4), 7.0, device="cuda")
+    with torch.no_grad(), pytest.raises(RuntimeError, match="InferenceMode"):
+        ops().gated_recurrence(x["gate"], x["update"], state_out=out)
+    assert (out == 7).all()
+    with torch.inference_mode():
+        assert ops().gated_recurrence(x["gate"], x["update"], state_out=out)[1] is not None and (out != 7).all()
