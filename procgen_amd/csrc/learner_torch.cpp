@@ -65,6 +65,18 @@ variable_list once(variable_list out) {
     return out;
 }
 
+// what else a node keeps for its backward pass: one object, since entries of saved_data of their own are copied list by list
+template <class T>
+T &keep(AutogradContext *ctx, c10::intrusive_ptr<T> x) {
+    T &kept = *x;
+    ctx->saved_data["kept"] = c10::IValue::make_capsule(std::move(x));
+    return kept;
+}
+template <class T>
+T &kept(AutogradContext *ctx) {
+    return static_cast<T &>(*ctx->saved_data["kept"].toCapsule());
+}
+
 // What a backward pass got back of the tensors that were saved.  Hooks (torch.autograd.graph.saved_tensors_hooks) may have kept them elsewhere meanwhile:
 // other strides are taken, anything else would be read as what it is not.
 void came_back(const Tensor &x, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
@@ -107,26 +119,33 @@ std::pair<Tensor, Tensor> recurrence_forward(const Tensor &gate, const Tensor &u
     return {h, last};
 }
 
+struct RecurrenceKept : torch::CustomClassHolder {
+    const std::array<int64_t, 3> shape;
+    const at::ScalarType type, first_type;
+    const at::Device device;
+    RecurrenceKept(const Tensor &gate, const Tensor &first)
+        : shape{gate.size(0), gate.size(1), gate.size(2)}, type(gate.scalar_type()), first_type(first.defined() ? first.scalar_type() : at::kByte), device(gate.device()) {}
+};
+
 struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
     static variable_list forward(AutogradContext *ctx, const Tensor &gate, const Tensor &update, const Maybe &first_, const Maybe &state_) {
         const Tensor first = or_none(first_), state = or_none(state_);
         Tensor checkpoints = floats({procgen_amd_recurrence_checkpoints((int)gate.size(0)), gate.size(1), gate.size(2)}, gate);
         auto [h, last] = recurrence_forward(gate, update, first, state, Tensor(), checkpoints);
         ctx->save_for_backward({gate, update, first, state, checkpoints});
-        ctx->saved_data["shape"] = std::vector<int64_t>{gate.size(0), gate.size(1), gate.size(2), (int64_t)gate.scalar_type(), first.defined() ? (int64_t)first.scalar_type() : 0, gate.get_device()};
+        keep(ctx, c10::make_intrusive<RecurrenceKept>(gate, first));
         ctx->set_materialize_grads(false);
         return {h, last};
     }
     static variable_list backward(AutogradContext *ctx, variable_list d) {
         const variable_list saved = ctx->get_saved_variables();
-        const std::vector<int64_t> s = ctx->saved_data["shape"].toIntVector();
-        const std::array<int64_t, 3> shape{s[0], s[1], s[2]}, checks{procgen_amd_recurrence_checkpoints((int)s[0]), s[1], s[2]};
-        const at::Device device(at::kCUDA, (at::DeviceIndex)s[5]);
+        const RecurrenceKept &k = kept<RecurrenceKept>(ctx);
+        const auto [T, N, D] = k.shape;
         const Tensor &gate = saved[0], &update = saved[1], &first = saved[2];
-        came_back(gate, shape, (at::ScalarType)s[3], device);
-        came_back(update, shape, (at::ScalarType)s[3], device);
-        if (first.defined()) came_back(first, {s[0], s[1]}, (at::ScalarType)s[4], device);
-        const Tensor state = dense(saved[3], {s[1], s[2]}, at::kFloat, device), checkpoints = dense(saved[4], checks, at::kFloat, device);
+        came_back(gate, k.shape, k.type, k.device);
+        came_back(update, k.shape, k.type, k.device);
+        if (first.defined()) came_back(first, {T, N}, k.first_type, k.device);
+        const Tensor state = dense(saved[3], {N, D}, at::kFloat, k.device), checkpoints = dense(saved[4], {procgen_amd_recurrence_checkpoints((int)T), N, D}, at::kFloat, k.device);
         Tensor work = recurrence_workspace(gate), d_h = grad_of(d[0]), d_last = d[1].defined() ? grad_of(d[1]).contiguous() : Tensor();
         Tensor d_gate = ctx->needs_input_grad(0) ? at::empty_like(gate) : Tensor(), d_update = ctx->needs_input_grad(1) ? at::empty_like(update) : Tensor();
         Tensor d_state = state.defined() && ctx->needs_input_grad(first.defined() ? 3 : 2) ? at::empty_like(state) : Tensor();
@@ -181,28 +200,22 @@ procgen_amd_rows rows_of(const Tensor &logits, const Layout &at, const Tensor &a
     a.workspace = data(work);
     return a;
 }
-// what a backward pass needs to know of the logits and actions that were saved
-struct Kind {
-    std::vector<int64_t> sizes;
-    at::ScalarType logits, actions;
-    at::Device device;
-    static void keep(AutogradContext *ctx, const Tensor &logits, const Tensor &actions) {
-        ctx->saved_data["sizes"] = logits.sizes().vec();
-        ctx->saved_data["kind"] = std::vector<int64_t>{(int64_t)logits.scalar_type(), (int64_t)actions.scalar_type(), logits.get_device()};
-    }
-    static Kind kept(AutogradContext *ctx) {
-        const std::vector<int64_t> k = ctx->saved_data["kind"].toIntVector();
-        return {ctx->saved_data["sizes"].toIntVector(), (at::ScalarType)k[0], (at::ScalarType)k[1], at::Device(at::kCUDA, (at::DeviceIndex)k[2])};
-    }
-    at::IntArrayRef rows() const { return at::IntArrayRef(sizes).slice(0, sizes.size() - 1); }
-    Tensor per_row(const Tensor &x, at::ScalarType type) const { return dense(x, rows(), type, device); }
-    // logits, laid out as `at` says or else contiguous
-    Tensor matrix(const Tensor &x, const std::vector<int64_t> &strides, Layout *at) const {
-        came_back(x, sizes, logits, device);
-        if (x.strides() == at::IntArrayRef(strides)) return x;
-        *at = Layout::contiguous(x);
-        return x.contiguous();
-    }
+struct PolicyArgs {
+    Layout at, ref_at;
+    double clip_low, clip_high, kl_coef, entropy_coef;
+};
+struct RowsKept : torch::CustomClassHolder {
+    const at::DimVector sizes, strides;
+    const at::ScalarType type, action_type;
+    const at::Device device;
+    const PolicyArgs p;  // of log-probabilities the first layout alone
+    at::DimVector ref_strides;
+    at::ScalarType valid_type = at::kByte;
+    Tensor work, d_logits;
+    int64_t capture = 0;
+    RowsKept(const Tensor &logits, const Tensor &actions, const PolicyArgs &args)
+        : sizes(logits.sizes()), strides(logits.strides()), type(logits.scalar_type()), action_type(actions.scalar_type()), device(logits.device()), p(args) {}
+    Tensor per_row(const Tensor &x, at::ScalarType t) const { return dense(x, at::IntArrayRef(sizes).slice(0, sizes.size() - 1), t, device); }
 };
 
 void logprobs_forward(const Tensor &logits, const Layout &at, const Tensor &actions, const Tensor &logp, const Tensor &entropy, const Tensor &lse) {
@@ -215,19 +228,18 @@ struct ActionLogprobs : torch::autograd::Function<ActionLogprobs> {
         Tensor logp = floats(actions.sizes(), logits), entropy = floats(actions.sizes(), logits), lse = floats({actions.numel(), 2}, logits);
         logprobs_forward(logits, at, actions, logp, entropy, lse);
         ctx->save_for_backward({logits, actions, lse, entropy});
-        Kind::keep(ctx, logits, actions);
-        ctx->saved_data["strides"] = logits.strides().vec();
-        ctx->saved_data["layout"] = std::vector<int64_t>{at.inner, at.outer_stride, at.inner_stride};
+        keep(ctx, c10::make_intrusive<RowsKept>(logits, actions, PolicyArgs{at, {}, 0, 0, 0, 0}));
         ctx->set_materialize_grads(false);
         return {logp, entropy};
     }
     static variable_list backward(AutogradContext *ctx, variable_list d) {
         const variable_list saved = ctx->get_saved_variables();
-        const std::vector<int64_t> l = ctx->saved_data["layout"].toIntVector();
-        Layout at{l[0], l[1], l[2]};
-        const Kind kind = Kind::kept(ctx);
-        const Tensor logits = kind.matrix(saved[0], ctx->saved_data["strides"].toIntVector(), &at), actions = kind.per_row(saved[1], kind.actions);
-        const Tensor lse = dense(saved[2], {actions.numel(), 2}, at::kFloat, kind.device), entropy = kind.per_row(saved[3], at::kFloat);
+        const RowsKept &k = kept<RowsKept>(ctx);
+        came_back(saved[0], k.sizes, k.type, k.device);
+        const bool moved = saved[0].strides() != at::IntArrayRef(k.strides);
+        const Tensor logits = moved ? saved[0].contiguous() : saved[0], actions = k.per_row(saved[1], k.action_type);
+        const Layout at = moved ? Layout::contiguous(logits) : k.p.at;
+        const Tensor lse = dense(saved[2], {actions.numel(), 2}, at::kFloat, k.device), entropy = k.per_row(saved[3], at::kFloat);
         Tensor d_logits = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
         Tensor d_logp = d[0].defined() ? grad_of(d[0]).contiguous() : Tensor(), d_entropy = d[1].defined() ? grad_of(d[1]).contiguous() : Tensor();
         const procgen_amd_rows a = rows_of(logits, at, actions, d_logits, Tensor());
@@ -251,10 +263,6 @@ std::pair<Tensor, Tensor> action_logprobs(const Tensor &logits, const Tensor &ac
     return {logp, entropy};
 }
 
-struct PolicyArgs {
-    Layout at, ref_at;
-    double clip_low, clip_high, kl_coef, entropy_coef;
-};
 procgen_amd_policy policy_of(const PolicyArgs &p, const Tensor &old, const Tensor &adv, const Tensor &valid, const Tensor &ref_logits, const Tensor &ref_logp) {
     procgen_amd_policy q = {};
     q.old_logprobs = data_as<float>(old), q.adv = data_as<float>(adv), q.valid = data_as<uint8_t>(valid);
@@ -286,42 +294,32 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         Tensor d_logits = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
         const PolicyOut out = policy_forward(p, d_logits, logits, actions, old, adv, valid, ref_logits, ref_logp);
         ctx->save_for_backward({logits, actions, old, adv, valid, ref_logits, ref_logp});
-        ctx->saved_data["strides"] = logits.strides().vec();
-        Kind::keep(ctx, logits, actions);
-        ctx->saved_data["ref_strides"] = ref_logits.defined() ? ref_logits.strides().vec() : std::vector<int64_t>();
-        ctx->saved_data["layout"] = std::vector<int64_t>{p.at.inner, p.at.outer_stride, p.at.inner_stride, p.ref_at.outer_stride, p.ref_at.inner_stride};
-        ctx->saved_data["coefs"] = std::vector<double>{p.clip_low, p.clip_high, p.kl_coef, p.entropy_coef};
-        ctx->saved_data["work"] = out.work;
-        ctx->saved_data["d_logits"] = d_logits;
-        ctx->saved_data["capture"] = (int64_t)procgen_amd_capture_id(stream_of(logits));
+        RowsKept &k = keep(ctx, c10::make_intrusive<RowsKept>(logits, actions, p));
+        if (ref_logits.defined()) k.ref_strides = at::DimVector(ref_logits.strides());
+        if (valid.defined()) k.valid_type = valid.scalar_type();
+        k.work = out.work, k.d_logits = d_logits;
+        k.capture = procgen_amd_capture_id(stream_of(logits));
         ctx->mark_non_differentiable({out.stats});
         return {out.loss, out.stats};
     }
     static variable_list backward(AutogradContext *ctx, variable_list d) {
         const variable_list saved = ctx->get_saved_variables();
-        const std::vector<int64_t> l = ctx->saved_data["layout"].toIntVector();
-        const auto coefs = ctx->saved_data["coefs"].toDoubleVector();
-        PolicyArgs p{{l[0], l[1], l[2]}, {l[0], l[3], l[4]}, coefs[0], coefs[1], coefs[2], coefs[3]};
-        const Kind kind = Kind::kept(ctx);
+        RowsKept &k = kept<RowsKept>(ctx);
+        PolicyArgs p = k.p;
         Tensor logits = saved[0], ref_logits = saved[5];
-        came_back(logits, kind.sizes, kind.logits, kind.device);
-        if (ref_logits.defined()) came_back(ref_logits, kind.sizes, kind.logits, kind.device);
-        const bool moved = logits.strides() != at::IntArrayRef(ctx->saved_data["strides"].toIntVector()) ||
-                           (ref_logits.defined() && ref_logits.strides() != at::IntArrayRef(ctx->saved_data["ref_strides"].toIntVector()));
-        if (moved) {  // the two share one split of their rows
+        came_back(logits, k.sizes, k.type, k.device);
+        if (ref_logits.defined()) came_back(ref_logits, k.sizes, k.type, k.device);
+        if (logits.strides() != at::IntArrayRef(k.strides) || (ref_logits.defined() && ref_logits.strides() != at::IntArrayRef(k.ref_strides))) {  // the two share one split of their rows
             logits = logits.contiguous();
             p.at = Layout::contiguous(logits);
             if (ref_logits.defined()) ref_logits = ref_logits.contiguous(), p.ref_at = Layout::contiguous(ref_logits);
         }
-        const Tensor actions = kind.per_row(saved[1], kind.actions), old = kind.per_row(saved[2], at::kFloat), adv = kind.per_row(saved[3], at::kFloat);
-        const Tensor valid = kind.per_row(saved[4], saved[4].defined() && saved[4].scalar_type() == at::kBool ? at::kBool : at::kByte), ref_logp = kind.per_row(saved[6], at::kFloat);
-        const Tensor work = ctx->saved_data["work"].toTensor(), scale = grad_of(d[0]).contiguous();
-        Tensor d_logits = ctx->saved_data["d_logits"].toTensor();
-        ctx->saved_data["d_logits"] = Tensor();
-        const int64_t capture = ctx->saved_data["capture"].toInt();
-        const bool held = d_logits.defined() && capture >= 0 && capture == procgen_amd_capture_id(stream_of(logits));
+        const Tensor actions = k.per_row(saved[1], k.action_type), old = k.per_row(saved[2], at::kFloat), adv = k.per_row(saved[3], at::kFloat);
+        const Tensor valid = k.per_row(saved[4], k.valid_type), ref_logp = k.per_row(saved[6], at::kFloat), scale = grad_of(d[0]).contiguous();
+        Tensor d_logits = std::move(k.d_logits);
+        const bool held = d_logits.defined() && k.capture >= 0 && k.capture == procgen_amd_capture_id(stream_of(logits));
         if (!held) d_logits = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
-        const procgen_amd_rows a = rows_of(logits, p.at, actions, d_logits, work);
+        const procgen_amd_rows a = rows_of(logits, p.at, actions, d_logits, k.work);
         procgen_amd_policy q = policy_of(p, old, adv, valid, ref_logits, ref_logp);
         q.scale = data_as<float>(scale);
         q.resume = held ? 3 : 1;
