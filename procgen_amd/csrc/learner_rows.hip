@@ -12,8 +12,8 @@
 // the maximum) has e = 0 and counts as 0 whatever it is multiplied with: product() is the hardware's multiplication in which zero times anything is zero.
 // Partial sums of a row are taken against the largest value their lane or wave has seen and rescaled when they meet (Stats::join), so a row is read once.
 //
-// Bound by memory: a column costs 12 operations for 4 to 8 bytes, 23 for 6 to 12 with a reference (a 1 GiB copy reaches 5.1 TB/s on the same card).  By
-// the number of columns:
+// Bound by memory: by the counters a bf16 column costs 12 vector instructions for 2 bytes without a gradient, 22 for 4 with one, 41 for 6 beside a reference,
+// everything about its row included (a 1 GiB copy reaches 5.1 TB/s on the same card).  By the number of columns:
 //   up to 32      a wave takes 64 rows through LDS, a lane per row: no reduction over lanes, coalesced although a row is no multiple of anything
 //                 (16 bits without a reference up to 63)
 //   up to 10240   a group of 4 to 256 lanes per row, the whole row in their registers between the sums and the gradient (5120 in float32; 4096 and 2048
@@ -412,8 +412,8 @@ constexpr int short_residents() {
     return MOST <= 8 ? (REF ? 4 : 6) : MOST <= 16 ? (REF ? (TURN ? 2 : 3) : sizeof(typename E::T) == 4 ? 4 : 5) : MOST <= 24 ? (REF ? 2 : sizeof(typename E::T) == 4 ? 3 : 4) : MOST > 32 || REF || sizeof(typename E::T) == 4 ? 2 : 3;
 }
 
-// Loss and gradient of 4 194 304 x 15 bf16: 67 to 76 us, 306 MB, 4.0 to 4.6 TB/s; without fetching ahead 98, with the register limit of six blocks (and
-// spills) 93, of four 78.  What is left is the issue of instructions: some 360 vector and 190 scalar ones for 64 rows.
+// Loss and gradient of 4 194 304 x 15 bf16: 65 to 74 us, 306 MB, 4.1 to 4.7 TB/s; without fetching ahead 98, with the register limit of six blocks (and
+// spills) 93, of four 78.  What is left is the issue of instructions: some 340 vector and 190 scalar ones for 64 rows.
 template <class E, int MOST, bool REF, class Op, bool TURN, bool APART>
 __global__ __launch_bounds__(BLOCK, (short_residents<E, MOST, REF, TURN>())) void short_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
@@ -560,10 +560,10 @@ struct Place {
 };
 
 // Rows that fit the registers of a group, of lanes inside of a wave or of two or four waves: the next rows are on their way while these are worked on.
-// Loss and gradient of 64 M bf16 logits at 64, 512, 1024, 2000 columns: 68, 55, 55, 57 us (4.2 to 4.9 TB/s), with a reference 91, 81, 81, 87.  Three, four
-// or five chunks a lane leave at most a quarter of the lanes without columns: at 127, 255, 300, 511, 2047 columns 85, 78, 66, 73, 68 us; with four alone, and
-// so up to half of them without, 127, 123, 97, 121, 106.  A group of two or four waves holds 4100, 5000, 8200 columns: 69, 56, 66 us, in batches of a block 113,
-// 90, 77; with a reference 107, 87, 104, in batches 232, 188, 148.
+// Loss and gradient of 64 M bf16 logits at 64, 512, 1024, 2000 columns: 70, 54, 54, 56 us (3.9 to 5.0 TB/s), with a reference 106, 96, 97, 102.  Three, four
+// or five chunks a lane leave at most a quarter of the lanes without columns: at 127, 255, 300, 511, 2047 columns 92, 79, 66, 74, 69 us; with four alone, and
+// so up to half of them without, 127, 123, 97, 121, 106.  A group of two or four waves holds 4100, 5000, 8200 columns: 67, 56, 65 us, in batches of a block 113,
+// 90, 77; with a reference 123, 107, 122, in batches 232, 188, 148.
 template <class E, int G, int CH, bool REF, class Op>
 __global__ __launch_bounds__(BLOCK) void group_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
@@ -678,8 +678,8 @@ __global__ __launch_bounds__(BLOCK) void group_rows(procgen_amd_rows p, Op op, c
 }
 
 // A block per row, in batches of G lanes times CH chunks; the next batch is on its way while one is summed up.
-// Loss and gradient of 2048 x 50021 bf16 with a reference: 154 us for 615 MB, 4.0 TB/s; some 230 MB are read twice, so that memory sees 5.5.  With rows at
-// their own alignment 204, without columns kept in LDS 173.  Log-probabilities of 1000 x 32001: 15 us, 4.3 TB/s.
+// Loss and gradient of 2048 x 50021 bf16 with a reference, a tenth of the rows left out: 154 us for 574 MB, 3.7 TB/s; some 240 MB are read twice, so that memory sees 5.3.  With rows at
+// their own alignment 204, without columns kept in LDS 173.  Log-probabilities of 1000 x 32001: 16 us, 4.0 TB/s.
 template <class E, int G, int CH, bool REF, class Op>
 __global__ __launch_bounds__(G, 4) void long_rows(procgen_amd_rows p, Op op, const void *ref, long long ref_outer, long long ref_inner, double *partial) {
     typedef typename E::T T;
@@ -816,7 +816,8 @@ __global__ __launch_bounds__(G, 4) void long_rows(procgen_amd_rows p, Op op, con
     if (partial) put_sums(sums, op, partial);
 }
 
-// The gradient of long rows' log-probabilities: the largest value, the log of the sum and the entropy are known, so every column stands for itself.  1000 x 32001 bf16: 24 us, 5.3 TB/s.
+// The gradient of long rows' log-probabilities: the largest value, the log of the sum and the entropy are known, so every column stands for itself.
+// 1000 x 32001 bf16: 25 us, 5.1 TB/s.
 template <class E>
 __global__ __launch_bounds__(BLOCK) void logprobs_gradient(procgen_amd_rows p, const procgen_amd_lse *lse, const float *entropy, const float *d_logp, const float *d_entropy) {
     typedef typename E::T T;

@@ -619,8 +619,9 @@ int vec_for(const procgen_amd_recurrence *a, bool backward) {
         if (a->D >= vec && (long long)a->N * ((a->D + vec - 1) / vec) >= FULL * (long long)WAVE) return vec;
     return 1;
 }
-// fn(VEC, WAVES): a window in segments has too few chains for more than one a lane.  With one a lane eight waves: 1024 x 64 x 512 bf16 forward 53 us,
-// backward 109, with four 66 and 126
+// fn(VEC, WAVES): a window in segments has few chains, and goes with one a lane: float32 32768 x 512 forward 57 us, backward 91, 4096 x 16 x 256 55 and 88, with two
+// 57 and 98, 58 and 98.  (Of 16 bits two a lane with twice the segments would take less: bf16 53 : 42 and 80 : 61, 49 : 36 and 73 : 54.)  With one a lane eight waves:
+// 1024 x 64 x 512 bf16 forward 53 us, backward 109, with four 66 and 126
 template <int MOST, class Fn>
 int by_shape(const Segments &g, int vec, Fn fn) {
     typedef std::integral_constant<int, 1> One;

@@ -284,7 +284,9 @@ def policy_loss(logits, actions, old_logprobs, advantages, *, clip=0.2, kl_coef=
     loss = mean over the valid rows of -objective + kl_coef * KL - entropy_coef * entropy.
 
     KL is KL(p | q) over all columns with q = softmax(ref_logits), or its estimator exp(d) - d - 1 with d = ref_logprobs - logp from the reference's
-    log-probability of the action taken; at most one of the two is given, and the term is 0 without.  clip: a number, or (below, above).  logits as for
+    log-probability of the action taken; at most one of the two is given, and the term is 0 without.  With kl_coef = 0 a reference is only watched: it
+    changes stats, and nothing else whatever it holds.  Where ref_logits excludes what the policy allows KL is infinite, or about as large as the numbers
+    that exclude it (infinite, too, where their sum passes float32's range).  clip: a number, or (below, above).  logits as for
     action_logprobs; actions, old_logprobs, advantages, valid (uint8 or bool, None: all), ref_logprobs: [...]; ref_logits like logits.  Rows that are
     not valid are not looked at, whatever they hold, and get a zero gradient; without a valid row the loss is 0.  A valid row without any finite
     column counts, with nothing to add.  Only the logits get a gradient, once."""
