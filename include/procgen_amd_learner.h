@@ -30,7 +30,7 @@ struct procgen_amd_array3 {
 /* Gated linear recurrence along t, every (n, d) a chain of its own:
  *     h[t] = keep[t] * gate[t] * h[t-1] + update[t],   keep[t] = (first[t][n] == 0),   h[-1] = state (zeros when NULL)
  * Where first is set the old state and the gate are not looked at, whatever they hold.  Products of neighbouring gates are formed on the way: where one
- * passes float's range, h behind it is not finite.
+ * passes float's range, h behind it is not finite unless h before it is zero (or first is set in between); gradients alike, from the last step to the first.
  * state, state_out: float [N][D], contiguous; state_out may be state (updated in place), or NULL.  checkpoints: NULL, or float
  * [procgen_amd_recurrence_checkpoints(T)][N][D], which the backward pass reads (it does not read state).  workspace: memory of
  * procgen_amd_recurrence_workspace(T, N, D) bytes (NULL when that is 0). */

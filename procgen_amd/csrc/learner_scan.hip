@@ -16,6 +16,7 @@
 #include "learner.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace pgamd {
 namespace learner {
@@ -42,15 +43,26 @@ struct Map {
         cut = false;
         for (int v = 0; v < VEC; v++) A[v] = 1.f, B[v] = 0.f;
     }
-    __device__ float at(float x, int v) const { return cut ? B[v] : fmaf(A[v], x, B[v]); }
+    // FAR: A may have passed float's range, which no step of it has: zero times it is zero
+    template <bool FAR>
+    __device__ float at(float x, int v) const {
+        return cut || (FAR && x == 0.f) ? B[v] : fmaf(A[v], x, B[v]);
+    }
     __device__ void then(const Map &m) {  // this map first, m behind it
         for (int v = 0; v < VEC; v++) {
-            B[v] = m.at(B[v], v);
+            B[v] = m.template at<true>(B[v], v);
             A[v] = A[v] * m.A[v];
         }
         cut = cut || m.cut;
     }
 };
+
+template <int VEC>
+__device__ inline bool any_nan(const float (&x)[VEC], const float (&y)[VEC], const float (&z)[VEC]) {  // in any lane of the wave
+    bool any = false;
+    for (int v = 0; v < VEC; v++) any = any || __builtin_isunordered(x[v], y[v]) || __builtin_isunordered(x[v], z[v]);
+    return __builtin_expect(__any(any), 0);
+}
 
 // the pieces' maps of a tile, by wave and lane
 template <int VEC, int WAVES>
@@ -128,7 +140,7 @@ __device__ inline void run_segments(float *x, const Segments &g, int from, int t
     __syncthreads();
     for (int k = 0; k < W; k++) {
         const Map<VEC> q = pieces.get(k, lane);
-        for (int v = 0; v < VEC; v++) x[v] = q.at(x[v], v);
+        for (int v = 0; v < VEC; v++) x[v] = q.template at<true>(x[v], v);
     }
     __syncthreads();
 }
@@ -292,14 +304,21 @@ __global__ __launch_bounds__(WAVES *WAVE) void recurrence_forward(procgen_amd_re
         if (t0 + TILE < end) load(t + TILE);  // the next tile is on its way while this one is joined
         pieces[odd].put(w, lane, compose<VEC, false, K>(a, b, cut));
         __syncthreads();
-        float y[VEC];
-        for (int v = 0; v < VEC; v++) y[v] = x[v];
-        for (int k = 0; k < W; k++) {
-            const Map<VEC> q = pieces[odd].get(k, lane);
-            for (int v = 0; v < VEC; v++) {
-                if (k == w) y[v] = x[v];
-                x[v] = q.at(x[v], v);
+        float y[VEC], start[VEC];
+        for (int v = 0; v < VEC; v++) start[v] = y[v] = x[v];
+        auto join = [&](auto far) {
+            for (int k = 0; k < W; k++) {
+                const Map<VEC> q = pieces[odd].get(k, lane);
+                for (int v = 0; v < VEC; v++) {
+                    if (k == w) y[v] = x[v];
+                    x[v] = q.template at<decltype(far)::value>(x[v], v);
+                }
             }
+        };
+        join(std::false_type());
+        if (any_nan(x, y, y)) {  // it may be an infinite product times zero: once more, with a question at every piece, which at once would cost up to a tenth of the time
+            for (int v = 0; v < VEC; v++) x[v] = y[v] = start[v];
+            join(std::true_type());
         }
         if (p.checkpoints && w * K % CHECK == 0 && t < end) store_state<VEC>(p.checkpoints + (long long)(t / CHECK) * chains, y, ch);
 #pragma unroll
@@ -355,15 +374,25 @@ __global__ __launch_bounds__(WAVES *WAVE) void recurrence_backward(procgen_amd_r
         fore[odd].put(w, lane, compose<VEC, false, K>(a, b, cut));
         back[odd].put(w, lane, compose<VEC, true, K>(a, d, cut));
         __syncthreads();
-        for (int v = 0; v < VEC; v++) before[v] = x[v], behind[v] = y[v];
-        for (int k = 0; k < W; k++) {
-            const Map<VEC> f = fore[odd].get(k, lane), q = back[odd].get(W - 1 - k, lane);
-            for (int v = 0; v < VEC; v++) {
-                if (k == w) before[v] = x[v];
-                x[v] = f.at(x[v], v);
-                if (W - 1 - k == w) behind[v] = y[v];
-                y[v] = q.at(y[v], v);
+        float first_x[VEC], first_y[VEC];
+        for (int v = 0; v < VEC; v++) before[v] = first_x[v] = x[v], behind[v] = first_y[v] = y[v];
+        auto join = [&](auto far) {
+            constexpr bool FAR = decltype(far)::value;
+#pragma clang loop unroll_count(FAR ? 1 : 4)
+            for (int k = 0; k < W; k++) {
+                const Map<VEC> f = fore[odd].get(k, lane), q = back[odd].get(W - 1 - k, lane);
+                for (int v = 0; v < VEC; v++) {
+                    if (k == w) before[v] = x[v];
+                    x[v] = f.template at<FAR>(x[v], v);
+                    if (W - 1 - k == w) behind[v] = y[v];
+                    y[v] = q.template at<FAR>(y[v], v);
+                }
             }
+        };
+        join(std::false_type());
+        if (any_nan(y, before, behind)) {
+            for (int v = 0; v < VEC; v++) before[v] = x[v] = first_x[v], behind[v] = y[v] = first_y[v];
+            join(std::true_type());
         }
 #pragma unroll
         for (int k = 0; k < K; k++)  // b becomes the value before the step
@@ -560,7 +589,7 @@ __global__ __launch_bounds__(WAVES *WAVE) void advantages(procgen_amd_advantage 
         float adv = y;
         for (int k = W - 1; k >= 0; k--) {
             if (k == w) adv = y;
-            y = pieces[odd].get(k, lane).at(y, 0);
+            y = pieces[odd].get(k, lane).template at<false>(y, 0);  // gamma lam is one at the most
         }
 #pragma unroll
         for (int k = K - 1; k >= 0; k--) {

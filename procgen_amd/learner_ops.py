@@ -136,7 +136,8 @@ def gated_recurrence(gate, update, first=None, state=None, state_out=None):
     gradients.  Differentiable in gate, update and state, once.
 
     Products of neighbouring gates are formed on the way (of 8 steps, and of up to the whole window where there are few chains): where such a product
-    passes float32's range -- gates larger than one over a long stretch -- h behind it is not finite, even if it began at zero."""
+    passes float32's range -- gates larger than one over a long stretch -- h behind it is not finite, unless h before it is zero or an episode begins in
+    between; gradients alike, from the last step to the first."""
     _tensor(gate, "gate", _FLOATS)
     shape = gate.shape
     if len(shape) not in (2, 3):
